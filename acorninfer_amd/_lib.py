@@ -75,6 +75,18 @@ _SIGNATURES = {
     "acorn_sample_workspace": [_i64, _i64, _vp],
     "acorn_sample_split": [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                            _i64, _vp],
+    "acorn_kv8_scatter": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                          _i64, _i64, _i64, _i32, _vp],
+    "acorn_kv8_gather": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                         _i64, _i64, _i64, _i64, _i32, _vp],
+    "acorn_qkv_epilogue_kv8": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                               _i64, _i64, _vp, _vp, _f32, _vp, _vp, _i32, _vp],
+    "acorn_paged_attention_kv8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                  _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp],
+    "acorn_paged_prefill_attention_kv8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32,
+                                          _vp, _i64, _vp],
+    "acorn_paged_prefill_workspace_kv8": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
     "acorn_kv_scatter": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32,
                          _vp],
 }

@@ -1,0 +1,787 @@
+// Attention over the 8-bit paged KV cache (format and layout: kv8.h):
+//   acorn_paged_attention_kv8          one new token per sequence, split over
+//                                      the cache's length and joined
+//   acorn_paged_prefill_attention_kv8  packed prompt rows, causal
+// Both turn bytes into bf16 / fp16 (exactly) and use the 16-bit MFMAs with fp32
+// sums. The fp8 MFMAs would take the bytes as they lie, with q in two or three
+// e4m3 terms, but add their products to fewer bits: measured against 64 bits
+// 1.6e-5 of the sum of magnitudes for normal numbers, 2.8e-4 where one in
+// sixteen is a hundred times larger, 2e-8 with the bf16 MFMA.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_common.h"
+#include "kv8.h"
+
+using namespace acorn;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Decode. A workgroup of NWV waves serves one (split, kv head, sequence); its
+// waves divide the split's groups of 16 tokens. Per step of two groups, with
+// lane = 16 r + c:
+//  * S^T = K q^T on v_mfma_f32_16x16x32: A = K (row = token c), from the tile's
+//    pieces as they are loaded, 8 conversions of two bytes per MFMA pair; a
+//    token's scale goes into its conversions. B = q^T (column = head c; columns
+//    past REP repeat the last head). Register i of lane (r, c) then holds the
+//    score of head c for token 4 r + i.
+//  * online softmax in that layout, the maximum moved only by scores that
+//    exceed it by more than kMaxSlack; p rounded to T and l the sum of the
+//    rounded values, so that the weights of the mean add up to 1.
+//  * O^T += V^T P^T on v_mfma_f32_16x16x32: B = the p of lane (r, c) as they
+//    stand (tokens 4 r .. 4 r + 3 of both groups); A = V^T, from the E dims of
+//    those tokens that the lane has loaded and converted, transposed by v_perm.
+// The wave's block ids are fetched two steps ahead of their tiles, DEPTH steps
+// of tiles are in flight. Loads are unconditional (wait counts stay static):
+// those past the wave's last group read one line of it.
+template <typename T, int D, int REP, int NWV, int DEPTH>
+__global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
+    const T* __restrict__ q, const uint8_t* __restrict__ k_tiles,
+    const uint8_t* __restrict__ v_tiles, const uint8_t* __restrict__ scales,
+    const int32_t* __restrict__ tables, const int32_t* __restrict__ lens, T* __restrict__ out,
+    float* __restrict__ ws_acc, float* __restrict__ ws_m, float* __restrict__ ws_l, int H, int KV,
+    int P, int num_blocks, int table_stride, int S, float scale_log2) {
+  constexpr int E = D / 16;                    // dims per lane of V = MFMAs per P V
+  constexpr int KP = D / 64;                   // 16-byte pieces per lane and tile, K or V
+  constexpr int KB = D / 32;                   // q.k MFMAs per group
+  __shared__ __align__(16) float sacc[NWV == 1 ? 1 : NWV][REP][D];
+  __shared__ float sm[NWV][REP], sl[NWV][REP];
+
+  const int kvh = blockIdx.x, sp = blockIdx.y, b = blockIdx.z;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int r = lane >> 4, c = lane & 15;
+  const int gshift = __builtin_ctz(P) - 4;     // groups per block, as a shift
+
+  const int L = min(max(lens[b], 0), table_stride * P);
+  const int groups = (L + kKv8Group - 1) / kKv8Group;
+  const int npages = (L + P - 1) / P;
+  const int pps = (table_stride + S - 1) / S;                 // pages per split
+  const int nsb = max(1, (npages + pps - 1) / pps);           // splits this sequence uses
+  if (sp >= nsb) return;                                      // uniform over the workgroup
+  const int wg0 = (sp * pps) << gshift, wg1 = min(wg0 + (pps << gshift), groups);
+  // this wave's groups, in pairs
+  const int per = ((wg1 - wg0 + NWV - 1) / NWV + 1) & ~1;
+  const int g0 = min(wg0 + wid * per, wg1), g1 = min(g0 + per, wg1);
+  const int glast = max(g1 - 1, 0);
+  const int32_t* trow = tables + (size_t)b * table_stride;
+
+  u32x4_t qb[KB];
+  const T* qp = q + ((size_t)b * H + kvh * REP + min(c, REP - 1)) * D;
+#pragma unroll
+  for (int j = 0; j < KB; ++j)
+    qb[j] = *(const u32x4_t*)(qp + 64 * (j / 2) + 16 * r + 8 * (j % 2));
+
+  auto block_of = [&](int g) -> size_t {       // of group g, clamped to the wave's last and the pool
+    const unsigned pg = (unsigned)trow[min(min(g, glast) >> gshift, table_stride - 1)];
+    return pg < (unsigned)num_blocks ? pg : 0u;
+  };
+  struct Step {
+    u32x4_t k[2][KP], v[2][KP];
+    uint32_t ks[2], vs[2];
+  };
+  auto load = [&](int g, const size_t (&blk)[2], Step& s) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int gc = min(g + u, glast);
+      const size_t tile = ((blk[u] * KV + kvh) << gshift) + (gc & ((1 << gshift) - 1));
+      const uint32_t off = g + u <= glast ? lane * 16 : 0;
+      const uint8_t* kb = k_tiles + tile * (16 * D);
+      const uint8_t* vb = v_tiles + tile * (16 * D);
+      const uint8_t* sb = scales + tile * 32;
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        s.k[u][i] = load_nt((const u32x4_t*)(kb + off + 1024 * i));
+        s.v[u][i] = load_nt((const u32x4_t*)(vb + off + 1024 * i));
+      }
+      s.ks[u] = sb[c];
+      s.vs[u] = *(const uint32_t*)(sb + 16 + 4 * r);
+    }
+  };
+  float m = -INFINITY, l = 0.f;
+  f32x4_t acc[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto consume = [&](int g, Step& s) {
+    f32x4_t sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      const float f = kv8_scale(s.ks[u]);
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+        sc[u] = mfma16x16x32<T>(kv8_cvt8<T>(s.k[u][j / 2][2 * (j % 2)], s.k[u][j / 2][2 * (j % 2) + 1], f),
+                                qb[j], sc[u]);
+    }
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * u + i] = sc[u][i] * scale_log2;
+    if (kKv8Group * (g + 2) > L || g + 2 > g1) {
+      // tokens past the sequence, or past the wave's groups: no weight, and V bytes and
+      // codes of 0 (a block may hold anything there)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (g + u >= g1 || kKv8Group * (g + u) + 4 * r + i >= L) {
+            x[4 * u + i] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < E / 4; ++w) {
+              const int at = E / 4 * i + w;
+              s.v[u][at / 4][at % 4] = 0u;
+            }
+            s.vs[u] &= ~(0xFFu << (8 * i));
+          }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+    if (__builtin_amdgcn_ballot_w64(mx > m + kMaxSlack) != 0) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < E; ++j) acc[j] *= alpha;
+    }
+    u32x4_t pb;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pb[i] = pack_dot<T>(__builtin_amdgcn_exp2f(x[2 * i] - m), __builtin_amdgcn_exp2f(x[2 * i + 1] - m), l);
+    // V: token i of group u, E dims in E / 2 words
+    uint32_t vt[2][4][E / 2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float f[4] = {kv8_scale_of<0>(s.vs[u]), kv8_scale_of<1>(s.vs[u]),
+                          kv8_scale_of<2>(s.vs[u]), kv8_scale_of<3>(s.vs[u])};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < E / 4; ++w) {
+          const int at = E / 4 * i + w;
+          vt[u][i][2 * w] = kv8_cvt2<T, false>(s.v[u][at / 4][at % 4], f[i]);
+          vt[u][i][2 * w + 1] = kv8_cvt2<T, true>(s.v[u][at / 4][at % 4], f[i]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+      const u32x4_t va = {__builtin_amdgcn_perm(vt[0][1][j / 2], vt[0][0][j / 2], sel),
+                          __builtin_amdgcn_perm(vt[0][3][j / 2], vt[0][2][j / 2], sel),
+                          __builtin_amdgcn_perm(vt[1][1][j / 2], vt[1][0][j / 2], sel),
+                          __builtin_amdgcn_perm(vt[1][3][j / 2], vt[1][2][j / 2], sel)};
+      acc[j] = mfma16x16x32<T>(va, pb, acc[j]);
+    }
+  };
+
+  if (g0 < g1) {
+    Step st[DEPTH];
+    size_t blk[2];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      blk[0] = block_of(g0 + 2 * i);
+      blk[1] = block_of(g0 + 2 * i + 1);
+      load(g0 + 2 * i, blk, st[i]);
+    }
+    blk[0] = block_of(g0 + 2 * DEPTH);
+    blk[1] = block_of(g0 + 2 * DEPTH + 1);
+    bool more = true;
+    for (int g = g0; more; g += 2 * DEPTH) {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        if (more) {
+          const int gi = g + 2 * i;
+          consume(gi, st[i]);
+          load(gi + 2 * DEPTH, blk, st[i]);
+          blk[0] = block_of(gi + 2 * DEPTH + 2);
+          blk[1] = block_of(gi + 2 * DEPTH + 3);
+          more = gi + 2 < g1;
+        }
+      }
+    }
+  }
+  // l: each lane summed its own tokens; add the four lane rows of a head
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  // register i of accumulator j of lane (r, c) holds dim E (4 r + i) + j of head c
+  if constexpr (NWV == 1) {
+    if (c < REP) {
+      const size_t orow = (size_t)b * H + kvh * REP + c;
+      if (nsb == 1) {
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[E / 2];
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j)
+            w[j] = pack2<T>(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+          __builtin_memcpy(__builtin_assume_aligned(out + orow * D + E * (4 * r + i), 2 * E), w, sizeof(w));
+        }
+      } else {
+        const size_t slot = orow * S + sp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[E];
+#pragma unroll
+          for (int j = 0; j < E; ++j) f[j] = acc[j][i];
+          __builtin_memcpy(__builtin_assume_aligned(ws_acc + slot * D + E * (4 * r + i), 16), f, sizeof(f));
+        }
+        if (r == 0) {
+          ws_m[slot] = m;
+          ws_l[slot] = l;
+        }
+      }
+    }
+    return;
+  }
+  if (c < REP) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = acc[j][i];
+      __builtin_memcpy(__builtin_assume_aligned(&sacc[wid][c][E * (4 * r + i)], 16), f, sizeof(f));
+    }
+    if (r == 0) {
+      sm[wid][c] = m;
+      sl[wid][c] = l;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < REP * D; e += NWV * kWave) {
+    const int h = e / D, d = e % D;
+    // (a wave that saw a NaN score keeps m of its other scores and has l and acc NaN)
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NWV; ++w) M = fmaxf(M, sm[w][h]);
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < NWV; ++w) {
+      // a wave without tokens has l = acc = 0
+      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][h] - M);
+      num += f * sacc[w][h][d];
+      den += f * sl[w][h];
+    }
+    const size_t orow = (size_t)b * H + kvh * REP + h;
+    if (nsb == 1) {
+      out[orow * D + d] = from_f32<T>(num / den);
+    } else {
+      const size_t slot = orow * S + sp;
+      ws_acc[slot * D + d] = num;
+      if (d == 0) {
+        ws_m[slot] = M;
+        ws_l[slot] = den;
+      }
+    }
+  }
+}
+
+struct DecodeArgs {
+  const void *q, *kt, *vt, *sc;
+  const int32_t *tables, *lens;
+  void* out;
+  float *ws_acc, *ws_ml;
+  int64_t B, H, KV, P, num_blocks, table_stride, S;
+  float scale;
+  hipStream_t st;
+};
+
+// Splits of at most this many groups of 16 tokens run as one wave, longer ones
+// as eight.
+constexpr int64_t kOneWaveGroups = 16;
+constexpr int kWaves = 8;
+
+template <typename T, int D, int REP>
+int launch_decode(const DecodeArgs& a) {
+  const int64_t pps = (a.table_stride + a.S - 1) / a.S;
+  const bool one = a.S > 1 && pps * (a.P / kKv8Group) <= kOneWaveGroups;
+  float* ws_m = a.ws_ml;
+  float* ws_l = a.ws_ml ? a.ws_ml + a.B * a.H * a.S : nullptr;
+  auto kfn = one ? kv8_decode_kernel<T, D, REP, 1, 2> : kv8_decode_kernel<T, D, REP, kWaves, 2>;
+  kfn<<<dim3((unsigned)a.KV, (unsigned)a.S, (unsigned)a.B), dim3((one ? 1 : kWaves) * kWave), 0, a.st>>>(
+      (const T*)a.q, (const uint8_t*)a.kt, (const uint8_t*)a.vt, (const uint8_t*)a.sc, a.tables,
+      a.lens, (T*)a.out, a.ws_acc, ws_m, ws_l, (int)a.H, (int)a.KV, (int)a.P, (int)a.num_blocks,
+      (int)a.table_stride, (int)a.S, a.scale * kLog2e);
+  ACORN_LAUNCH_CHECK();
+  if (a.S > 1) {
+    paged_attn_combine_kernel<T, D, false>
+        <<<dim3((unsigned)(a.B * a.H)), dim3(kCombineWaves * kWave), 0, a.st>>>(
+            a.ws_acc, ws_m, ws_l, (T*)a.out, a.lens, (int)a.H, (int)a.P, (int)a.table_stride,
+            (int)a.S);
+    ACORN_LAUNCH_CHECK();
+  }
+  return ACORN_OK;
+}
+
+template <typename T, int D>
+int decode_rep(const DecodeArgs& a) {
+  switch (a.H / a.KV) {
+    case 1: return launch_decode<T, D, 1>(a);
+    case 2: return launch_decode<T, D, 2>(a);
+    case 4: return launch_decode<T, D, 4>(a);
+    case 8: return launch_decode<T, D, 8>(a);
+  }
+  return ACORN_ERR_UNSUPPORTED;
+}
+
+// ---------------------------------------------------------------------------
+// Prefill: the query-tiled kernel of the 16-bit cache (paged_attention.hip) over
+// 8-bit tiles. A workgroup serves the REP q heads of a kv head for WQ query
+// tokens, wave (head, group) QW blocks of 16; the keys are walked in chunks of
+// 64, which the workgroup turns into 16 bits once, on their way into LDS:
+// per chunk and thread (4 waves, D = 128) two 16-byte pieces of K and two of V,
+// 32 conversions against some 290 other VALU instructions, and half the loads
+// of a 16-bit cache. Per 32 keys and query block: S^T = K Q^T, the online
+// softmax per query column, O^T += V^T P^T with V^T from LDS by
+// ds_read_b64_tr_b16, the P V MFMAs one step behind the scores'. Masked scores
+// are set to -inf whatever they are, and V bytes are finite, so a row that holds
+// NaN reaches only the queries that see it; past the last key bytes are taken as 0.
+// SPLIT, WIN, the partials and their merge: as there.
+template <typename T, int D, int REP, int QG, int KC, int QW, bool SPLIT, bool WIN>
+__global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
+    const T* __restrict__ q, const uint8_t* __restrict__ k_tiles,
+    const uint8_t* __restrict__ v_tiles, const uint8_t* __restrict__ scales,
+    const int32_t* __restrict__ tables, const int32_t* __restrict__ seq_row0,
+    const int32_t* __restrict__ seq_pos0, const int32_t* __restrict__ seq_nq, T* __restrict__ out,
+    int R, int H, int KV, int P, int num_blocks, int table_stride, float scale_log2, int max_nq,
+    int S, int cps, float* __restrict__ ws, int cap) {
+  constexpr int NT = REP * QG * kWave;           // threads
+  constexpr int KB = D / 32, DPL = D / 16;
+  constexpr int PITCH = 2 * D + 32;              // bytes per staged row (padded against LDS conflicts)
+  constexpr int WQ = QG * QW * 16;               // query rows per workgroup
+  constexpr int TC = KC / kKv8Group;             // tiles per chunk, K or V
+  constexpr int PCS = TC * D;                    // 16-byte pieces per chunk, K or V
+  constexpr int PPT = 2 * PCS / NT;              // pieces per thread per chunk
+  static_assert(2 * PCS % NT == 0 && D % kWave == 0, "whole pieces per thread, one tile per wave");
+  __shared__ __align__(16) uint8_t kvs[2][2 * KC * PITCH];       // [buffer][K rows | V rows]
+  const int kvh = blockIdx.y, n = blockIdx.z;
+  const int tid = threadIdx.x;
+  const int wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const int r = lane >> 4, c = lane & 15;
+  const int hq = wid % REP, sub = wid / REP;
+  const int h = kvh * REP + hq;
+  const PrefillSeq sq = prefill_seq<WIN>(seq_row0, seq_pos0, seq_nq, n, R, max_nq, cap);
+  // (rows placed past their table row's pages are not served)
+  const int pos0 = sq.pos0, row0 = sq.row0, nq = WIN ? sq.nq : min(sq.nq, cap - pos0);
+  const int tile_q = SPLIT ? (gridDim.x - 1 - blockIdx.x) / S : gridDim.x - 1 - blockIdx.x;
+  const int wg_j0 = tile_q * WQ;                                // longest tiles first
+  if (wg_j0 >= nq) return;                                      // uniform over the workgroup
+  const int j0 = wg_j0 + sub * QW * 16;                         // this wave's first query row
+  const int nvalid = max(0, min(QW * 16, nq - j0));             // 0: the wave only stages
+  const int L = pos0 + min(wg_j0 + WQ, nq);                     // keys of the workgroup's last query
+  const int total = (L + KC - 1) / KC;
+  const int sp = SPLIT ? (gridDim.x - 1 - blockIdx.x) % S : 0;
+  const int cb = SPLIT ? sp * cps : 0;
+  const int nchunks = SPLIT ? min(cb + cps, total) : total;
+  if (cb >= nchunks) {                           // uniform over the workgroup
+    // a window's tile before its sequence's first token sees no key
+    if (WIN && total <= 0 && sp == 0) {
+#pragma unroll
+      for (int qw = 0; qw < QW; ++qw)
+        if (16 * qw + c < nvalid) {
+          T* o = out + ((size_t)(row0 + j0 + 16 * qw + c) * H + h) * D + 4 * r;
+#pragma unroll
+          for (int jj = 0; jj < DPL; ++jj)
+            *(u32x2_t*)(o + 16 * jj) = u32x2_t{pack2<T>(NAN, NAN), pack2<T>(NAN, NAN)};
+        }
+    }
+    return;
+  }
+  const int32_t* trow = tables + (size_t)n * table_stride;
+  const int gshift = __builtin_ctz(P) - 4;
+  const int glast = (L - 1) / kKv8Group;
+
+  // the queries: block qw's column c is query row j0 + 16 qw + c (clamped)
+  u32x4_t qb[QW][KB];
+  int pc[QW];
+#pragma unroll
+  for (int qw = 0; qw < QW; ++qw) {
+    const int jc = min(16 * qw + c, max(nvalid - 1, 0));
+    pc[qw] = pos0 + j0 + jc;
+    const size_t qrow = (size_t)(row0 + min(j0 + jc, nq - 1));
+#pragma unroll
+    for (int jb = 0; jb < KB; ++jb)
+      qb[qw][jb] = *(const u32x4_t*)(q + (qrow * H + h) * D + 32 * jb + 8 * r);
+  }
+
+  // Staging. Piece x = i NT + tid of a chunk: K's for x < PCS, V's from there; piece
+  // x % D of tile x / D. K: dims 16 (x % D / 16) .. of token x % 16. V: the E dims of
+  // 16 / E tokens (kv8.h). A wave's pieces are of one kind and one tile (D and PCS are
+  // multiples of 64), so the block ids are scalar loads.
+  constexpr int E = D / 16, TP = 16 / E;
+  u32x4_t stage[PPT];
+  uint32_t code[PPT];
+  auto of_k = [&](int i) {                       // the wave's i-th pieces are K's (uniform)
+    return (i + 1) * NT <= PCS || (i * NT < PCS && i * NT + wid * kWave < PCS);
+  };
+  auto tile_at = [&](int chunk, int i) -> size_t {
+    const int x = i * NT + wid * kWave;
+    const int g = min(chunk * TC + (x % PCS) / D, glast);
+    const unsigned pg = (unsigned)trow[min(g >> gshift, table_stride - 1)];
+    const size_t blk = pg < (unsigned)num_blocks ? pg : 0u;
+    return ((blk * KV + kvh) << gshift) + (g & ((1 << gshift) - 1));
+  };
+  auto load_chunk = [&](const size_t (&tl)[PPT]) {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) {
+      const int x0 = i * NT + wid * kWave;       // the wave's first piece
+      const int p = x0 % D + lane;               // piece of the tile
+      const uint8_t* src = (of_k(i) ? k_tiles : v_tiles) + tl[i] * (16 * D);
+      const uint8_t* sb = scales + tl[i] * 32;
+      stage[i] = *(const u32x4_t*)(src + p * 16);
+      if (of_k(i)) {
+        code[i] = sb[p % 16];
+      } else if constexpr (TP == 2) {
+        code[i] = *(const uint16_t*)(sb + 16 + 4 * (p % 64 / 16) + 2 * (p / 64));
+      } else {
+        code[i] = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
+      }
+    }
+  };
+  auto store_chunk = [&](int bf, int chunk) {
+    const bool tail = chunk * KC + KC > L;       // uniform
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) {
+      const int x0 = i * NT + wid * kWave;
+      const int p = x0 % D + lane;
+      const int t0 = (x0 % PCS) / D * kKv8Group;   // the tile's first row of the chunk
+      if (of_k(i)) {
+        const float f = kv8_scale(code[i]);
+        uint8_t* dst = kvs[bf] + (t0 + p % 16) * PITCH + p / 16 * 32;
+        *(u32x4_t*)dst = kv8_cvt8<T>(stage[i][0], stage[i][1], f);
+        *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(stage[i][2], stage[i][3], f);
+      } else {
+        const int t = t0 + 4 * (p % 64 / 16) + TP * (p / 64);
+        uint8_t* dst = kvs[bf] + KC * PITCH + t * PITCH + p % 16 * (2 * E);
+#pragma unroll
+        for (int j = 0; j < TP; ++j) {
+          const float f = kv8_scale_finite(code[i] >> (8 * j) & 0xFFu);
+          const bool off = tail && chunk * KC + t + j >= L;
+          if constexpr (TP == 2) {
+            *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(off ? 0u : stage[i][2 * j], off ? 0u : stage[i][2 * j + 1], f);
+          } else {
+            const uint32_t w = off ? 0u : stage[i][j];
+            *(u32x2_t*)(dst + j * PITCH) = u32x2_t{kv8_cvt2<T, false>(w, f), kv8_cvt2<T, true>(w, f)};
+          }
+        }
+      }
+    }
+  };
+
+  float m[QW], l[QW], nm[QW];                    // nm: -m (0 while m is -inf)
+  f32x4_t acc[QW][DPL];
+#pragma unroll
+  for (int qw = 0; qw < QW; ++qw) {
+    m[qw] = -INFINITY;
+    l[qw] = nm[qw] = 0.f;
+#pragma unroll
+    for (int jj = 0; jj < DPL; ++jj) acc[qw][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t vlane = (uint32_t)((4 * r + (c >> 2)) * PITCH + 8 * (c & 3));
+  u32x4_t va[DPL], pb[QW];
+#pragma unroll
+  for (int jj = 0; jj < DPL; ++jj) va[jj] = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int qw = 0; qw < QW; ++qw) pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
+  const int tlast = pos0 + j0 + min(16 * QW, nvalid) - 1;   // the wave's last query
+  auto pv = [&]() {
+#pragma unroll
+    for (int jj = 0; jj < DPL; ++jj)
+#pragma unroll
+      for (int qw = 0; qw < QW; ++qw) acc[qw][jj] = mfma16x16x32<T>(va[jj], pb[qw], acc[qw][jj]);
+  };
+  auto step = [&](int bf, int s32, int t0) {
+    if (t0 > tlast) return;                      // keys after every query of the wave
+    const uint8_t* kbuf = kvs[bf] + 32 * s32 * PITCH;
+    const uint8_t* vbuf = kvs[bf] + KC * PITCH + 32 * s32 * PITCH;
+    u32x4_t kf[2][KB];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int jb = 0; jb < KB; ++jb)
+        kf[hh][jb] = *(const u32x4_t*)(kbuf + (16 * hh + c) * PITCH + 2 * (32 * jb + 8 * r));
+    f32x4_t sc[QW][2];
+    bool live[QW];
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) {
+      // the block's queries all precede these keys, or it has none: nothing to add
+      live[qw] = 16 * qw < nvalid && t0 <= pos0 + j0 + min(16 * qw + 15, nvalid - 1);
+      sc[qw][0] = sc[qw][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int jb = 0; jb < KB; ++jb)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int qw = 0; qw < QW; ++qw)
+          sc[qw][hh] = mfma16x16x32<T>(kf[hh][jb], qb[qw][jb], sc[qw][hh]);
+    pv();
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) {
+      if (!live[qw]) {
+        pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
+        continue;
+      }
+      float sv[8];                               // raw scores; scaled inside the exp2
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sv[4 * hh + i] = sc[qw][hh][i];
+      if (t0 + 31 > pos0 + j0 + 16 * qw) {       // the keys cross some column's diagonal
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t0 + 16 * hh + 4 * r + i > pc[qw]) sv[4 * hh + i] = -INFINITY;
+      }
+      float mx = sv[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sv[i]);
+      mx *= scale_log2;                          // scale_log2 > 0
+      if (__builtin_amdgcn_ballot_w64(mx > m[qw] + kMaxSlack) != 0) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m[qw], mx);
+        // (a query that has seen no key yet keeps -inf: alpha 0, p = exp2(-inf))
+        nm[qw] = mn == -INFINITY ? 0.f : -mn;
+        const float alpha = __builtin_amdgcn_exp2f(m[qw] + nm[qw]);
+        m[qw] = mn;
+        l[qw] *= alpha;
+#pragma unroll
+        for (int jj = 0; jj < DPL; ++jj) acc[qw][jj] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i], scale_log2, nm[qw]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i + 1], scale_log2, nm[qw]));
+        pb[qw][i] = pack_dot<T>(p0, p1, l[qw]);
+      }
+    }
+    typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+    const __attribute__((address_space(3))) uint8_t* vl =
+        (const __attribute__((address_space(3))) uint8_t*)vbuf + vlane;
+#pragma unroll
+    for (int jj = 0; jj < DPL; ++jj) {
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + 32 * jj));
+      const s16x4_t hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + 16 * PITCH + 32 * jj));
+      const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+      va[jj] = u32x4_t{l2[0], l2[1], h2[0], h2[1]};
+    }
+  };
+
+  // prologue: chunk 0 staged, chunk 1's loads in flight
+  size_t tl[PPT];
+  auto tiles_of = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) tl[i] = tile_at(min(chunk, nchunks - 1), i);
+  };
+  tiles_of(cb);
+  load_chunk(tl);
+  tiles_of(cb + 1);
+  store_chunk(0, cb);
+  load_chunk(tl);
+  __syncthreads();
+  for (int ci = cb; ci < nchunks; ++ci) {
+    const int bf = (ci - cb) & 1;
+    tiles_of(ci + 2);                            // two chunks ahead
+    __builtin_amdgcn_sched_barrier(0);
+    if (nvalid > 0) {
+#pragma unroll
+      for (int s32 = 0; s32 < KC / 32; ++s32) step(bf, s32, ci * KC + 32 * s32);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    store_chunk(bf ^ 1, min(ci + 1, nchunks - 1));   // its buffer was last read in ci - 1
+    __builtin_amdgcn_sched_barrier(0);
+    load_chunk(tl);
+    __syncthreads();
+  }
+  if (nvalid == 0) return;
+  pv();
+  if (SPLIT && total > cps) {                    // one run of several: its fp32 partial
+    const size_t slots = (size_t)prefill_slots(gridDim.z, R, max_nq) * H;
+    float2* ml = (float2*)(ws + (size_t)S * slots * D);
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) {
+      float lt = l[qw];
+      lt += __shfl_xor(lt, 16);
+      lt += __shfl_xor(lt, 32);
+      if (16 * qw + c < nvalid) {
+        const size_t slot = (size_t)sp * slots +
+                            (size_t)prefill_slot(gridDim.z, R, max_nq, n, row0, j0 + 16 * qw + c) * H + h;
+#pragma unroll
+        for (int jj = 0; jj < DPL; ++jj)
+          *(f32x4_t*)(ws + slot * D + 16 * jj + 4 * r) = acc[qw][jj];
+        if (r == 0) ml[slot] = make_float2(m[qw], lt);
+      }
+    }
+    return;
+  }
+  // lane (r, c) of block qw holds dims 16 jj + 4 r + i of query column 16 qw + c
+#pragma unroll
+  for (int qw = 0; qw < QW; ++qw) {
+    float lt = l[qw];
+    lt += __shfl_xor(lt, 16);
+    lt += __shfl_xor(lt, 32);
+    if (16 * qw + c < nvalid) {
+      const size_t orow = (size_t)(row0 + j0 + 16 * qw + c) * H + h;
+      const float inv = 1.0f / lt;
+#pragma unroll
+      for (int jj = 0; jj < DPL; ++jj) {
+        const u32x2_t w = {pack2<T>(acc[qw][jj][0] * inv, acc[qw][jj][1] * inv),
+                           pack2<T>(acc[qw][jj][2] * inv, acc[qw][jj][3] * inv)};
+        *(u32x2_t*)(out + orow * D + 16 * jj + 4 * r) = w;
+      }
+    }
+  }
+}
+
+struct PrefillArgs {
+  const void *q, *kt, *vt, *sc;
+  const int32_t *tables, *row0, *pos0, *nq;
+  void* out;
+  int64_t N, R, max_nq, H, KV, P, num_blocks, table_stride;
+  float scale;
+  PrefillPlan plan;
+  float* ws;
+  hipStream_t st;
+};
+
+template <typename T, int D, int REP, int QW, bool SPLIT, bool WIN>
+int launch_prefill(const PrefillArgs& a) {
+  constexpr int QG = REP >= 4 ? 1 : 4 / REP;
+  constexpr int WQ = 16 * QW * QG;
+  const int64_t tiles = (a.max_nq + WQ - 1) / WQ;
+  const int S = SPLIT ? a.plan.S : 1;
+  const int cap = (int)std::min<int64_t>(a.table_stride * a.P, 0x7fffffff);
+  kv8_prefill_kernel<T, D, REP, QG, kPrefillChunk, QW, SPLIT, WIN>
+      <<<dim3((unsigned)(tiles * S), (unsigned)a.KV, (unsigned)a.N), dim3(REP * QG * kWave), 0,
+         a.st>>>((const T*)a.q, (const uint8_t*)a.kt, (const uint8_t*)a.vt, (const uint8_t*)a.sc,
+                 a.tables, a.row0, a.pos0, a.nq, (T*)a.out, (int)a.R, (int)a.H, (int)a.KV,
+                 (int)a.P, (int)a.num_blocks, (int)a.table_stride, a.scale * kLog2e,
+                 (int)a.max_nq, S, a.plan.cps, a.ws, cap);
+  ACORN_LAUNCH_CHECK();
+  if (SPLIT) {
+    constexpr int pairs = kPrefillCombineNT / (D / 4);
+    paged_prefill_combine_kernel<T, D, WIN, !WIN>
+        <<<dim3((unsigned)((a.max_nq * a.H + pairs - 1) / pairs), (unsigned)a.N),
+           dim3(kPrefillCombineNT), 0, a.st>>>(a.ws, a.row0, a.pos0, a.nq, (T*)a.out, (int)a.R,
+                                               (int)a.H, (int)a.max_nq, S, a.plan.cps, WQ, cap);
+    ACORN_LAUNCH_CHECK();
+  }
+  return ACORN_OK;
+}
+
+template <typename T, int D, int REP, bool WIN>
+int prefill_form(const PrefillArgs& a) {
+  if (a.plan.S > 1)
+    return a.plan.qw == 1 ? launch_prefill<T, D, REP, 1, true, WIN>(a)
+                          : launch_prefill<T, D, REP, 2, true, WIN>(a);
+  return a.plan.qw == 1 ? launch_prefill<T, D, REP, 1, false, WIN>(a)
+                        : launch_prefill<T, D, REP, 2, false, WIN>(a);
+}
+
+template <typename T, int D>
+int prefill_rep(const PrefillArgs& a) {
+  switch (a.H / a.KV) {
+#define ACORN_REP(n) \
+  case n: return a.nq ? prefill_form<T, D, n, false>(a) : prefill_form<T, D, n, true>(a);
+    ACORN_REP(1)
+    ACORN_REP(2)
+    ACORN_REP(4)
+    ACORN_REP(8)
+#undef ACORN_REP
+  }
+  return ACORN_ERR_UNSUPPORTED;
+}
+
+int attn_shape(int64_t N, int64_t H, int64_t KV, int64_t D, int64_t P, int64_t num_blocks,
+               int64_t table_stride) {
+  if (N < 0 || N > 65535 || H <= 0 || KV <= 0 || KV > 65535 || H % KV != 0 || D <= 0 || P <= 0 ||
+      num_blocks <= 0 || num_blocks > 0x7fffffff || table_stride < 1)
+    return ACORN_ERR_SHAPE;
+  if ((P & (P - 1)) != 0 || P % kKv8Group != 0 || P > 65536 || table_stride > 0x7fffffff / P - 1)
+    return ACORN_ERR_SHAPE;
+  const int64_t rep = H / KV;
+  if ((D != 64 && D != 128) || !(rep == 1 || rep == 2 || rep == 4 || rep == 8))
+    return ACORN_ERR_UNSUPPORTED;
+  return ACORN_OK;
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" int acorn_paged_attention_kv8(const void* q, const void* k_tiles, const void* v_tiles,
+                                         const void* scales, const int32_t* tables,
+                                         const int32_t* seq_lens, void* out, float* ws_acc,
+                                         float* ws_ml, int64_t B, int64_t H, int64_t KV, int64_t D,
+                                         int64_t P, int64_t num_blocks, int64_t table_stride,
+                                         int64_t num_splits, float scale, int dtype,
+                                         void* stream) {
+  const int rc = attn_shape(B, H, KV, D, P, num_blocks, table_stride);
+  if (rc != ACORN_OK) return rc;
+  if (num_splits < 1 || num_splits > 65535) return ACORN_ERR_SHAPE;
+  if (B == 0) return ACORN_OK;
+  if (!q || !k_tiles || !v_tiles || !scales || !tables || !seq_lens || !out) return ACORN_ERR_VALUE;
+  if (num_splits > 1 && (!ws_acc || !ws_ml)) return ACORN_ERR_VALUE;
+  if (!aligned16({q, k_tiles, v_tiles, scales, out, ws_acc})) return ACORN_ERR_VALUE;
+  const DecodeArgs a{q,  k_tiles, v_tiles, scales, tables,       seq_lens,   out,   ws_acc, ws_ml,
+                     B,  H,       KV,      P,      num_blocks,   table_stride, num_splits, scale,
+                     (hipStream_t)stream};
+  switch (dtype) {
+    case ACORN_F16: return D == 64 ? decode_rep<_Float16, 64>(a) : decode_rep<_Float16, 128>(a);
+    case ACORN_BF16: return D == 64 ? decode_rep<__bf16, 64>(a) : decode_rep<__bf16, 128>(a);
+  }
+  return ACORN_ERR_DTYPE;
+}
+
+extern "C" int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t max_nq, int64_t H,
+                                                 int64_t KV, int64_t D, int64_t P,
+                                                 int64_t table_stride, int64_t* bytes) {
+  const int rc = attn_shape(N, H, KV, D, P, 1, table_stride);
+  if (rc != ACORN_OK) return rc;
+  if (R < 0 || max_nq < 0 || R > 0x7fffffff || max_nq > 0x7fffffff) return ACORN_ERR_SHAPE;
+  if (!bytes) return ACORN_ERR_VALUE;
+  *bytes = N == 0 || R == 0 || max_nq == 0
+               ? 0
+               : prefill_plan(N, R, max_nq, H, KV, D, P, table_stride).ws_bytes;
+  return ACORN_OK;
+}
+
+extern "C" int acorn_paged_prefill_attention_kv8(
+    const void* q, const void* k_tiles, const void* v_tiles, const void* scales,
+    const int32_t* tables, const int32_t* seq_row0, const int32_t* seq_pos0,
+    const int32_t* seq_nq, void* out, int64_t N, int64_t R, int64_t max_nq, int64_t H, int64_t KV,
+    int64_t D, int64_t P, int64_t num_blocks, int64_t table_stride, float scale, int dtype,
+    void* ws, int64_t ws_bytes, void* stream) {
+  const int rc = attn_shape(N, H, KV, D, P, num_blocks, table_stride);
+  if (rc != ACORN_OK) return rc;
+  if (R < 0 || max_nq < 0 || R > 0x7fffffff || max_nq > 0x7fffffff) return ACORN_ERR_SHAPE;
+  if (N == 0 || R == 0 || max_nq == 0) return ACORN_OK;
+  if (!q || !k_tiles || !v_tiles || !scales || !tables || !seq_pos0 || !out || !seq_row0 != !seq_nq)
+    return ACORN_ERR_VALUE;
+  if (!seq_nq && R != N * max_nq) return ACORN_ERR_SHAPE;
+  if (!aligned16({q, k_tiles, v_tiles, scales, out, ws})) return ACORN_ERR_VALUE;
+  PrefillArgs a{q, k_tiles, v_tiles, scales, tables, seq_row0, seq_pos0, seq_nq, out, N, R, max_nq,
+                H, KV, P, num_blocks, table_stride, scale,
+                prefill_plan(N, R, max_nq, H, KV, D, P, table_stride), (float*)ws,
+                (hipStream_t)stream};
+  if (!ws || ws_bytes < a.plan.ws_bytes) a.plan.S = 1;   // nothing is split
+  switch (dtype) {
+    case ACORN_F16: return D == 64 ? prefill_rep<_Float16, 64>(a) : prefill_rep<_Float16, 128>(a);
+    case ACORN_BF16: return D == 64 ? prefill_rep<__bf16, 64>(a) : prefill_rep<__bf16, 128>(a);
+  }
+  return ACORN_ERR_DTYPE;
+}

@@ -454,6 +454,89 @@ int acorn_sample_split(const void* logits, int64_t rows, int64_t vocab, int dtyp
 /* *bytes = workspace of acorn_sample_split (0: none is used). No GPU access. */
 int acorn_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes);
 
+/*
+ * The 8-bit paged KV cache. A layer's cache is three byte arrays over the pool's
+ * blocks of P tokens (P a power of two, a multiple of 16), in groups of 16 tokens:
+ *   k_tiles, v_tiles [num_blocks, KV, P/16, 16*D] and scales [num_blocks, KV, P/16, 32],
+ * 16-byte aligned, D in {64, 128}. Byte b of token t (of the group), dim d, stands for
+ * e4m3(b) * 2^(code - 127), code the token's: scales byte t for k, 16 + t for v, the
+ * least (1 or more) with which the row's largest magnitude is at most 448 * 2^(code-127).
+ *   k: b at (d/16)*256 + t*16 + d%16
+ *   v, E = D/16, TP = 16/E: b at (t%4/TP)*1024 + (16*(t/4) + d/E)*16 + (t%TP)*E + d%E
+ * A (token, kv head) whose k or v row holds an infinity or NaN is held as NaN (codes
+ * 255, bytes 0). Memory of zeros is an empty cache. fp16 magnitudes above 63456 are
+ * held as 61440, so that what is read is an fp16; a cache written from another type is
+ * read in fp16 only where its values fit. No counterpart in the reference.
+ *
+ * acorn_kv8_scatter: rows k, v of `dtype` (any), row i, head h at k + i*k_row_stride +
+ * h*k_head_stride (elements; each D/16 values aligned to their size or 16 bytes), are
+ * written at (pages[i], slots[i]); a target outside the pool is skipped. Two rows with
+ * one target leave it undefined.
+ */
+int acorn_kv8_scatter(const void* k, const void* v, void* k_tiles, void* v_tiles, void* scales,
+                      const int64_t* pages, const int64_t* slots, int64_t rows, int64_t kv_heads,
+                      int64_t head_dim, int64_t page_size, int64_t num_blocks,
+                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                      int64_t v_head_stride, int dtype, void* stream);
+
+/*
+ * The 8-bit cache read back: tokens seq_pos0[n] + j, j < seq_nq[n], of sequence n
+ * (tables [N, table_stride] int32) as rows seq_row0[n] + j of k_out, v_out [R, KV, D] of
+ * `dtype` (any), rounded once. max_nq >= every seq_nq[n]. Rows that no sequence covers,
+ * rows past R or past the table row's pages are not written.
+ */
+int acorn_kv8_gather(const void* k_tiles, const void* v_tiles, const void* scales,
+                     const int32_t* tables, const int32_t* seq_row0, const int32_t* seq_pos0,
+                     const int32_t* seq_nq, void* k_out, void* v_out, int64_t N, int64_t R,
+                     int64_t max_nq, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                     int64_t num_blocks, int64_t table_stride, int dtype, void* stream);
+
+/*
+ * acorn_qkv_epilogue for the 8-bit cache: `nsplit` fp32 planes part[s, batch,
+ * (H + 2*KV)*D], added in order (nsplit == 0: one plane of `dtype`), give q_out
+ * [batch, H, D] (per-head RMSNorm and RoPE, rounded to `dtype` once) and k (the same)
+ * and v, quantised at (pages[b], slots[b]) from their 32-bit values; the angles are
+ * positions * inv_freq without that product's rounding. q_w, k_w [D] of `dtype`
+ * (fp16 / bf16); part, q_out, q_w, k_w 16-byte aligned.
+ */
+int acorn_qkv_epilogue_kv8(const void* part, int64_t nsplit, void* q_out, void* k_tiles,
+                           void* v_tiles, void* scales, const int64_t* pages,
+                           const int64_t* slots, int64_t batch, int64_t q_heads,
+                           int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                           int64_t num_blocks, const void* q_w, const void* k_w, float eps,
+                           const int64_t* positions, const float* inv_freq, int dtype,
+                           void* stream);
+
+/*
+ * acorn_paged_attention over the 8-bit cache: q, out [B, H, D] fp16 / bf16, D in
+ * {64, 128}, H/KV in {1, 2, 4, 8}. num_splits > 1: page-aligned splits of
+ * ceil(table_stride / num_splits) pages, whose fp32 partials ws_acc [B*H*num_splits*D],
+ * ws_ml [2*B*H*num_splits] a second launch joins. A length is taken as at most the
+ * tokens its table row has pages for; a row that sees no token is NaN.
+ */
+int acorn_paged_attention_kv8(const void* q, const void* k_tiles, const void* v_tiles,
+                              const void* scales, const int32_t* tables, const int32_t* seq_lens,
+                              void* out, float* ws_acc, float* ws_ml, int64_t B, int64_t H,
+                              int64_t KV, int64_t D, int64_t P, int64_t num_blocks,
+                              int64_t table_stride, int64_t num_splits, float scale, int dtype,
+                              void* stream);
+
+/*
+ * acorn_paged_prefill_attention_ws over the 8-bit cache (windows included: seq_row0 and
+ * seq_nq both NULL). Rows at positions past their table row's pages are not written.
+ * ws: at least the bytes acorn_paged_prefill_workspace_kv8 reports, or nothing is split.
+ */
+int acorn_paged_prefill_attention_kv8(const void* q, const void* k_tiles, const void* v_tiles,
+                                      const void* scales, const int32_t* tables,
+                                      const int32_t* seq_row0, const int32_t* seq_pos0,
+                                      const int32_t* seq_nq, void* out, int64_t N, int64_t R,
+                                      int64_t max_nq, int64_t H, int64_t KV, int64_t D, int64_t P,
+                                      int64_t num_blocks, int64_t table_stride, float scale,
+                                      int dtype, void* ws, int64_t ws_bytes, void* stream);
+/* *bytes = workspace of acorn_paged_prefill_attention_kv8 (0: none). No GPU access. */
+int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t max_nq, int64_t H, int64_t KV,
+                                      int64_t D, int64_t P, int64_t table_stride, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,9 @@ from typing import NamedTuple
 
 import torch
 
-from acorninfer_amd._lib import check, dtype_code, lib, ptr, require_gpu, stream_ptr
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
+
+from acorninfer_amd._lib import check, dtype_code, lib, ptr, require_gpu
 
 GROUP = 16               # tokens of a tile
 MI355X_CUS = 256
@@ -81,59 +83,85 @@ def kv8_pages(num_blocks: int, kv_heads: int, head_dim: int, page_size: int, dev
                       for n in (GROUP * head_dim, GROUP * head_dim, 2 * GROUP)))
 
 
-def _check_pages(kv: KV8Pages) -> None:
+# The checks of a call take a few microseconds on the host, as long as a small launch takes on
+# the GPU: they look at each tensor once and at nothing that a tensor property does not hold.
+def _pool(kv: KV8Pages) -> tuple[int, int, int, int]:
+    """(num_blocks, kv_heads, head_dim, page_size) of pages that are as they should be."""
     k, v, s = kv
-    assert k.dim() == 4 and k.shape == v.shape and k.shape[3] % GROUP == 0, \
+    shape = k.shape
+    assert len(shape) == 4 and shape == v.shape and shape[3] % GROUP == 0, \
         "tiles are [num_blocks, KV, P // 16, 16 * D]"
-    assert s.shape == (*k.shape[:3], 2 * GROUP), "scales are [num_blocks, KV, P // 16, 32]"
-    for t in kv:
-        assert t.dtype == torch.uint8 and t.is_contiguous(), "pages are contiguous uint8"
+    NB, KV, G, n = shape
+    assert s.shape == (NB, KV, G, 2 * GROUP), "scales are [num_blocks, KV, P // 16, 32]"
+    assert k.dtype is v.dtype is s.dtype is torch.uint8 and k.is_contiguous() and \
+        v.is_contiguous() and s.is_contiguous(), "pages are contiguous uint8"
+    return NB, KV, n // GROUP, G * GROUP
 
 
-def _on(device: torch.device, *tensors) -> None:
-    """Kernels launch on one device's stream and reach every tensor by its pointer."""
-    require_gpu(*tensors)
+def _device(first: torch.Tensor, *tensors: torch.Tensor) -> int:
+    """The index of the one GPU that holds the tensors: a kernel launches on one device's stream
+    and reaches every tensor by its pointer."""
+    dev = first.get_device()
     for t in tensors:
-        assert t is None or t.device == device, f"tensors on {t.device} and {device}"
+        if t.get_device() != dev:
+            require_gpu(first, *tensors)
+            raise AssertionError(f"tensors on {first.device} and {t.device}")
+    if dev < 0:
+        require_gpu(first)
+    return dev
+
+
+def _call(name: str, dev: int, *args) -> None:
+    """Launch on the current stream of device `dev`, with that device current."""
+    fn = getattr(lib(), "acorn_" + name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        check(rc, name)
 
 
 def _check_targets(pages: torch.Tensor, slots: torch.Tensor, rows: int) -> None:
     for t in (pages, slots):
-        assert t.shape == (rows,) and t.dtype == torch.int64 and t.is_contiguous(), \
+        assert t.dtype is torch.int64 and t.shape == (rows,) and t.is_contiguous(), \
             "pages and slots are contiguous int64, one per row"
 
 
-def _check_tables(kv: KV8Pages, N: int, tables: torch.Tensor, *meta: torch.Tensor) -> int:
+def _check_tables(N: int, tables: torch.Tensor, *meta: torch.Tensor) -> int:
     """Block tables and per-sequence metadata; the table's width (1 for an empty batch)."""
-    assert tables.dim() == 2 and tables.shape[0] == N
     for t in meta:
-        assert t.shape == (N,)
-    for t in (tables, *meta):
-        assert t.dtype == torch.int32 and t.is_contiguous(), "tables and metadata are int32"
-    assert N == 0 or tables.shape[1] >= 1, "tables must hold at least one page per sequence"
-    return max(1, tables.shape[1])
+        assert t.dtype is torch.int32 and t.shape == (N,) and t.is_contiguous(), \
+            "lengths and metadata are contiguous int32, one per sequence"
+    assert tables.dtype is torch.int32 and tables.dim() == 2 and tables.is_contiguous(), \
+        "tables are contiguous int32 [N, pages]"
+    n, W = tables.shape
+    assert n == N and (W >= 1 or N == 0), "tables must hold at least one page per sequence"
+    return max(1, W)
 
 
-def _check_out(out: torch.Tensor, shape: tuple, dtype: torch.dtype, device) -> None:
+def _check_out(out: torch.Tensor, shape: tuple, dtype: torch.dtype, dev: int) -> None:
     assert tuple(out.shape) == tuple(shape), f"out must be {tuple(shape)}, not {tuple(out.shape)}"
     assert out.dtype == dtype, f"out dtype {out.dtype} != {dtype}"
-    assert out.device == device and out.is_contiguous(), "out must be contiguous on the inputs' device"
+    assert out.get_device() == dev and out.is_contiguous() and out.data_ptr() % 16 == 0, \
+        "out must be contiguous on the inputs' device, from a 16-byte boundary"
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [R, KV, D] as the kernel reads it: dims side by side, each lane's D / 16 values aligned."""
     size = x.element_size()
     step = min(16, x.shape[2] // 16 * size)
-    if x.stride(2) != 1 or x.data_ptr() % step or any(x.stride(i) * size % step for i in (0, 1)):
-        x = x.contiguous()
-        if x.data_ptr() % step:
-            x = x.clone()
+    rs, hs, ds = x.stride()
+    if ds != 1 or x.data_ptr() % step or rs * size % step or hs * size % step:
+        return x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
     """x contiguous from a 16-byte boundary (a view into a tensor may start anywhere)."""
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x.clone() if x.data_ptr() % 16 else x
 
 
@@ -142,22 +170,18 @@ def kv8_scatter(k: torch.Tensor, v: torch.Tensor, kv: KV8Pages, pages: torch.Ten
     """Quantise rows k, v [R, KV, D] (fp32 / fp16 / bf16, any strides) into the cache at
     (pages[i], slots[i]) (int64). A target outside the pool is skipped, as in
     PagedKVCache.scatter_decode; two rows with one target leave it undefined."""
-    _check_pages(kv)
-    dev = kv.k.device
-    _on(dev, *kv, k, v, pages, slots)
-    assert k.dim() == 3 and k.shape == v.shape and k.shape[1:] == (kv.kv_heads, kv.head_dim), \
-        f"k is {tuple(k.shape)}, v {tuple(v.shape)}; the pool holds {kv.kv_heads} kv heads of " \
-        f"{kv.head_dim}"
-    assert k.dtype == v.dtype
+    NB, KV, D, P = _pool(kv)
+    dev = _device(kv.k, kv.v, kv.scales, k, v, pages, slots)
     R = k.shape[0]
+    assert k.shape == v.shape == (R, KV, D), \
+        f"k is {tuple(k.shape)}, v {tuple(v.shape)}; the pool holds {KV} kv heads of {D}"
+    assert k.dtype is v.dtype
     _check_targets(pages, slots, R)
     k, v = _rows(k), _rows(v)
-    with torch.cuda.device(dev):
-        rc = lib().acorn_kv8_scatter(
-            ptr(k), ptr(v), *map(ptr, kv), ptr(pages), ptr(slots), R, kv.kv_heads, kv.head_dim,
-            kv.page_size, kv.num_blocks, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            dtype_code(k), stream_ptr(dev))
-    check(rc, "kv8_scatter")
+    (ks, kh, _), (vs, vh, _) = k.stride(), v.stride()
+    _call("kv8_scatter", dev, k.data_ptr(), v.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(),
+          kv.scales.data_ptr(), pages.data_ptr(), slots.data_ptr(), R, KV, D, P, NB, ks, kh, vs, vh,
+          dtype_code(k))
 
 
 def kv8_gather(kv: KV8Pages, tables: torch.Tensor, seq_row0: torch.Tensor, seq_pos0: torch.Tensor,
@@ -168,22 +192,21 @@ def kv8_gather(kv: KV8Pages, tables: torch.Tensor, seq_row0: torch.Tensor, seq_p
     """The cache read back: k, v [rows, KV, D] of `dtype`, where row seq_row0[n] + j holds token
     seq_pos0[n] + j (j < seq_nq[n] <= max_nq) of the sequence with block table tables[n]. Rows
     that no sequence covers, or past their table row's pages, are not written."""
-    _check_pages(kv)
-    dev = kv.k.device
-    _on(dev, *kv, tables, seq_row0, seq_pos0, seq_nq)
-    W = _check_tables(kv, seq_row0.shape[0], tables, seq_row0, seq_pos0, seq_nq)
-    shape = (int(rows), kv.kv_heads, kv.head_dim)
-    assert int(rows) >= 0 and int(max_nq) >= 0
+    NB, KV, D, P = _pool(kv)
+    dev = _device(kv.k, kv.v, kv.scales, tables, seq_row0, seq_pos0, seq_nq)
+    N = seq_row0.shape[0]
+    W = _check_tables(N, tables, seq_row0, seq_pos0, seq_nq)
+    R, max_nq = int(rows), int(max_nq)
+    assert R >= 0 and max_nq >= 0
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
-    for o in out:
-        _check_out(o, shape, dtype, dev)
-    with torch.cuda.device(dev):
-        rc = lib().acorn_kv8_gather(
-            *map(ptr, kv), ptr(tables), ptr(seq_row0), ptr(seq_pos0), ptr(seq_nq), ptr(out[0]),
-            ptr(out[1]), seq_row0.shape[0], int(rows), int(max_nq), kv.kv_heads, kv.head_dim,
-            kv.page_size, kv.num_blocks, W, dtype_code(out[0]), stream_ptr(dev))
-    check(rc, "kv8_gather")
+        k = torch.empty((R, KV, D), dtype=dtype, device=kv.k.device)
+        out = (k, torch.empty_like(k))
+    else:
+        for o in out:
+            _check_out(o, (R, KV, D), dtype, dev)
+    _call("kv8_gather", dev, kv.k.data_ptr(), kv.v.data_ptr(), kv.scales.data_ptr(),
+          tables.data_ptr(), seq_row0.data_ptr(), seq_pos0.data_ptr(), seq_nq.data_ptr(),
+          out[0].data_ptr(), out[1].data_ptr(), N, R, max_nq, KV, D, P, NB, W, dtype_code(out[0]))
     return out
 
 
@@ -196,32 +219,31 @@ def qkv_norm_rope_kv8(qkv: torch.Tensor, kv: KV8Pages, pages: torch.Tensor, slot
     [R, H, D] (per-head RMSNorm with q_weight [D], RoPE at positions [R] int64 with inv_freq
     [D / 2] fp32) in q_weight's dtype; k (the same with k_weight) and v are quantised into the
     cache at (pages[i], slots[i]), straight from their 32-bit values."""
-    _check_pages(kv)
-    dev = kv.k.device
-    _on(dev, *kv, qkv, pages, slots, positions, inv_freq, q_weight, k_weight)
-    H, KV, D = int(q_heads), kv.kv_heads, kv.head_dim
+    NB, KV, D, P = _pool(kv)
+    dev = _device(kv.k, kv.v, kv.scales, qkv, pages, slots, positions, inv_freq, q_weight, k_weight)
+    H = int(q_heads)
     dtype = q_weight.dtype
-    assert qkv.dim() in (2, 3) and qkv.shape[-1] == (H + 2 * KV) * D and H >= 1, \
+    shape = qkv.shape
+    assert len(shape) in (2, 3) and shape[-1] == (H + 2 * KV) * D and H >= 1, \
         f"qkv rows hold {(H + 2 * KV) * D} values"
-    assert qkv.dtype == (torch.float32 if qkv.dim() == 3 else dtype), \
+    planes = shape[0] if len(shape) == 3 else 0
+    assert qkv.dtype is (torch.float32 if len(shape) == 3 else dtype), \
         "qkv is [S, R, width] fp32 or [R, width] of the weights' dtype"
-    planes = qkv.shape[0] if qkv.dim() == 3 else 0
-    assert qkv.dim() == 2 or planes >= 1
-    R = qkv.shape[-2]
+    assert len(shape) == 2 or planes >= 1
+    R = shape[-2]
     _check_targets(pages, slots, R)
-    assert positions.shape == (R,) and positions.dtype == torch.int64 and positions.is_contiguous()
-    assert inv_freq.shape == (D // 2,) and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
-    assert q_weight.shape == k_weight.shape == (D,) and k_weight.dtype == dtype
+    assert positions.shape == (R,) and positions.dtype is torch.int64 and positions.is_contiguous()
+    assert inv_freq.shape == (D // 2,) and inv_freq.dtype is torch.float32 and inv_freq.is_contiguous()
+    assert q_weight.shape == k_weight.shape == (D,) and k_weight.dtype is dtype
     qkv, qw, kw = _aligned(qkv), _aligned(q_weight), _aligned(k_weight)
     if out is None:
-        out = torch.empty((R, H, D), dtype=dtype, device=dev)
-    _check_out(out, (R, H, D), dtype, dev)
-    with torch.cuda.device(dev):
-        rc = lib().acorn_qkv_epilogue_kv8(
-            ptr(qkv), planes, ptr(out), *map(ptr, kv), ptr(pages), ptr(slots), R, H, KV, D,
-            kv.page_size, kv.num_blocks, ptr(qw), ptr(kw), float(eps), ptr(positions),
-            ptr(inv_freq), dtype_code(out), stream_ptr(dev))
-    check(rc, "qkv_norm_rope_kv8")
+        out = torch.empty((R, H, D), dtype=dtype, device=qkv.device)
+    else:
+        _check_out(out, (R, H, D), dtype, dev)
+    _call("qkv_epilogue_kv8", dev, qkv.data_ptr(), planes, out.data_ptr(), kv.k.data_ptr(),
+          kv.v.data_ptr(), kv.scales.data_ptr(), pages.data_ptr(), slots.data_ptr(), R, H, KV, D, P,
+          NB, qw.data_ptr(), kw.data_ptr(), float(eps), positions.data_ptr(), inv_freq.data_ptr(),
+          dtype_code(out))
     return out
 
 
@@ -242,17 +264,15 @@ def kv8_workspace(batch: int, num_heads: int, head_dim: int, num_splits: int, de
     if num_splits <= 1:
         return None
     n = batch * num_heads * num_splits
-    return (torch.empty(n * head_dim, dtype=torch.float32, device=device),
-            torch.empty(2 * n, dtype=torch.float32, device=device))
+    both = torch.empty(n * (head_dim + 2), dtype=torch.float32, device=device)
+    return both[:n * head_dim], both[n * head_dim:]
 
 
-def _check_attention(q: torch.Tensor, kv: KV8Pages) -> None:
-    assert q.shape[-1] == kv.head_dim and q.shape[-2] % kv.kv_heads == 0, \
-        f"q heads {tuple(q.shape[-2:])} over {kv.kv_heads} kv heads of {kv.head_dim}"
-    if not kv8_attention_supported(q.dtype, kv.head_dim, kv.page_size, q.shape[-2], kv.kv_heads):
-        raise NotImplementedError(
-            f"attention over the 8-bit cache: {q.dtype}, head_dim {kv.head_dim}, page_size "
-            f"{kv.page_size}, {q.shape[-2]} / {kv.kv_heads} heads")
+def _check_attention(q: torch.Tensor, H: int, KV: int, D: int, P: int) -> None:
+    assert q.shape[-1] == D and H >= KV and H % KV == 0, \
+        f"q heads {tuple(q.shape[-2:])} over {KV} kv heads of {D}"
+    if q.dtype not in (torch.bfloat16, torch.float16) or H // KV not in (1, 2, 4, 8):
+        raise NotImplementedError(f"attention over the 8-bit cache: {q.dtype}, {H} / {KV} heads")
 
 
 def paged_decode_attention_kv8(q: torch.Tensor, kv: KV8Pages, tables: torch.Tensor,
@@ -265,32 +285,32 @@ def paged_decode_attention_kv8(q: torch.Tensor, kv: KV8Pages, tables: torch.Tens
     num_splits page-aligned splits of a sequence (None: kv8_splits). `out` / `workspace`
     (kv8_workspace of the same sizes) let a caller pass address-stable buffers. A length is taken
     as at most the tokens its table row has pages for; a row that sees no token is NaN."""
-    _check_pages(kv)
-    dev = q.device
-    _on(dev, q, *kv, tables, seq_lens)
+    NB, KV, D, P = _pool(kv)
+    dev = _device(q, kv.k, kv.v, kv.scales, tables, seq_lens)
     assert q.dim() == 3
-    B, H, D = q.shape
-    _check_attention(q, kv)
-    W = _check_tables(kv, B, tables, seq_lens)
-    S = kv8_splits(B, kv.kv_heads, W, kv.page_size) if num_splits is None else int(num_splits)
+    B, H, _ = q.shape
+    _check_attention(q, H, KV, D, P)
+    W = _check_tables(B, tables, seq_lens)
+    S = kv8_splits(B, KV, W, P) if num_splits is None else int(num_splits)
     assert S >= 1
-    q2 = _aligned(q)
+    q = _aligned(q)
     if out is None:
-        out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
-    _check_out(out, (B, H, D), q.dtype, dev)
-    if workspace is None:
-        workspace = kv8_workspace(B, H, D, S, dev)
-    acc, ml = workspace if workspace is not None and S > 1 else (None, None)
+        out = torch.empty_like(q)
+    else:
+        _check_out(out, (B, H, D), q.dtype, dev)
+    ws = (None, None)
     if S > 1:
-        for t, n in ((acc, B * H * S * D), (ml, 2 * B * H * S)):
-            assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() >= n and \
-                t.device == dev, "workspace: kv8_workspace of the same sizes"
-    with torch.cuda.device(dev):
-        rc = lib().acorn_paged_attention_kv8(
-            ptr(q2), *map(ptr, kv), ptr(tables), ptr(seq_lens), ptr(out), ptr(acc), ptr(ml), B, H,
-            kv.kv_heads, D, kv.page_size, kv.num_blocks, W, S, float(D ** -0.5), dtype_code(q2),
-            stream_ptr(dev))
-    check(rc, "paged_decode_attention_kv8")
+        ws = workspace
+        if ws is None:
+            ws = kv8_workspace(B, H, D, S, q.device)
+        elif B:
+            for t, n in ((ws[0], B * H * S * D), (ws[1], 2 * B * H * S)):
+                assert t.dtype is torch.float32 and t.is_contiguous() and t.numel() >= n and \
+                    t.get_device() == dev and t.data_ptr() % 16 == 0, \
+                    "workspace: kv8_workspace of the same sizes"
+    _call("paged_attention_kv8", dev, q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(),
+          kv.scales.data_ptr(), tables.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ptr(ws[0]),
+          ptr(ws[1]), B, H, KV, D, P, NB, W, S, float(D ** -0.5), dtype_code(q))
     return out
 
 
@@ -309,16 +329,13 @@ def prefill_workspace_kv8(N: int, R: int, max_nq: int, H: int, KV: int, D: int, 
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
-def _prefill(q2, kv, tables, row0, pos0, nq, out, N, R, max_nq, W) -> None:
-    H, D = q2.shape[-2:]
-    dev = q2.device
-    ws = prefill_workspace_kv8(N, R, max_nq, H, kv.kv_heads, D, kv.page_size, W, dev)
-    with torch.cuda.device(dev):
-        rc = lib().acorn_paged_prefill_attention_kv8(
-            ptr(q2), *map(ptr, kv), ptr(tables), ptr(row0), ptr(pos0), ptr(nq), ptr(out), N, R,
-            max_nq, H, kv.kv_heads, D, kv.page_size, kv.num_blocks, W, float(D ** -0.5),
-            dtype_code(q2), ptr(ws), 0 if ws is None else ws.numel(), stream_ptr(dev))
-    check(rc, "paged_prefill_attention_kv8")
+def _prefill(dev, q, kv, pool, tables, row0, pos0, nq, out, N, R, max_nq, H, W) -> None:
+    NB, KV, D, P = pool
+    ws = prefill_workspace_kv8(N, R, max_nq, H, KV, D, P, W, q.device)
+    _call("paged_prefill_attention_kv8", dev, q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(),
+          kv.scales.data_ptr(), tables.data_ptr(), ptr(row0), pos0.data_ptr(), ptr(nq),
+          out.data_ptr(), N, R, max_nq, H, KV, D, P, NB, W, float(D ** -0.5), dtype_code(q), ptr(ws),
+          0 if ws is None else ws.numel())
 
 
 def paged_prefill_attention_kv8(q: torch.Tensor, kv: KV8Pages, tables: torch.Tensor,
@@ -330,20 +347,20 @@ def paged_prefill_attention_kv8(q: torch.Tensor, kv: KV8Pages, tables: torch.Ten
     seq_pos0[n] + j and attends to the sequence's tokens 0 .. its own position, which are in the
     cache. Rows not covered by a sequence, or past their table row's pages, are left as they were
     in `out`."""
-    _check_pages(kv)
-    dev = q.device
-    _on(dev, q, *kv, tables, seq_row0, seq_pos0, seq_nq)
+    pool = _pool(kv)
+    dev = _device(q, kv.k, kv.v, kv.scales, tables, seq_row0, seq_pos0, seq_nq)
     assert q.dim() == 3
     R, H, D = q.shape
-    _check_attention(q, kv)
+    _check_attention(q, H, *pool[1:])
     N = seq_row0.shape[0]
-    W = _check_tables(kv, N, tables, seq_row0, seq_pos0, seq_nq)
+    W = _check_tables(N, tables, seq_row0, seq_pos0, seq_nq)
     assert int(max_nq) >= 0
-    q2 = _aligned(q)
+    q = _aligned(q)
     if out is None:
-        out = torch.empty((R, H, D), dtype=q.dtype, device=dev)
-    _check_out(out, (R, H, D), q.dtype, dev)
-    _prefill(q2, kv, tables, seq_row0, seq_pos0, seq_nq, out, N, R, int(max_nq), W)
+        out = torch.empty_like(q)
+    else:
+        _check_out(out, (R, H, D), q.dtype, dev)
+    _prefill(dev, q, kv, pool, tables, seq_row0, seq_pos0, seq_nq, out, N, R, int(max_nq), H, W)
     return out
 
 
@@ -357,12 +374,11 @@ def paged_verify_attention_kv8(q: torch.Tensor, kv: KV8Pages, tables: torch.Tens
     assert M >= 1, "verify window must be non-empty"
     if M == 1:
         return paged_decode_attention_kv8(q[:, 0], kv, tables, seq_lens)[:, None]
-    _check_pages(kv)
-    dev = q.device
-    _on(dev, q, *kv, tables, seq_lens)
-    _check_attention(q, kv)
-    W = _check_tables(kv, B, tables, seq_lens)
-    q2 = _aligned(q)
-    out = torch.empty_like(q2)
-    _prefill(q2, kv, tables, None, seq_lens, None, out, B, B * M, M, W)
+    pool = _pool(kv)
+    dev = _device(q, kv.k, kv.v, kv.scales, tables, seq_lens)
+    _check_attention(q, H, *pool[1:])
+    W = _check_tables(B, tables, seq_lens)
+    q = _aligned(q)
+    out = torch.empty_like(q)
+    _prefill(dev, q, kv, pool, tables, None, seq_lens, None, out, B, B * M, M, H, W)
     return out

@@ -331,19 +331,34 @@ int decode_rep(const DecodeArgs& a) {
 }
 
 // ---------------------------------------------------------------------------
-// Prefill: the query-tiled kernel of the 16-bit cache (paged_attention.hip) over
-// 8-bit tiles. A workgroup serves the REP q heads of a kv head for WQ query
-// tokens, wave (head, group) QW blocks of 16; the keys are walked in chunks of
-// 64, which the workgroup turns into 16 bits once, on their way into LDS:
-// per chunk and thread (4 waves, D = 128) two 16-byte pieces of K and two of V,
-// 32 conversions against some 290 other VALU instructions, and half the loads
-// of a 16-bit cache. Per 32 keys and query block: S^T = K Q^T, the online
-// softmax per query column, O^T += V^T P^T with V^T from LDS by
-// ds_read_b64_tr_b16, the P V MFMAs one step behind the scores'. Masked scores
-// are set to -inf whatever they are, and V bytes are finite, so a row that holds
-// NaN reaches only the queries that see it; past the last key bytes are taken as 0.
-// SPLIT, WIN, the partials and their merge: as there.
-template <typename T, int D, int REP, int QG, int KC, int QW, bool SPLIT, bool WIN>
+// Prefill: query-tiled flash attention, causal. A workgroup serves the REP q heads
+// of a kv head for WQ query tokens, wave (head, group) QW blocks of 16 of them; it
+// walks the keys in steps of 32. Per step and query block, as in decode but with 16
+// queries of one head as the MFMA's columns: S^T = K Q^T, the online softmax per
+// query column (the maximum moved only by scores that exceed it by kMaxSlack, the
+// scale inside the exp2 argument), O^T += V^T P^T. The sums of P are the row of ones
+// that an MFMA with a ones operand adds up.
+//
+// Bytes become T once per workgroup, on their way into LDS (rows padded by 32
+// bytes: neither the score operand's reads nor the transposing ds_read_b64_tr_b16
+// of V conflict). What bounds the kernel is that a step's MFMAs (512 cycles of a
+// SIMD at QW = 2), VALU work (about 600: 16 exponentials of 16 cycles each among
+// it) and LDS reads take as long as each other, so they have to run at the same
+// time. An iteration therefore holds three steps' work without dependences between
+// them: the probabilities of step s, the P V MFMAs of step s - 1 and the score
+// MFMAs of step s + 1, issued alternately (the scheduling groups below), while V of
+// step s moves from LDS into registers and K of step s + 2 and V of step s + 1
+// from registers into LDS. K and V have two LDS buffers each, with one barrier per
+// step. A rare branch at the end of an iteration moves the maximum: it first
+// adds the P V that is still due.
+//
+// Masked scores are set to -inf whatever they are, and V bytes are finite, so a row
+// that holds NaN reaches only the queries that see it; V rows past the last key are
+// taken as 0. Steps before the workgroup's first query need no mask.
+// SPLIT, WIN, partials and merge: as in paged_attention.hip. The kv head is the
+// grid's fastest index: workgroups are dealt to the 8 XCDs round robin, so with a
+// multiple of 8 kv heads a head's keys stay in one XCD's L2.
+template <typename T, int D, int REP, int QG, int QW, bool SPLIT, bool WIN>
 __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ k_tiles,
     const uint8_t* __restrict__ v_tiles, const uint8_t* __restrict__ scales,
@@ -352,15 +367,15 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     int R, int H, int KV, int P, int num_blocks, int table_stride, float scale_log2, int max_nq,
     int S, int cps, float* __restrict__ ws, int cap) {
   constexpr int NT = REP * QG * kWave;           // threads
-  constexpr int KB = D / 32, DPL = D / 16;
-  constexpr int PITCH = 2 * D + 32;              // bytes per staged row (padded against LDS conflicts)
+  constexpr int KB = D / 32, E = D / 16, TP = 16 / E;
+  constexpr int PITCH = 2 * D + 32;              // bytes per staged row
+  constexpr int KC = 32;                         // keys per step
   constexpr int WQ = QG * QW * 16;               // query rows per workgroup
-  constexpr int TC = KC / kKv8Group;             // tiles per chunk, K or V
-  constexpr int PCS = TC * D;                    // 16-byte pieces per chunk, K or V
-  constexpr int PPT = 2 * PCS / NT;              // pieces per thread per chunk
-  static_assert(2 * PCS % NT == 0 && D % kWave == 0, "whole pieces per thread, one tile per wave");
-  __shared__ __align__(16) uint8_t kvs[2][2 * KC * PITCH];       // [buffer][K rows | V rows]
-  const int kvh = blockIdx.y, n = blockIdx.z;
+  constexpr int PCS = KC / kKv8Group * D;        // 16-byte pieces per step, K or V
+  constexpr int PPT = (2 * PCS + NT - 1) / NT;   // pieces per thread per step
+  static_assert((2 * PCS) % NT == 0 || 2 * PCS < NT, "whole pieces per thread");
+  __shared__ __align__(16) uint8_t ks[2][KC * PITCH], vs[2][KC * PITCH];
+  const int kvh = blockIdx.x % KV, n = blockIdx.y;
   const int tid = threadIdx.x;
   const int wid = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lane = tid % kWave;
@@ -370,17 +385,17 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
   const PrefillSeq sq = prefill_seq<WIN>(seq_row0, seq_pos0, seq_nq, n, R, max_nq, cap);
   // (rows placed past their table row's pages are not served)
   const int pos0 = sq.pos0, row0 = sq.row0, nq = WIN ? sq.nq : min(sq.nq, cap - pos0);
-  const int tile_q = SPLIT ? (gridDim.x - 1 - blockIdx.x) / S : gridDim.x - 1 - blockIdx.x;
-  const int wg_j0 = tile_q * WQ;                                // longest tiles first
+  const int by = (int)((gridDim.x - 1 - blockIdx.x) / KV);      // longest tiles first
+  const int tile_q = SPLIT ? by / S : by;
+  const int wg_j0 = tile_q * WQ;
   if (wg_j0 >= nq) return;                                      // uniform over the workgroup
   const int j0 = wg_j0 + sub * QW * 16;                         // this wave's first query row
   const int nvalid = max(0, min(QW * 16, nq - j0));             // 0: the wave only stages
   const int L = pos0 + min(wg_j0 + WQ, nq);                     // keys of the workgroup's last query
-  const int total = (L + KC - 1) / KC;
-  const int sp = SPLIT ? (gridDim.x - 1 - blockIdx.x) % S : 0;
+  const int total = (L + kPrefillChunk - 1) / kPrefillChunk;
+  const int sp = SPLIT ? by % S : 0;
   const int cb = SPLIT ? sp * cps : 0;
-  const int nchunks = SPLIT ? min(cb + cps, total) : total;
-  if (cb >= nchunks) {                           // uniform over the workgroup
+  if (cb >= total) {                             // uniform over the workgroup
     // a window's tile before its sequence's first token sees no key
     if (WIN && total <= 0 && sp == 0) {
 #pragma unroll
@@ -388,12 +403,17 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
         if (16 * qw + c < nvalid) {
           T* o = out + ((size_t)(row0 + j0 + 16 * qw + c) * H + h) * D + 4 * r;
 #pragma unroll
-          for (int jj = 0; jj < DPL; ++jj)
+          for (int jj = 0; jj < E; ++jj)
             *(u32x2_t*)(o + 16 * jj) = u32x2_t{pack2<T>(NAN, NAN), pack2<T>(NAN, NAN)};
         }
     }
     return;
   }
+  // this workgroup's steps [s0, s1); those before sm need no mask
+  constexpr int SPC = kPrefillChunk / KC;
+  const int steps = (L + KC - 1) / KC;
+  const int s0 = cb * SPC, s1 = SPLIT ? min((cb + cps) * SPC, steps) : steps;
+  const int sm = min(max((pos0 + wg_j0 + 1) / KC, s0), s1);
   const int32_t* trow = tables + (size_t)n * table_stride;
   const int gshift = __builtin_ctz(P) - 4;
   const int glast = (L - 1) / kKv8Group;
@@ -411,164 +431,118 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       qb[qw][jb] = *(const u32x4_t*)(q + (qrow * H + h) * D + 32 * jb + 8 * r);
   }
 
-  // Staging. Piece x = i NT + tid of a chunk: K's for x < PCS, V's from there; piece
-  // x % D of tile x / D. K: dims 16 (x % D / 16) .. of token x % 16. V: the E dims of
-  // 16 / E tokens (kv8.h). A wave's pieces are of one kind and one tile (D and PCS are
-  // multiples of 64), so the block ids are scalar loads.
-  constexpr int E = D / 16, TP = 16 / E;
+  // Staging. Piece x = i NT + tid of a step: K's for x < PCS, V's from there; piece x % D
+  // of tile x / D. K: dims 16 (x % D / 16) .. of token x % 16. V: the E dims of TP tokens
+  // (kv8.h). A wave's pieces are of one kind and one tile (D and PCS are multiples of
+  // 64), so the block ids are scalar loads. An iteration stages K of the step after V's.
   u32x4_t stage[PPT];
   uint32_t code[PPT];
-  auto of_k = [&](int i) {                       // the wave's i-th pieces are K's (uniform)
-    return (i + 1) * NT <= PCS || (i * NT < PCS && i * NT + wid * kWave < PCS);
-  };
-  auto tile_at = [&](int chunk, int i) -> size_t {
-    const int x = i * NT + wid * kWave;
-    const int g = min(chunk * TC + (x % PCS) / D, glast);
+  size_t tl[PPT];
+  const bool stages = 2 * PCS >= NT || wid * kWave < 2 * PCS;
+  auto first = [&](int i) { return i * NT + wid * kWave; };     // the wave's first piece
+  auto of_k = [&](int i) { return (i + 1) * NT <= PCS || (i * NT < PCS && first(i) < PCS); };
+  auto find = [&](int i, int step) {
+    const int g = min(2 * step + (first(i) % PCS) / D, glast);
     const unsigned pg = (unsigned)trow[min(g >> gshift, table_stride - 1)];
     const size_t blk = pg < (unsigned)num_blocks ? pg : 0u;
-    return ((blk * KV + kvh) << gshift) + (g & ((1 << gshift) - 1));
+    tl[i] = ((blk * KV + kvh) << gshift) + (g & ((1 << gshift) - 1));
   };
-  auto load_chunk = [&](const size_t (&tl)[PPT]) {
-#pragma unroll
-    for (int i = 0; i < PPT; ++i) {
-      const int x0 = i * NT + wid * kWave;       // the wave's first piece
-      const int p = x0 % D + lane;               // piece of the tile
-      const uint8_t* src = (of_k(i) ? k_tiles : v_tiles) + tl[i] * (16 * D);
-      const uint8_t* sb = scales + tl[i] * 32;
-      stage[i] = *(const u32x4_t*)(src + p * 16);
-      if (of_k(i)) {
-        code[i] = sb[p % 16];
-      } else if constexpr (TP == 2) {
-        code[i] = *(const uint16_t*)(sb + 16 + 4 * (p % 64 / 16) + 2 * (p / 64));
-      } else {
-        code[i] = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
-      }
+  auto load = [&](int i) {
+    const int p = first(i) % D + lane;           // piece of the tile
+    const uint8_t* src = (of_k(i) ? k_tiles : v_tiles) + tl[i] * (16 * D);
+    const uint8_t* sb = scales + tl[i] * 32;
+    stage[i] = *(const u32x4_t*)(src + p * 16);
+    if (of_k(i)) {
+      code[i] = sb[p % 16];
+    } else if constexpr (TP == 2) {
+      code[i] = *(const uint16_t*)(sb + 16 + 4 * (p % 64 / 16) + 2 * (p / 64));
+    } else {
+      code[i] = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
     }
   };
-  auto store_chunk = [&](int bf, int chunk) {
-    const bool tail = chunk * KC + KC > L;       // uniform
+  auto store = [&](int i, int step) {
+    const int p = first(i) % D + lane;
+    const int t0 = (first(i) % PCS) / D * kKv8Group;            // the tile's first row
+    if (of_k(i)) {
+      const float f = kv8_scale(code[i]);
+      uint8_t* dst = ks[step & 1] + (t0 + p % 16) * PITCH + p / 16 * 32;
+      *(u32x4_t*)dst = kv8_cvt8<T>(stage[i][0], stage[i][1], f);
+      *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(stage[i][2], stage[i][3], f);
+    } else {
+      const int t = t0 + 4 * (p % 64 / 16) + TP * (p / 64);
+      uint8_t* dst = vs[step & 1] + t * PITCH + p % 16 * (2 * E);
+      if (step * KC + KC > L) {                  // uniform: rows past the last key
 #pragma unroll
-    for (int i = 0; i < PPT; ++i) {
-      const int x0 = i * NT + wid * kWave;
-      const int p = x0 % D + lane;
-      const int t0 = (x0 % PCS) / D * kKv8Group;   // the tile's first row of the chunk
-      if (of_k(i)) {
-        const float f = kv8_scale(code[i]);
-        uint8_t* dst = kvs[bf] + (t0 + p % 16) * PITCH + p / 16 * 32;
-        *(u32x4_t*)dst = kv8_cvt8<T>(stage[i][0], stage[i][1], f);
-        *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(stage[i][2], stage[i][3], f);
-      } else {
-        const int t = t0 + 4 * (p % 64 / 16) + TP * (p / 64);
-        uint8_t* dst = kvs[bf] + KC * PITCH + t * PITCH + p % 16 * (2 * E);
+        for (int j = 0; j < TP; ++j)
+          if (step * KC + t + j >= L) {
 #pragma unroll
-        for (int j = 0; j < TP; ++j) {
-          const float f = kv8_scale_finite(code[i] >> (8 * j) & 0xFFu);
-          const bool off = tail && chunk * KC + t + j >= L;
-          if constexpr (TP == 2) {
-            *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(off ? 0u : stage[i][2 * j], off ? 0u : stage[i][2 * j + 1], f);
-          } else {
-            const uint32_t w = off ? 0u : stage[i][j];
-            *(u32x2_t*)(dst + j * PITCH) = u32x2_t{kv8_cvt2<T, false>(w, f), kv8_cvt2<T, true>(w, f)};
+            for (int w = 0; w < E / 4; ++w) stage[i][E / 4 * j + w] = 0u;
           }
-        }
+      }
+#pragma unroll
+      for (int j = 0; j < TP; ++j) {
+        const float f = kv8_scale_finite(code[i] >> (8 * j) & 0xFFu);
+        if constexpr (TP == 2)
+          *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(stage[i][2 * j], stage[i][2 * j + 1], f);
+        else
+          *(u32x2_t*)(dst + j * PITCH) =
+              u32x2_t{kv8_cvt2<T, false>(stage[i][j], f), kv8_cvt2<T, true>(stage[i][j], f)};
       }
     }
   };
+  // the step that piece i belongs to in iteration s, and a step's clamp
+  auto step_of = [&](int i, int s) { return of_k(i) ? s + 2 : s + 1; };
 
-  float m[QW], l[QW], nm[QW];                    // nm: -m (0 while m is -inf)
-  f32x4_t acc[QW][DPL];
+  float m[QW], nm[QW];                           // nm: -m (0 while m is -inf)
+  f32x4_t acc[QW][E], accl[QW], sc[QW][2];
+  u32x4_t va[E], pb[QW];
+  const uint32_t one2 = std::is_same<T, __bf16>::value ? 0x3F803F80u : 0x3C003C00u;
+  const u32x4_t ones = {one2, one2, one2, one2};
 #pragma unroll
   for (int qw = 0; qw < QW; ++qw) {
     m[qw] = -INFINITY;
-    l[qw] = nm[qw] = 0.f;
+    nm[qw] = 0.f;
+    accl[qw] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int jj = 0; jj < DPL; ++jj) acc[qw][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int jj = 0; jj < E; ++jj) acc[qw][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+#pragma unroll
+  for (int jj = 0; jj < E; ++jj) va[jj] = u32x4_t{0u, 0u, 0u, 0u};
   const uint32_t vlane = (uint32_t)((4 * r + (c >> 2)) * PITCH + 8 * (c & 3));
-  u32x4_t va[DPL], pb[QW];
-#pragma unroll
-  for (int jj = 0; jj < DPL; ++jj) va[jj] = u32x4_t{0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int qw = 0; qw < QW; ++qw) pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
-  const int tlast = pos0 + j0 + min(16 * QW, nvalid) - 1;   // the wave's last query
+
   auto pv = [&]() {
 #pragma unroll
-    for (int jj = 0; jj < DPL; ++jj)
+    for (int jj = 0; jj < E; ++jj)
 #pragma unroll
       for (int qw = 0; qw < QW; ++qw) acc[qw][jj] = mfma16x16x32<T>(va[jj], pb[qw], acc[qw][jj]);
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) accl[qw] = mfma16x16x32<T>(ones, pb[qw], accl[qw]);
   };
-  auto step = [&](int bf, int s32, int t0) {
-    if (t0 > tlast) return;                      // keys after every query of the wave
-    const uint8_t* kbuf = kvs[bf] + 32 * s32 * PITCH;
-    const uint8_t* vbuf = kvs[bf] + KC * PITCH + 32 * s32 * PITCH;
-    u32x4_t kf[2][KB];
+  u32x4_t kf[2][KB];
+  auto read_k = [&](int step) {
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
       for (int jb = 0; jb < KB; ++jb)
-        kf[hh][jb] = *(const u32x4_t*)(kbuf + (16 * hh + c) * PITCH + 2 * (32 * jb + 8 * r));
-    f32x4_t sc[QW][2];
-    bool live[QW];
+        kf[hh][jb] = *(const u32x4_t*)(ks[step & 1] + (16 * hh + c) * PITCH + 2 * (32 * jb + 8 * r));
+  };
+  auto scores = [&]() {
 #pragma unroll
-    for (int qw = 0; qw < QW; ++qw) {
-      // the block's queries all precede these keys, or it has none: nothing to add
-      live[qw] = 16 * qw < nvalid && t0 <= pos0 + j0 + min(16 * qw + 15, nvalid - 1);
-      sc[qw][0] = sc[qw][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int qw = 0; qw < QW; ++qw) sc[qw][0] = sc[qw][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int jb = 0; jb < KB; ++jb)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int qw = 0; qw < QW; ++qw)
-          sc[qw][hh] = mfma16x16x32<T>(kf[hh][jb], qb[qw][jb], sc[qw][hh]);
-    pv();
-#pragma unroll
-    for (int qw = 0; qw < QW; ++qw) {
-      if (!live[qw]) {
-        pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
-        continue;
-      }
-      float sv[8];                               // raw scores; scaled inside the exp2
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sv[4 * hh + i] = sc[qw][hh][i];
-      if (t0 + 31 > pos0 + j0 + 16 * qw) {       // the keys cross some column's diagonal
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (t0 + 16 * hh + 4 * r + i > pc[qw]) sv[4 * hh + i] = -INFINITY;
-      }
-      float mx = sv[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sv[i]);
-      mx *= scale_log2;                          // scale_log2 > 0
-      if (__builtin_amdgcn_ballot_w64(mx > m[qw] + kMaxSlack) != 0) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m[qw], mx);
-        // (a query that has seen no key yet keeps -inf: alpha 0, p = exp2(-inf))
-        nm[qw] = mn == -INFINITY ? 0.f : -mn;
-        const float alpha = __builtin_amdgcn_exp2f(m[qw] + nm[qw]);
-        m[qw] = mn;
-        l[qw] *= alpha;
-#pragma unroll
-        for (int jj = 0; jj < DPL; ++jj) acc[qw][jj] *= alpha;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i], scale_log2, nm[qw]));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i + 1], scale_log2, nm[qw]));
-        pb[qw][i] = pack_dot<T>(p0, p1, l[qw]);
-      }
-    }
+        for (int qw = 0; qw < QW; ++qw) sc[qw][hh] = mfma16x16x32<T>(kf[hh][jb], qb[qw][jb], sc[qw][hh]);
+  };
+  auto read_v = [&](int step) {
     typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
     const __attribute__((address_space(3))) uint8_t* vl =
-        (const __attribute__((address_space(3))) uint8_t*)vbuf + vlane;
+        (const __attribute__((address_space(3))) uint8_t*)vs[step & 1] + vlane;
 #pragma unroll
-    for (int jj = 0; jj < DPL; ++jj) {
+    for (int jj = 0; jj < E; ++jj) {
       const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + 32 * jj));
       const s16x4_t hi =
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vl + 16 * PITCH + 32 * jj));
@@ -576,71 +550,133 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       va[jj] = u32x4_t{l2[0], l2[1], h2[0], h2[1]};
     }
   };
-
-  // prologue: chunk 0 staged, chunk 1's loads in flight
-  size_t tl[PPT];
-  auto tiles_of = [&](int chunk) {
+  // the scores of `step` (raw; lane (r, c) holds keys 4 r .. 4 r + 3 of each half for query
+  // c of a block), masked, and the maxima
+  auto settle = [&](int step, auto masked) {
+    if constexpr (decltype(masked)::value) {
 #pragma unroll
-    for (int i = 0; i < PPT; ++i) tl[i] = tile_at(min(chunk, nchunks - 1), i);
-  };
-  tiles_of(cb);
-  load_chunk(tl);
-  tiles_of(cb + 1);
-  store_chunk(0, cb);
-  load_chunk(tl);
-  __syncthreads();
-  for (int ci = cb; ci < nchunks; ++ci) {
-    const int bf = (ci - cb) & 1;
-    tiles_of(ci + 2);                            // two chunks ahead
-    __builtin_amdgcn_sched_barrier(0);
-    if (nvalid > 0) {
+      for (int qw = 0; qw < QW; ++qw)
 #pragma unroll
-      for (int s32 = 0; s32 < KC / 32; ++s32) step(bf, s32, ci * KC + 32 * s32);
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (step * KC + 16 * hh + 4 * r + i > pc[qw]) sc[qw][hh][i] = -INFINITY;
     }
-    __builtin_amdgcn_sched_barrier(0);
-    store_chunk(bf ^ 1, min(ci + 1, nchunks - 1));   // its buffer was last read in ci - 1
-    __builtin_amdgcn_sched_barrier(0);
-    load_chunk(tl);
-    __syncthreads();
+    float mx[QW];
+    bool up = false;
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) {
+      mx[qw] = sc[qw][0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx[qw] = fmaxf(mx[qw], sc[qw][i / 4][i % 4]);
+      mx[qw] *= scale_log2;                      // scale_log2 > 0
+      up |= mx[qw] > m[qw] + kMaxSlack;
+    }
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+      pv();                                      // due with the old maximum
+#pragma unroll
+      for (int qw = 0; qw < QW; ++qw) {
+        pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
+        float x = fmaxf(mx[qw], __shfl_xor(mx[qw], 16));
+        x = fmaxf(x, __shfl_xor(x, 32));
+        const float mn = fmaxf(m[qw], x);
+        // (a query that has seen no key yet keeps -inf: alpha 0, p = exp2(-inf))
+        nm[qw] = mn == -INFINITY ? 0.f : -mn;
+        const float alpha = __builtin_amdgcn_exp2f(m[qw] + nm[qw]);
+        m[qw] = mn;
+        accl[qw] *= alpha;
+#pragma unroll
+        for (int jj = 0; jj < E; ++jj) acc[qw][jj] *= alpha;
+      }
+    }
+  };
+
+  // prologue: K of steps s0 and s0 + 1, V of s0 staged; the pieces of iteration s0 in flight
+#pragma unroll
+  for (int d = -2; d <= 0; ++d) {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i)
+      if (stages && (d == 0 || of_k(i) || d == -1)) {
+        find(i, step_of(i, s0 + d));
+        load(i);
+      }
+    if (d < 0) {
+#pragma unroll
+      for (int i = 0; i < PPT; ++i)
+        if (stages && (of_k(i) || d == -1)) store(i, step_of(i, s0 + d));
+    }
   }
+#pragma unroll
+  for (int i = 0; i < PPT; ++i)
+    if (stages) find(i, step_of(i, s0 + 1));
+  __syncthreads();
+  read_k(s0);
+  scores();
+  if (s0 < sm) settle(s0, std::false_type{});
+  else settle(s0, std::true_type{});
+  __syncthreads();
+
+  auto iteration = [&](int s, auto masked) {
+    read_k(s + 1);
+    u32x4_t pn[QW];
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(sc[qw][i / 2][2 * (i % 2)], scale_log2, nm[qw]));
+        const float p1 = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(sc[qw][i / 2][2 * (i % 2) + 1], scale_log2, nm[qw]));
+        if constexpr (std::is_same<T, __bf16>::value) pn[qw][i] = pack_bf16x2(p0, p1);
+        else pn[qw][i] = pack2<T>(p0, p1);
+      }
+    pv();
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) pb[qw] = pn[qw];
+    scores();
+    read_v(s);
+#pragma unroll
+    for (int i = 0; i < PPT; ++i)
+      if (stages) {
+        store(i, step_of(i, s));
+        load(i);                                 // of iteration s + 1
+        find(i, step_of(i, s + 2));
+      }
+    settle(s + 1, masked);
+    __syncthreads();
+  };
+  for (int s = s0; s < sm - 1; ++s) iteration(s, std::false_type{});
+  for (int s = max(sm - 1, s0); s < s1; ++s) iteration(s, std::true_type{});
   if (nvalid == 0) return;
   pv();
   if (SPLIT && total > cps) {                    // one run of several: its fp32 partial
-    const size_t slots = (size_t)prefill_slots(gridDim.z, R, max_nq) * H;
+    const size_t slots = (size_t)prefill_slots(gridDim.y, R, max_nq) * H;
     float2* ml = (float2*)(ws + (size_t)S * slots * D);
 #pragma unroll
-    for (int qw = 0; qw < QW; ++qw) {
-      float lt = l[qw];
-      lt += __shfl_xor(lt, 16);
-      lt += __shfl_xor(lt, 32);
+    for (int qw = 0; qw < QW; ++qw)
       if (16 * qw + c < nvalid) {
         const size_t slot = (size_t)sp * slots +
-                            (size_t)prefill_slot(gridDim.z, R, max_nq, n, row0, j0 + 16 * qw + c) * H + h;
+                            (size_t)prefill_slot(gridDim.y, R, max_nq, n, row0, j0 + 16 * qw + c) * H + h;
 #pragma unroll
-        for (int jj = 0; jj < DPL; ++jj)
+        for (int jj = 0; jj < E; ++jj)
           *(f32x4_t*)(ws + slot * D + 16 * jj + 4 * r) = acc[qw][jj];
-        if (r == 0) ml[slot] = make_float2(m[qw], lt);
+        if (r == 0) ml[slot] = make_float2(m[qw], accl[qw][0]);
       }
-    }
     return;
   }
   // lane (r, c) of block qw holds dims 16 jj + 4 r + i of query column 16 qw + c
 #pragma unroll
-  for (int qw = 0; qw < QW; ++qw) {
-    float lt = l[qw];
-    lt += __shfl_xor(lt, 16);
-    lt += __shfl_xor(lt, 32);
+  for (int qw = 0; qw < QW; ++qw)
     if (16 * qw + c < nvalid) {
       const size_t orow = (size_t)(row0 + j0 + 16 * qw + c) * H + h;
-      const float inv = 1.0f / lt;
+      const float inv = 1.0f / accl[qw][0];
 #pragma unroll
-      for (int jj = 0; jj < DPL; ++jj) {
+      for (int jj = 0; jj < E; ++jj) {
         const u32x2_t w = {pack2<T>(acc[qw][jj][0] * inv, acc[qw][jj][1] * inv),
                            pack2<T>(acc[qw][jj][2] * inv, acc[qw][jj][3] * inv)};
         *(u32x2_t*)(out + orow * D + 16 * jj + 4 * r) = w;
       }
     }
-  }
 }
 
 struct PrefillArgs {
@@ -661,8 +697,9 @@ int launch_prefill(const PrefillArgs& a) {
   const int64_t tiles = (a.max_nq + WQ - 1) / WQ;
   const int S = SPLIT ? a.plan.S : 1;
   const int cap = (int)std::min<int64_t>(a.table_stride * a.P, 0x7fffffff);
-  kv8_prefill_kernel<T, D, REP, QG, kPrefillChunk, QW, SPLIT, WIN>
-      <<<dim3((unsigned)(tiles * S), (unsigned)a.KV, (unsigned)a.N), dim3(REP * QG * kWave), 0,
+  if (tiles * S > 0x7fffffff / a.KV) return ACORN_ERR_SHAPE;
+  kv8_prefill_kernel<T, D, REP, QG, QW, SPLIT, WIN>
+      <<<dim3((unsigned)(a.KV * tiles * S), (unsigned)a.N), dim3(REP * QG * kWave), 0,
          a.st>>>((const T*)a.q, (const uint8_t*)a.kt, (const uint8_t*)a.vt, (const uint8_t*)a.sc,
                  a.tables, a.row0, a.pos0, a.nq, (T*)a.out, (int)a.R, (int)a.H, (int)a.KV,
                  (int)a.P, (int)a.num_blocks, (int)a.table_stride, a.scale * kLog2e,

@@ -17,6 +17,28 @@ using namespace acorn;
 
 namespace {
 
+// Two floats rounded to T, lo in the low half: one instruction for either type.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 f = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, t2));
+}
+// ... and their sum added to `sum` after the rounding.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const uint32_t u = pack_pair<T>(lo, hi);
+  if constexpr (std::is_same<T, __bf16>::value)
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, u),
+                                          __builtin_bit_cast(t2, 0x3F803F80u), sum, false);
+  else
+    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, u), __builtin_bit_cast(t2, 0x3C003C00u),
+                                 sum, false);
+  return u;
+}
+
 // ---------------------------------------------------------------------------
 // Decode. A workgroup of NWV waves serves one (split, kv head, sequence); its
 // waves divide the split's groups of 16 tokens. Per step of two groups, with
@@ -153,7 +175,7 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
     u32x4_t pb;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      pb[i] = pack_dot<T>(__builtin_amdgcn_exp2f(x[2 * i] - m), __builtin_amdgcn_exp2f(x[2 * i + 1] - m), l);
+      pb[i] = pack_pair_sum<T>(__builtin_amdgcn_exp2f(x[2 * i] - m), __builtin_amdgcn_exp2f(x[2 * i + 1] - m), l);
     // V: token i of group u, E dims in E / 2 words
     uint32_t vt[2][4][E / 2];
 #pragma unroll
@@ -220,7 +242,7 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
           uint32_t w[E / 2];
 #pragma unroll
           for (int j = 0; j < E / 2; ++j)
-            w[j] = pack2<T>(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+            w[j] = pack_pair<T>(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
           __builtin_memcpy(__builtin_assume_aligned(out + orow * D + E * (4 * r + i), 2 * E), w, sizeof(w));
         }
       } else {
@@ -336,21 +358,22 @@ int decode_rep(const DecodeArgs& a) {
 // walks the keys in steps of 32. Per step and query block, as in decode but with 16
 // queries of one head as the MFMA's columns: S^T = K Q^T, the online softmax per
 // query column (the maximum moved only by scores that exceed it by kMaxSlack, the
-// scale inside the exp2 argument), O^T += V^T P^T. The sums of P are the row of ones
-// that an MFMA with a ones operand adds up.
+// scale inside the exp2 argument), O^T += V^T P^T. The sum of a query's P is what an
+// MFMA with ones in place of V^T adds up.
 //
 // Bytes become T once per workgroup, on their way into LDS (rows padded by 32
 // bytes: neither the score operand's reads nor the transposing ds_read_b64_tr_b16
-// of V conflict). What bounds the kernel is that a step's MFMAs (512 cycles of a
-// SIMD at QW = 2), VALU work (about 600: 16 exponentials of 16 cycles each among
-// it) and LDS reads take as long as each other, so they have to run at the same
-// time. An iteration therefore holds three steps' work without dependences between
-// them: the probabilities of step s, the P V MFMAs of step s - 1 and the score
-// MFMAs of step s + 1, issued alternately (the scheduling groups below), while V of
-// step s moves from LDS into registers and K of step s + 2 and V of step s + 1
-// from registers into LDS. K and V have two LDS buffers each, with one barrier per
-// step. A rare branch at the end of an iteration moves the maximum: it first
-// adds the P V that is still due.
+// of V conflict). A step's MFMAs (544 cycles of a SIMD at QW = 2, D = 128) and VALU
+// instructions (about 600: 16 exponentials of 16 cycles among some 100) take as long
+// as each other, so they have to run at the same time: an iteration holds three
+// steps' work without dependences between them, the probabilities of step s, the score
+// MFMAs of step s + 1 and the P V MFMAs of step s - 1, while K of step s + 2 and V of
+// step s move from registers into LDS. K and V have two LDS buffers each, with one
+// barrier per step. 8192 causal tokens, 32 / 8 heads: 521 us (1055 TFLOP/s; a large
+// library product reaches 1208); the steps' parts one after another 772; P V of step
+// s - 1 ahead of the scores, V held in registers over the barrier, 569. Fixed orders
+// of MFMA and VALU instructions (scheduling groups) and wave priorities around
+// the MFMAs were slower than the compiler's order, 530 to 600.
 //
 // Masked scores are set to -inf whatever they are, and V bytes are finite, so a row
 // that holds NaN reaches only the queries that see it; V rows past the last key are
@@ -404,7 +427,7 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
           T* o = out + ((size_t)(row0 + j0 + 16 * qw + c) * H + h) * D + 4 * r;
 #pragma unroll
           for (int jj = 0; jj < E; ++jj)
-            *(u32x2_t*)(o + 16 * jj) = u32x2_t{pack2<T>(NAN, NAN), pack2<T>(NAN, NAN)};
+            *(u32x2_t*)(o + 16 * jj) = u32x2_t{pack_pair<T>(NAN, NAN), pack_pair<T>(NAN, NAN)};
         }
     }
     return;
@@ -460,24 +483,23 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       code[i] = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
     }
   };
-  auto store = [&](int i, int step) {
+  auto store = [&](int i, int step, int buf, auto tail) {      // the pieces of `step`
     const int p = first(i) % D + lane;
     const int t0 = (first(i) % PCS) / D * kKv8Group;            // the tile's first row
     if (of_k(i)) {
       const float f = kv8_scale(code[i]);
-      uint8_t* dst = ks[step & 1] + (t0 + p % 16) * PITCH + p / 16 * 32;
+      uint8_t* dst = ks[buf] + (t0 + p % 16) * PITCH + p / 16 * 32;
       *(u32x4_t*)dst = kv8_cvt8<T>(stage[i][0], stage[i][1], f);
       *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(stage[i][2], stage[i][3], f);
     } else {
       const int t = t0 + 4 * (p % 64 / 16) + TP * (p / 64);
-      uint8_t* dst = vs[step & 1] + t * PITCH + p % 16 * (2 * E);
-      if (step * KC + KC > L) {                  // uniform: rows past the last key
+      uint8_t* dst = vs[buf] + t * PITCH + p % 16 * (2 * E);
+      if constexpr (decltype(tail)::value) {     // rows past the last key
 #pragma unroll
         for (int j = 0; j < TP; ++j)
-          if (step * KC + t + j >= L) {
 #pragma unroll
-            for (int w = 0; w < E / 4; ++w) stage[i][E / 4 * j + w] = 0u;
-          }
+          for (int w = 0; w < E / 4; ++w)
+            stage[i][E / 4 * j + w] = step * KC + t + j < L ? stage[i][E / 4 * j + w] : 0u;
       }
 #pragma unroll
       for (int j = 0; j < TP; ++j) {
@@ -491,7 +513,7 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     }
   };
   // the step that piece i belongs to in iteration s, and a step's clamp
-  auto step_of = [&](int i, int s) { return of_k(i) ? s + 2 : s + 1; };
+  auto step_of = [&](int i, int s) { return of_k(i) ? s + 2 : s; };
 
   float m[QW], nm[QW];                           // nm: -m (0 while m is -inf)
   f32x4_t acc[QW][E], accl[QW], sc[QW][2];
@@ -507,8 +529,6 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
 #pragma unroll
     for (int jj = 0; jj < E; ++jj) acc[qw][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-#pragma unroll
-  for (int jj = 0; jj < E; ++jj) va[jj] = u32x4_t{0u, 0u, 0u, 0u};
   const uint32_t vlane = (uint32_t)((4 * r + (c >> 2)) * PITCH + 8 * (c & 3));
 
   auto pv = [&]() {
@@ -551,8 +571,21 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     }
   };
   // the scores of `step` (raw; lane (r, c) holds keys 4 r .. 4 r + 3 of each half for query
-  // c of a block), masked, and the maxima
+  // c of a block), masked, and the maxima. A move of the maximum by 2^-alpha applies to
+  // the sums one iteration later, once the P V that is still due has been added to them.
+  float alpha[QW];
+#pragma unroll
+  for (int qw = 0; qw < QW; ++qw) alpha[qw] = 1.f;
+  bool moved = false;                            // uniform
   auto settle = [&](int step, auto masked) {
+    if (__builtin_expect(moved, 0)) {
+#pragma unroll
+      for (int qw = 0; qw < QW; ++qw) {
+        accl[qw] *= alpha[qw];
+#pragma unroll
+        for (int jj = 0; jj < E; ++jj) acc[qw][jj] *= alpha[qw];
+      }
+    }
     if constexpr (decltype(masked)::value) {
 #pragma unroll
       for (int qw = 0; qw < QW; ++qw)
@@ -572,39 +605,35 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       mx[qw] *= scale_log2;                      // scale_log2 > 0
       up |= mx[qw] > m[qw] + kMaxSlack;
     }
-    if (__builtin_amdgcn_ballot_w64(up) != 0) {
-      pv();                                      // due with the old maximum
+    moved = __builtin_amdgcn_ballot_w64(up) != 0;
+    if (__builtin_expect(moved, 0)) {
 #pragma unroll
       for (int qw = 0; qw < QW; ++qw) {
-        pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
         float x = fmaxf(mx[qw], __shfl_xor(mx[qw], 16));
         x = fmaxf(x, __shfl_xor(x, 32));
         const float mn = fmaxf(m[qw], x);
         // (a query that has seen no key yet keeps -inf: alpha 0, p = exp2(-inf))
         nm[qw] = mn == -INFINITY ? 0.f : -mn;
-        const float alpha = __builtin_amdgcn_exp2f(m[qw] + nm[qw]);
+        alpha[qw] = __builtin_amdgcn_exp2f(m[qw] + nm[qw]);
         m[qw] = mn;
-        accl[qw] *= alpha;
-#pragma unroll
-        for (int jj = 0; jj < E; ++jj) acc[qw][jj] *= alpha;
       }
     }
   };
 
-  // prologue: K of steps s0 and s0 + 1, V of s0 staged; the pieces of iteration s0 in flight
+  // prologue: K of steps s0 and s0 + 1 staged, the pieces of iteration s0 in flight; as V of
+  // step s0 - 1, which the first iteration multiplies by P = 0, that of s0
 #pragma unroll
   for (int d = -2; d <= 0; ++d) {
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
-      if (stages && (d == 0 || of_k(i) || d == -1)) {
+      if (stages && (d == 0 || of_k(i))) {
         find(i, step_of(i, s0 + d));
         load(i);
       }
-    if (d < 0) {
 #pragma unroll
-      for (int i = 0; i < PPT; ++i)
-        if (stages && (of_k(i) || d == -1)) store(i, step_of(i, s0 + d));
-    }
+    for (int i = 0; i < PPT; ++i)
+      if (stages && of_k(i) == (d < 0))
+        store(i, step_of(i, s0 + d), (of_k(i) ? s0 + d : s0 - 1) & 1, std::true_type{});
   }
 #pragma unroll
   for (int i = 0; i < PPT; ++i)
@@ -627,28 +656,40 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
             __builtin_fmaf(sc[qw][i / 2][2 * (i % 2)], scale_log2, nm[qw]));
         const float p1 = __builtin_amdgcn_exp2f(
             __builtin_fmaf(sc[qw][i / 2][2 * (i % 2) + 1], scale_log2, nm[qw]));
-        if constexpr (std::is_same<T, __bf16>::value) pn[qw][i] = pack_bf16x2(p0, p1);
-        else pn[qw][i] = pack2<T>(p0, p1);
+        pn[qw][i] = pack_pair<T>(p0, p1);
       }
+    scores();
+    read_v(s - 1);
     pv();
 #pragma unroll
     for (int qw = 0; qw < QW; ++qw) pb[qw] = pn[qw];
-    scores();
-    read_v(s);
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
       if (stages) {
-        store(i, step_of(i, s));
+        store(i, step_of(i, s), s & 1, masked);
         load(i);                                 // of iteration s + 1
         find(i, step_of(i, s + 2));
       }
+    // (without this the probabilities' work, next needed in the iteration to come, would sink
+    // behind settle's branch, away from the MFMAs)
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) asm volatile("" : "+v"(pb[qw]));
     settle(s + 1, masked);
     __syncthreads();
   };
   for (int s = s0; s < sm - 1; ++s) iteration(s, std::false_type{});
   for (int s = max(sm - 1, s0); s < s1; ++s) iteration(s, std::true_type{});
   if (nvalid == 0) return;
+  read_v(s1 - 1);
   pv();
+  if (moved) {
+#pragma unroll
+    for (int qw = 0; qw < QW; ++qw) {
+      accl[qw] *= alpha[qw];
+#pragma unroll
+      for (int jj = 0; jj < E; ++jj) acc[qw][jj] *= alpha[qw];
+    }
+  }
   if (SPLIT && total > cps) {                    // one run of several: its fp32 partial
     const size_t slots = (size_t)prefill_slots(gridDim.y, R, max_nq) * H;
     float2* ml = (float2*)(ws + (size_t)S * slots * D);
@@ -672,8 +713,8 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       const float inv = 1.0f / accl[qw][0];
 #pragma unroll
       for (int jj = 0; jj < E; ++jj) {
-        const u32x2_t w = {pack2<T>(acc[qw][jj][0] * inv, acc[qw][jj][1] * inv),
-                           pack2<T>(acc[qw][jj][2] * inv, acc[qw][jj][3] * inv)};
+        const u32x2_t w = {pack_pair<T>(acc[qw][jj][0] * inv, acc[qw][jj][1] * inv),
+                           pack_pair<T>(acc[qw][jj][2] * inv, acc[qw][jj][3] * inv)};
         *(u32x2_t*)(out + orow * D + 16 * jj + 4 * r) = w;
       }
     }

@@ -16,6 +16,8 @@ in:
   m-token window per sequence with the same scatter kernel,
   `ensure_append_capacity_n` reserves the window, `set_lens` rolls a length
   back after a partial accept.
+- `PagedKV8Cache`: the same cache in 8 bits (ops/kv8.py), about half the memory
+  and half the bytes attention reads. No counterpart in the reference.
 - `PagedCacheView` (pager.py:151-259): the block table is a `list[int]`
   shared with the caller; written length is tracked per layer; token t of a
   sequence lives at (table[t // P], t % P). `ensure_append_capacity`
@@ -29,6 +31,7 @@ from __future__ import annotations
 import torch
 
 from acorninfer_amd._lib import check, dtype_code, lib, ptr, stream_ptr
+from acorninfer_amd.ops.kv8 import (GROUP, KV8Pages, kv8_gather, kv8_scatter, kv8_supported)
 
 
 class BlockExhausted(Exception):
@@ -77,6 +80,8 @@ class BlockAllocator:
 class PagedKVCache:
     """Physical page storage for every layer, one contiguous pool per K / V."""
 
+    scale_pool: torch.Tensor | None = None     # (of an 8-bit cache)
+
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, page_size: int,
                  allocator: BlockAllocator, device, dtype: torch.dtype):
         self.num_layers = num_layers
@@ -87,6 +92,11 @@ class PagedKVCache:
         self.device = torch.device(device)
         self.dtype = dtype
         self.num_blocks = allocator.total
+        self._allocate()
+
+    def _allocate(self) -> None:
+        num_layers, page_size = self.num_layers, self.page_size
+        num_kv_heads, head_dim, dtype = self.num_kv_heads, self.head_dim, self.dtype
         shape = (num_layers, self.num_blocks, page_size, num_kv_heads, head_dim)
         self.k_pool = torch.zeros(shape, device=self.device, dtype=dtype)
         self.v_pool = torch.zeros(shape, device=self.device, dtype=dtype)
@@ -119,6 +129,21 @@ class PagedKVCache:
             raise IndexError(f"(page, slot) outside the pool of {self.num_blocks} blocks x "
                              f"{self.page_size} slots")
 
+    def _scatter(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor,
+                 slots: torch.Tensor, op: str) -> None:
+        """Rows k, v (contiguous, the cache's dtype) at (pages[i], slots[i]) on the device."""
+        rc = lib().acorn_kv_scatter(
+            ptr(k), ptr(v), ptr(self.k_pages[layer_idx]), ptr(self.v_pages[layer_idx]),
+            ptr(pages), ptr(slots), pages.shape[0], self.num_kv_heads, self.head_dim,
+            self.page_size, self.num_blocks, dtype_code(k), stream_ptr(self.device))
+        check(rc, op)
+
+    def _put(self, layer_idx: int, rows: torch.Tensor, slots: torch.Tensor, k: torch.Tensor,
+             v: torch.Tensor) -> None:
+        """k, v [s, KV, D] at (rows[i], slots[i])."""
+        self.k_pages[layer_idx][rows, slots] = k.to(self.dtype)
+        self.v_pages[layer_idx][rows, slots] = v.to(self.dtype)
+
     def scatter_decode(self, views: list["PagedCacheView"], layer_idx: int, k: torch.Tensor,
                        v: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor) -> None:
         """Decode-step batched write (pager.py:87-113): k_pages[l][pages[b], slots[b]] =
@@ -134,11 +159,7 @@ class PagedKVCache:
         vc = v.to(self.dtype).contiguous()
         pg = pages.to(device=self.device, dtype=torch.int64).contiguous()
         sl = slots.to(device=self.device, dtype=torch.int64).contiguous()
-        rc = lib().acorn_kv_scatter(
-            ptr(kc), ptr(vc), ptr(self.k_pages[layer_idx]), ptr(self.v_pages[layer_idx]),
-            ptr(pg), ptr(sl), B, self.num_kv_heads, self.head_dim, self.page_size,
-            self.num_blocks, dtype_code(kc), stream_ptr(self.device))
-        check(rc, "scatter_decode")
+        self._scatter(layer_idx, kc, vc, pg, sl, "scatter_decode")
         for view in views:
             view._lens[layer_idx] = view._lens.get(layer_idx, 0) + 1
 
@@ -161,13 +182,45 @@ class PagedKVCache:
         vc = v.permute(0, 2, 1, 3).reshape(B * m, v.shape[1], v.shape[3]).to(self.dtype).contiguous()
         pg = pages.reshape(-1).to(device=self.device, dtype=torch.int64).contiguous()
         sl = slots.reshape(-1).to(device=self.device, dtype=torch.int64).contiguous()
-        rc = lib().acorn_kv_scatter(
-            ptr(kc), ptr(vc), ptr(self.k_pages[layer_idx]), ptr(self.v_pages[layer_idx]),
-            ptr(pg), ptr(sl), B * m, self.num_kv_heads, self.head_dim, self.page_size,
-            self.num_blocks, dtype_code(kc), stream_ptr(self.device))
-        check(rc, "scatter_verify")
+        self._scatter(layer_idx, kc, vc, pg, sl, "scatter_verify")
         for view in views:
             view._lens[layer_idx] = view._lens.get(layer_idx, 0) + m
+
+
+class PagedKV8Cache(PagedKVCache):
+    """The cache in 8 bits: per layer a KV8Pages (`pages[l]`), views of one pool of K tiles, one
+    of V tiles and one of scale codes. `dtype` is the activations' (bf16, or fp16): rows are
+    rounded to it before they are quantised, and what is read back has it."""
+
+    def _allocate(self) -> None:
+        if not kv8_supported(self.head_dim, self.page_size) or \
+                self.dtype not in (torch.bfloat16, torch.float16):
+            raise NotImplementedError(f"8-bit cache: head_dim {self.head_dim}, page_size "
+                                      f"{self.page_size}, {self.dtype}")
+        shape = (self.num_layers, self.num_blocks, self.num_kv_heads, self.page_size // GROUP)
+        self.k_pool, self.v_pool, self.scale_pool = (
+            torch.zeros(*shape, n, device=self.device, dtype=torch.uint8)
+            for n in (GROUP * self.head_dim, GROUP * self.head_dim, 2 * GROUP))
+        self.pages = [KV8Pages(self.k_pool[i], self.v_pool[i], self.scale_pool[i])
+                      for i in range(self.num_layers)]
+        self.k_pages = [p.k for p in self.pages]
+        self.v_pages = [p.v for p in self.pages]
+
+    def _scatter(self, layer_idx, k, v, pages, slots, op) -> None:
+        n, KV, D = pages.shape[0], self.num_kv_heads, self.head_dim
+        kv8_scatter(k.view(n, KV, D), v.view(n, KV, D), self.pages[layer_idx], pages, slots)
+
+    def _put(self, layer_idx, rows, slots, k, v) -> None:
+        kv8_scatter(k.to(self.dtype), v.to(self.dtype), self.pages[layer_idx], rows, slots)
+
+    def read(self, layer_idx: int, view: "PagedCacheView") -> tuple[torch.Tensor, torch.Tensor]:
+        """A sequence's K and V [1, KV, seq_len, D] in the activations' dtype."""
+        n = view._lens.get(layer_idx, 0)
+        meta = torch.tensor([[0], [0], [n]], device=self.device, dtype=torch.int32)
+        tab = torch.tensor([view.table or [0]], device=self.device, dtype=torch.int32)
+        k, v = kv8_gather(self.pages[layer_idx], tab, meta[0], meta[1], meta[2], n, n,
+                          dtype=self.dtype)
+        return k.permute(1, 0, 2)[None], v.permute(1, 0, 2)[None]
 
 
 class PagedCacheView:
@@ -199,8 +252,7 @@ class PagedCacheView:
                             device=c.device, dtype=torch.long)
         slots = torch.tensor([p % c.page_size for p in positions],
                              device=c.device, dtype=torch.long)
-        c.k_pages[layer_idx][rows, slots] = k_new[0].permute(1, 0, 2).to(c.dtype)
-        c.v_pages[layer_idx][rows, slots] = v_new[0].permute(1, 0, 2).to(c.dtype)
+        c._put(layer_idx, rows, slots, k_new[0].permute(1, 0, 2), v_new[0].permute(1, 0, 2))
         self._lens[layer_idx] = base + s
 
     def reserve(self, n: int) -> list[tuple[int, int]]:
@@ -245,6 +297,8 @@ class PagedCacheView:
                ) -> tuple[torch.Tensor, torch.Tensor]:
         """write + gather the full [1, KV, seq_len, D] K and V."""
         self.write(layer_idx, k_new, v_new)
+        if self.cache.scale_pool is not None:
+            return self.cache.read(layer_idx, self)
         return (self._gather(layer_idx, self.cache.k_pages),
                 self._gather(layer_idx, self.cache.v_pages))
 

@@ -20,7 +20,8 @@ from dataclasses import dataclass
 
 import torch
 
-from acorninfer_amd.cache.pager import BlockAllocator, PagedCacheView, PagedKVCache
+from acorninfer_amd.cache.pager import (BlockAllocator, PagedCacheView, PagedKV8Cache,
+                                        PagedKVCache)
 from acorninfer_amd.engine.graph_runner import BUCKETS, DecodeGraphRunner
 from acorninfer_amd.engine.scheduler import Scheduler
 from acorninfer_amd.engine.sequence import RequestStatus, Sequence
@@ -42,7 +43,11 @@ class Engine:
     def __init__(self, model: Qwen3DecodeModel, *, num_blocks: int = 1024, page_size: int = 16,
                  max_running: int = 8, watermark_blocks: int = 8,
                  chunked_budget: int | None = None, max_model_len: int = 4096,
-                 capture: bool = True, seed: int = 0):
+                 capture: bool = True, seed: int = 0, kv_format: str = "16bit"):
+        """kv_format: "16bit" keeps the cache in the activations' dtype, "8bit" in
+        PagedKV8Cache."""
+        if kv_format not in ("16bit", "8bit"):
+            raise ValueError(f"kv_format must be '16bit' or '8bit', not {kv_format!r}")
         if watermark_blocks >= num_blocks:
             raise ValueError(f"watermark_blocks ({watermark_blocks}) must be < num_blocks "
                              f"({num_blocks})")
@@ -53,8 +58,10 @@ class Engine:
         self.model = model
         self.page_size = page_size
         self.allocator = BlockAllocator(num_blocks)
-        self.cache = PagedKVCache(cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim,
-                                  page_size, self.allocator, model.device, model.dtype)
+        make = PagedKV8Cache if kv_format == "8bit" else PagedKVCache
+        self.cache = make(cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim,
+                          page_size, self.allocator, model.device, model.dtype)
+        model.kv8_page(self.cache)               # refuses a model it is not built for
         self.scheduler = Scheduler(self.allocator, page_size, max_running, watermark_blocks,
                                    chunked_budget)
         # the runner keeps one resident block (the padding rows' KV target)

@@ -76,7 +76,7 @@ class DecodeGraphRunner:
         return st
 
     def _build(self, bk: int) -> _Bucket:
-        buf = self.model.buffers(bk, self.max_pages)
+        buf = self.model.buffers(bk, self.max_pages, kv8_page=self.model.kv8_page(self.cache))
         W = self.max_pages
         e64, e32, ef = buf.meta_ends
         pin, pin_i64, pin_i32, pin_f32 = [], [], [], []
@@ -102,7 +102,8 @@ class DecodeGraphRunner:
     def _body(self, st: _Bucket) -> None:
         c = self.cache
         # the sampler writes the next ids over buf.ids (device-fed decode_loop)
-        self.model.step(st.buf, c.k_pool, c.v_pool, c.num_blocks, c.page_size)
+        self.model.step(st.buf, c.k_pool, c.v_pool, c.num_blocks, c.page_size,
+                        scale_pool=getattr(c, "scale_pool", None))
 
     def _capture(self, st: _Bucket) -> None:
         s = torch.cuda.Stream(self.device)

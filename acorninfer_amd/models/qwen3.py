@@ -41,6 +41,7 @@ from acorninfer_amd._lib import (BF16, WFMT_BF16, WFMT_BF16B, WFMT_W4, WFMT_W4B,
                                  check,
                                  dtype_code, lib, ptr, stream_ptr)
 from acorninfer_amd.config import Qwen3Config
+from acorninfer_amd.ops.kv8 import kv8_attention_supported, kv8_splits, prefill_workspace_kv8
 from acorninfer_amd.ops.paged_attention import prefill_supported, prefill_workspace
 from acorninfer_amd.quant import quantize as Q
 from acorninfer_amd.sampler import sample_workspace
@@ -502,16 +503,36 @@ class Qwen3DecodeModel:
 
     # ------------------------------------------------------------------ decode --
     def buffers(self, batch: int, max_pages: int, num_splits: int | None = None,
-                tilings: dict | None = None, *, prefill: bool = False) -> "StepBuffers":
+                tilings: dict | None = None, *, prefill: bool = False,
+                kv8_page: int = 0) -> "StepBuffers":
         return StepBuffers(self, batch, max_pages, num_splits,
                            tilings if tilings is not None else self.tilings.get(batch),
-                           prefill=prefill)
+                           prefill=prefill, kv8_page=kv8_page)
+
+    def kv8_page(self, cache) -> int:
+        """StepBuffers.kv8_page for steps over `cache`: its page size where it is an 8-bit one
+        (NotImplementedError for a model whose attention it is not built for), else 0."""
+        if getattr(cache, "scale_pool", None) is None:
+            return 0
+        cfg = self.cfg
+        if cache.dtype != self.dtype or not kv8_attention_supported(
+                self.dtype, cfg.head_dim, cache.page_size, cfg.num_attention_heads,
+                cfg.num_key_value_heads):
+            raise NotImplementedError(
+                f"8-bit cache of {cache.dtype} under a model in {self.dtype} with head_dim "
+                f"{cfg.head_dim}, {cfg.num_attention_heads} / {cfg.num_key_value_heads} heads")
+        return cache.page_size
 
     def step(self, buf: "StepBuffers", k_pool: torch.Tensor, v_pool: torch.Tensor,
              num_blocks: int, page_size: int, *, fused_attn: bool = True,
              head_rows: torch.Tensor | None = None,
-             segments: "PrefillSegments | None" = None) -> torch.Tensor | None:
+             segments: "PrefillSegments | None" = None,
+             scale_pool: torch.Tensor | None = None) -> torch.Tensor | None:
         """Launch one decode step on the current stream.
+
+        scale_pool: the pools are an 8-bit cache's (PagedKV8Cache); the qkv
+        epilogue then quantises the new k/v (acorn_qkv_epilogue_kv8) and
+        attention is the 8-bit cache's (a launch each).
 
         fused_attn=False keeps the qkv epilogue (which writes every row's new
         k/v) and K3 as two launches; rows that attend to each other's new
@@ -538,7 +559,8 @@ class Qwen3DecodeModel:
         dt = dtype_code(buf.x)
         wdt = dtype_code(self.norm)
         eps = float(cfg.rms_norm_eps)
-        layer_elems = num_blocks * page_size * nkv * D
+        layer_elems = num_blocks * page_size * nkv * D      # (bytes of an 8-bit cache's tiles)
+        kv8 = scale_pool is not None
         esz = k_pool.element_size()
         kbase, vbase = k_pool.data_ptr(), v_pool.data_ptr()
 
@@ -546,12 +568,13 @@ class Qwen3DecodeModel:
                                 dt, st), "embedding")
         # K3 runs the qkv epilogue itself where it supports the shape (one
         # launch fewer per layer, the same bits)
-        fused_attn = fused_attn and not buf.direct and bool(
+        fused_attn = fused_attn and not buf.direct and not kv8 and bool(
             L.acorn_paged_attention_qkv_supported(nq, nkv, D, page_size, buf.max_pages,
                                                   buf.num_splits, dt, wdt))
 
         # (one workspace for the layers' prefill attention, which run in order)
-        ws_attn = None if segments is None else prefill_workspace(
+        ws_attn = None if segments is None else (
+            prefill_workspace_kv8 if kv8 else prefill_workspace)(
             segments.count, B, segments.max_nq, nq, nkv, D, page_size, segments.tables.shape[1],
             self.device)
 
@@ -592,7 +615,29 @@ class Qwen3DecodeModel:
                               stream=st)
             kp = kbase + li * layer_elems * esz
             vp = vbase + li * layer_elems * esz
-            if fused_attn:
+            if kv8:
+                sc = scale_pool.data_ptr() + li * num_blocks * page_size * nkv * 2
+                check(L.acorn_qkv_epilogue_kv8(
+                    ptr(y_qkv) if buf.direct else ptr(buf.part_qkv),
+                    0 if buf.direct else cq.ksplit, ptr(buf.q), kp, vp, sc, ptr(buf.pages),
+                    ptr(buf.slots), B, nq, nkv, D, page_size, num_blocks, ptr(lw.q_norm),
+                    ptr(lw.k_norm), eps, ptr(buf.positions), ptr(self.inv_freq), dt, st),
+                    "qkv_epilogue_kv8")
+                if segments is not None:
+                    sg = segments
+                    check(L.acorn_paged_prefill_attention_kv8(
+                        ptr(buf.q), kp, vp, sc, ptr(sg.tables), ptr(sg.row0), ptr(sg.pos0),
+                        ptr(sg.nq), ptr(buf.attn), sg.count, B, sg.max_nq, nq, nkv, D,
+                        page_size, num_blocks, sg.tables.shape[1], float(self.scale), dt,
+                        ptr(ws_attn), 0 if ws_attn is None else ws_attn.numel(), st),
+                        "prefill attention kv8")
+                else:
+                    check(L.acorn_paged_attention_kv8(
+                        ptr(buf.q), kp, vp, sc, ptr(buf.tables), ptr(buf.lens), ptr(buf.attn),
+                        ptr(buf.ws_acc), ptr(buf.ws_ml), B, nq, nkv, D, page_size, num_blocks,
+                        buf.max_pages, buf.num_splits, float(self.scale), dt, st),
+                        "attention kv8")
+            elif fused_attn:
                 check(L.acorn_paged_attention_qkv(
                     ptr(buf.part_qkv), cq.ksplit, kp, vp, ptr(buf.pages), ptr(buf.slots),
                     ptr(buf.tables), ptr(buf.lens), ptr(buf.attn), ptr(buf.ws_acc),
@@ -914,14 +959,15 @@ class Qwen3DecodeModel:
                                         lens_override=[int(v.seq_len) + 1 for v in views])
         else:
             positions, tables, lens, (pages, slots) = prepared
-        buf = self.buffers(B, tables.shape[1])
+        buf = self.buffers(B, tables.shape[1], kv8_page=self.kv8_page(cache))
         buf.ids.copy_(input_ids.view(-1))
         buf.positions.copy_(positions)
         buf.pages.copy_(pages)
         buf.slots.copy_(slots)
         buf.lens.copy_(lens)
         buf.tables.copy_(tables)
-        self.step(buf, cache.k_pool, cache.v_pool, cache.num_blocks, cache.page_size)
+        self.step(buf, cache.k_pool, cache.v_pool, cache.num_blocks, cache.page_size,
+                  scale_pool=getattr(cache, "scale_pool", None))
         for v in views:
             for li in range(self.cfg.num_hidden_layers):
                 v._lens[li] = v._lens.get(li, 0) + 1
@@ -1009,7 +1055,8 @@ class Qwen3DecodeModel:
             Rb = r1 - r0
             # the step buffers of the last shape are kept (a prompt batch often repeats it)
             # (the prefill kernel reads per-sequence tables: no per-row table)
-            key = (Rb, 1 if tiled else W, self.prefill_gemm, self.prefill_direct)
+            kv8_page = self.kv8_page(cache)
+            key = (Rb, 1 if tiled else W, self.prefill_gemm, self.prefill_direct, kv8_page)
             cached = getattr(self, "_extend_buf", None)
             if cached is None or cached[0] != key:
                 self._extend_buf = None
@@ -1023,7 +1070,8 @@ class Qwen3DecodeModel:
                     lib_t = {n: lin.plan(Rb)[0] for n, lin in (
                         ("qkv", lw.qkv), ("o", lw.o), ("gate_up", lw.gate_up),
                         ("down", lw.down))}
-                self._extend_buf = (key, self.buffers(Rb, key[1], tilings=lib_t, prefill=True))
+                self._extend_buf = (key, self.buffers(Rb, key[1], tilings=lib_t, prefill=True,
+                                                       kv8_page=kv8_page))
             buf = self._extend_buf[1]
             buf.ids.copy_(ids_all[r0:r1])
             buf.positions.copy_(pos_all[r0:r1])
@@ -1040,7 +1088,8 @@ class Qwen3DecodeModel:
                         buf.tables[a - r0:b - r0].copy_(seq_tabs[i].expand(b - a, W))
             heads = last[(last >= r0) & (last < r1)] - r0
             outs.append(self.step(buf, cache.k_pool, cache.v_pool, cache.num_blocks, P,
-                                  fused_attn=False, head_rows=heads.to(dev), segments=segs))
+                                  fused_attn=False, head_rows=heads.to(dev), segments=segs,
+                                  scale_pool=getattr(cache, "scale_pool", None)))
         for v, n in zip(views, chunk_lens):
             for li in range(self.cfg.num_hidden_layers):
                 v._lens[li] = v._lens.get(li, 0) + n
@@ -1148,6 +1197,7 @@ class StepBuffers:
     tilings: dict | None = None       # name -> requested Tiling (0 fields = planner)
     cfgs: dict = field(default_factory=dict)
     prefill: bool = False             # prompt rows: no decode logits / lm_head workspace
+    kv8_page: int = 0                 # page size of the 8-bit cache the step reads; 0: 16 bits
 
     def __post_init__(self):
         m = self.model
@@ -1155,6 +1205,8 @@ class StepBuffers:
         B = self.batch
         H, D = cfg.hidden_size, cfg.head_dim
         nq, nkv, inter = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.intermediate_size
+        if self.num_splits is None and self.kv8_page:
+            self.num_splits = kv8_splits(B, nkv, self.max_pages, self.kv8_page)
         if self.num_splits is None:
             self.num_splits = attention_splits(B, nkv, self.max_pages,
                                                q_per_kv=1 if self.prefill else nq // nkv)

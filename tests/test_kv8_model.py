@@ -1,0 +1,215 @@
+"""The 8-bit cache in use: PagedKV8Cache, the model's prefill and decode steps over it, the graph
+runner and the Engine (kv_format="8bit")."""
+import pytest
+import torch
+
+from acorninfer_amd.cache.pager import BlockAllocator, PagedCacheView, PagedKV8Cache, PagedKVCache
+from acorninfer_amd.config import Qwen3Config
+from oracle.kv8_ref import Pool, attend, tolerance
+
+SEED = 20261111
+
+
+def _cache(layers, KV, D, P, blocks, dtype, device="cuda"):
+    alloc = BlockAllocator(blocks)
+    return alloc, PagedKV8Cache(layers, KV, D, P, alloc, device, dtype)
+
+
+# ---- CPU -------------------------------------------------------------------------------------
+
+
+def test_shapes_and_refusals_without_a_gpu():
+    alloc, c = _cache(3, 2, 64, 32, 7, torch.bfloat16, "cpu")
+    assert c.k_pool.shape == c.v_pool.shape == (3, 7, 2, 2, 1024)
+    assert c.scale_pool.shape == (3, 7, 2, 2, 32)
+    assert all(x.numel() * x.element_size() for x in c.pages[2])
+    held = sum(x.numel() for x in (c.k_pool, c.v_pool, c.scale_pool))
+    assert held == 3 * 7 * 32 * 2 * (2 * 64 + 2)
+    assert PagedKVCache(1, 2, 64, 16, BlockAllocator(1), "cpu", torch.float32).scale_pool is None
+    for D, P, dtype in ((16, 16, torch.bfloat16), (128, 8, torch.bfloat16), (128, 16, torch.float32)):
+        with pytest.raises(NotImplementedError):
+            _cache(1, 2, D, P, 2, dtype, "cpu")
+    k = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(IndexError):                    # host targets are checked as in 16 bits
+        c.scatter_decode([PagedCacheView(c)], 0, k, k, torch.tensor([9]), torch.tensor([0]))
+    with pytest.raises(AssertionError):
+        c.scatter_decode([PagedCacheView(c)], 0, k[..., :32], k, torch.tensor([0]), torch.tensor([0]))
+
+
+# ---- GPU -------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pager_writes_and_reads(dtype):
+    """write, scatter_decode, scatter_verify with a rollback, and what update reads back: the
+    oracle's values, in the layer written and no other."""
+    KV, D, P = 3, 128, 16
+    alloc, c = _cache(2, KV, D, P, 12, dtype)
+    g = torch.Generator().manual_seed(1)
+    view = PagedCacheView(c)
+    k, v = torch.randn(2, 60, KV, D, generator=g).to(dtype)
+
+    def rows(a, b):
+        return [x[a:b].permute(1, 0, 2)[None].cuda() for x in (k, v)]
+
+    view.write(1, *rows(0, 21))
+    pages, slots = (torch.tensor([x]) for x in view.ensure_append_capacity(1))
+    one = [x.transpose(0, 1).transpose(0, 1) for x in rows(21, 22)]
+    c.scatter_decode([view], 1, *one, pages, slots)
+    t = view.ensure_append_capacity_n(1, 5)
+    pages, slots = (torch.tensor([[x[i] for x in t]]) for i in (0, 1))
+    c.scatter_verify([view], 1, *rows(40, 45), pages, slots)
+    view.set_lens(1, 22)                               # rejected: written again
+    c.scatter_verify([view], 1, *rows(22, 27), pages, slots)
+    gk, gv = view.update(1, *rows(27, 60))
+    assert gk.shape == (1, KV, 60, D) and view._lens == {1: 60}
+    pool = Pool(4, KV, D, P)
+    at = torch.arange(60)
+    pool.put(k, v, at // P, at % P, dtype == torch.float16)
+    for got, want in zip((gk, gv), pool.values(range(4), range(60))):
+        assert torch.equal(got[0].permute(1, 0, 2).cpu(), want.to(dtype))
+    assert not c.k_pool[0].any() and not c.scale_pool[0].any()
+
+
+def _model(dtype, layers=2):
+    from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, random_state_dict
+    cfg = Qwen3Config.qwen3_0_6b().with_layers(layers)
+    sd = random_state_dict(cfg, seed=SEED, std=0.05, dtype=dtype)
+    return cfg, Qwen3DecodeModel.from_state_dict(cfg, sd, dtype=dtype, device="cuda")
+
+
+def _attention_of_the_last_layer(model, buf, cache, table, lens, rows):
+    """buf.attn, row by row, against 64-bit attention of buf.q over what the last layer's cache
+    holds."""
+    cfg = model.cfg
+    H, D = cfg.num_attention_heads, cfg.head_dim
+    pool = Pool.of(cache.pages[-1], cache.page_size)
+    q, out = buf.q.cpu(), buf.attn.view(-1, H, D).cpu()
+    for r in rows:
+        k, v = pool.values(table[r], range(lens[r]))
+        want, mean, big = attend(q[r], k, v)
+        err = (out[r].double() - want).abs()
+        assert (err <= tolerance(want, mean, big, model.dtype, lens[r])).all(), r
+
+
+@pytest.mark.gpu
+def test_prefill_then_decode_together():
+    """Packed prompts, a chunk more, then decode steps: after each the last layer's attention is
+    that of its q over the cache's rows, whose values lie within a rounding to 8 bits of what a
+    16-bit cache under the same model holds."""
+    cfg, model = _model(torch.bfloat16)
+    KV, D, P = cfg.num_key_value_heads, cfg.head_dim, 16
+    alloc, c8 = _cache(cfg.num_hidden_layers, KV, D, P, 40, torch.bfloat16)
+    alloc16 = BlockAllocator(40)
+    c16 = PagedKVCache(cfg.num_hidden_layers, KV, D, P, alloc16, "cuda", torch.bfloat16)
+    g = torch.Generator().manual_seed(3)
+    lens = [37, 5, 90]
+    ids = torch.randint(0, cfg.vocab_size, (3, 90), generator=g)
+    views, views16 = [PagedCacheView(c8) for _ in lens], [PagedCacheView(c16) for _ in lens]
+    a = model.forward_prefill_batch(ids, views, real_lens=lens)
+    buf = model._extend_buf[1]
+    assert a.shape == (3, cfg.vocab_size) and torch.isfinite(a).all() and buf.kv8_page == P
+    rows = [(n, p + 1) for n, L in enumerate(lens) for p in range(L)]
+    _attention_of_the_last_layer(model, buf, c8, [views[n].table for n, _ in rows], [L for _, L in rows],
+                                 list(range(0, sum(lens), 7)) + [sum(lens) - 1])
+    model.forward_prefill_batch(ids, views16, real_lens=lens)
+    # layer 0's rows are made of the same projection on either side: k is rounded to e4m3 from 32
+    # bits here, on the other side to bf16 four times (norm, two products, their sum: each 2^-8
+    # of a magnitude at most |a| + |b|); v once
+    for n, v8 in enumerate(views):
+        for got, pages, slack in zip(c8.read(0, v8), (c16.k_pages, c16.v_pages), (4, 1)):
+            want = views16[n]._gather(0, pages).double()
+            far = (got.double() - want).abs()
+            mag = want.abs() + want.roll(D // 2, -1).abs()
+            top = want.abs().amax(-1, keepdim=True)
+            assert (far <= 2.0 ** -4 * (want.abs() + slack * 2.0 ** -8 * mag) + slack * 2.0 ** -8 * mag
+                    + 2.0 ** -17 * top).all()
+    more = torch.randint(0, cfg.vocab_size, (3, 20), generator=g)
+    model.forward_extend(more, views, starts=lens, chunk_lens=[20, 1, 7])
+    lens = [lens[0] + 20, lens[1] + 1, lens[2] + 7]
+    assert [v.seq_len for v in views] == lens
+    for _ in range(3):
+        from acorninfer_amd.ops.paged_attention import build_tables
+        step_ids = torch.randint(0, cfg.vocab_size, (3, 1), generator=g).cuda()
+        made = []
+        keep = model.buffers
+        model.buffers = lambda *x, **y: made.append(keep(*x, **y)) or made[-1]
+        try:
+            logits = model.forward_decode(step_ids, views)
+        finally:
+            del model.buffers
+        lens = [n + 1 for n in lens]
+        assert torch.isfinite(logits).all() and [v.seq_len for v in views] == lens
+        _attention_of_the_last_layer(model, made[0], c8, [v.table for v in views], lens, range(3))
+    for v in views:
+        for b in v.table:
+            alloc.free(b)
+    alloc.assert_balanced()
+
+
+@pytest.mark.gpu
+def test_captured_steps_equal_eager_ones():
+    """Replays of the captured step, with eager work between them, give the eager runner's tokens
+    and logits bit for bit; padding rows leave the other blocks alone."""
+    from types import SimpleNamespace
+    from acorninfer_amd.engine.graph_runner import DecodeGraphRunner
+    cfg, model = _model(torch.bfloat16)
+    outs = []
+    for capture in (True, False):
+        alloc, c = _cache(cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim, 16, 24,
+                          torch.bfloat16)
+        runner = DecodeGraphRunner(model, c, alloc, max_model_len=96, capture=capture, buckets=(4,))
+        views = [PagedCacheView(c) for _ in range(3)]
+        seqs = [SimpleNamespace(generated_ids=[i + 5]) for i in range(3)]
+        trace = []
+        for _ in range(20):
+            toks = runner.decode_batch(seqs, views)
+            for s, t in zip(seqs, toks):
+                s.generated_ids.append(t)
+            trace.append((toks, runner.last_logits[:3].clone()))
+            torch.randn(100, device="cuda").sum().item()
+        outs.append((trace, c))
+    for (ta, la), (tb, lb) in zip(outs[0][0], outs[1][0]):
+        assert ta == tb and torch.equal(la, lb)
+    for a, b in zip(outs[0][1].pages, outs[1][1].pages):
+        for x, y in zip(a, b):
+            assert torch.equal(x[:-1], y[:-1])         # (the last block holds padding)
+
+
+@pytest.mark.gpu
+def test_engine_runs_on_the_8_bit_cache():
+    """Requests of different lengths through chunked prefill, preemption and the captured step, to
+    their end, and no block left behind."""
+    from acorninfer_amd.engine.engine import Engine
+    from acorninfer_amd.sampler import SamplingParams
+    cfg, model = _model(torch.bfloat16)
+    eng = Engine(model, num_blocks=20, max_running=3, watermark_blocks=1, chunked_budget=16,
+                 max_model_len=128, kv_format="8bit")
+    assert isinstance(eng.cache, PagedKV8Cache)
+    g = torch.Generator().manual_seed(4)
+    ids = [eng.submit(torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist(),
+                      SamplingParams(temperature=t), max_tokens=m, eos_ids=frozenset({-1}))
+           for n, m, t in ((5, 40, 0.0), (37, 30, 0.0), (16, 50, 0.7), (60, 4, 0.0), (2, 30, 0.0))]
+    steps = 0
+    while eng.has_pending():
+        eng.step()
+        steps += 1
+        assert steps < 800
+    for i, m in zip(ids, (40, 30, 50, 4, 30)):
+        assert eng.seqs[i].stop_reason == "length" and len(eng.seqs[i].generated_ids) == m
+        eng.drop(i)
+    eng.assert_balanced()
+
+
+@pytest.mark.gpu
+def test_models_it_is_not_built_for_are_refused():
+    from acorninfer_amd.engine.engine import Engine
+    cfg, model = _model(torch.float32, layers=1)
+    with pytest.raises(NotImplementedError):
+        Engine(model, num_blocks=20, kv_format="8bit")
+    with pytest.raises(ValueError):
+        Engine(model, num_blocks=20, kv_format="fp8")
+    _, c = _cache(1, cfg.num_key_value_heads, cfg.head_dim, 16, 4, torch.bfloat16)
+    with pytest.raises(NotImplementedError):
+        model.forward_decode(torch.zeros(1, 1, dtype=torch.int64, device="cuda"), [PagedCacheView(c)])

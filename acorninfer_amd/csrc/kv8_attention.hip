@@ -54,9 +54,14 @@ __device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum
 //  * O^T += V^T P^T on v_mfma_f32_16x16x32: B = the p of lane (r, c) as they
 //    stand (tokens 4 r .. 4 r + 3 of both groups); A = V^T, from the E dims of
 //    those tokens that the lane has loaded and converted, transposed by v_perm.
-// The wave's block ids are fetched two steps ahead of their tiles, DEPTH steps
+// The wave's block ids are fetched one step ahead of their tiles, DEPTH steps
 // of tiles are in flight. Loads are unconditional (wait counts stay static):
 // those past the wave's last group read one line of it.
+// Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 110 us, 5.15
+// TB/s; one of 131000, 16 / 8 heads, 47.8 us, 5.65 TB/s (a large read reaches about
+// 5.5 with the default policy; non-temporal loads, whole lines read once, are worth a
+// tenth here: 119.7 and 53.8 us without). Three steps in flight or four waves per
+// workgroup change nothing; held to 128 registers for four waves per SIMD, 185 us.
 template <typename T, int D, int REP, int NWV, int DEPTH>
 __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ k_tiles,
@@ -315,7 +320,7 @@ struct DecodeArgs {
 };
 
 // Splits of at most this many groups of 16 tokens run as one wave, longer ones
-// as eight.
+// as eight (the split rule and what it measured: ops/kv8.py).
 constexpr int64_t kOneWaveGroups = 16;
 constexpr int kWaves = 8;
 

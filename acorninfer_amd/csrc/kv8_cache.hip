@@ -3,7 +3,9 @@
 //   acorn_qkv_epilogue_kv8  the qkv projection's output -> q, and k, v into the cache
 //   acorn_kv8_gather        rows of sequences out of it
 // All three are bound by memory: per (token, kv head) D values of k and of v on
-// one side and 2 D + 2 bytes on the other.
+// one side and 2 D + 2 bytes on the other. 8 kv heads of 128: 7013 tokens written from
+// fp16 9.4 us, 4.6 TB/s; 28535 tokens read into bf16 29.7 us, 5.9 TB/s; 8 tokens
+// written, or 333 read, 3 us, the latency of a launch and two dependent loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,6 +26,8 @@ __device__ __forceinline__ void load_row(const T* p, float (&f)[E]) {
   for (int i = 0; i < E; ++i) f[i] = to_f32(r[i]);
 }
 
+// 16 lanes per (row, head), the workgroup 16 rows of one head: consecutive tokens, as a
+// rule one tile, whose lines one L2 then completes.
 template <typename T, int D>
 __global__ __launch_bounds__(kNT) void kv8_scatter_kernel(
     const T* __restrict__ k, const T* __restrict__ v, uint8_t* __restrict__ k_tiles,
@@ -120,6 +124,25 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// cos and sin of pos * f, within two units of the last place of 32 bits: the product
+// (exact in 64 bits) reduced to a quarter turn there (Cody and Waite), the rest in two
+// floats. The angle as a float would be off by up to 2^-12 at 8192 tokens, and k, which
+// is quantised from 32 bits, would fall on the other side of a border 2^-12 / 2^-4 as often.
+__device__ __forceinline__ void angle(int64_t pos, float f, float& c, float& s) {
+  const double a = (double)pos * (double)f;
+  const double n = __builtin_rint(a * 0.63661977236758134308);           // 2 / pi
+  const double r = __builtin_fma(n, -6.1232339957367660e-17,             // pi / 2 in two parts
+                                 __builtin_fma(n, -1.5707963267948966, a));
+  const float rh = (float)r, rl = (float)(r - (double)rh);
+  const float c0 = cosf(rh), s0 = sinf(rh);
+  const float cr = c0 - s0 * rl, sr = s0 + c0 * rl;
+  const int q = (int)((int64_t)n & 3);
+  c = q & 1 ? sr : cr;
+  s = q & 1 ? cr : sr;
+  if (q == 1 || q == 2) c = -c;
+  if (q >= 2) s = -s;
+}
+
 // The qkv projection's output of a token (H q heads, KV k heads, KV v heads of D
 // values: S fp32 planes that are added in order, or one plane of T) to
 //   q: per-head RMSNorm and RoPE, rounded to T once, and
@@ -128,9 +151,11 @@ __device__ __forceinline__ float row_sum(float v) {
 // follows the roundings of a 16-bit cache's path: here k would be rounded twice.
 // One workgroup per (token, part of its heads): 16 lanes per head, E dims each;
 // a lane's rotation partner, D / 2 dims away, is 8 lanes away. The angles are
-// the same for every head: the first D / 2 threads compute them into LDS, as
-// pos * inv_freq in two floats (the product's rounding error would be 2^-12 of
-// a turn's radian at 8192: as large as the rounding of q).
+// the same for every head: the first D / 2 threads compute them into LDS while
+// the first heads are on their way; after that a head is loaded while the one before
+// it is worked on. 5164 tokens in bf16, 32 / 8 heads: 27 us, 4.3 TB/s (a large copy:
+// 4.8); without the prefetch and with the angles once per 16 heads 32.8, with tokens
+// dealt to the XCDs one by one 29.2. 8 tokens, three planes: 4.4 us, latency.
 template <typename T, typename PT, int D>
 __global__ __launch_bounds__(kNT) void qkv_epilogue_kv8_kernel(
     const PT* __restrict__ part, int nsplit, T* __restrict__ q_out, uint8_t* __restrict__ k_tiles,
@@ -138,30 +163,17 @@ __global__ __launch_bounds__(kNT) void qkv_epilogue_kv8_kernel(
     const int64_t* __restrict__ pages, const int64_t* __restrict__ slots, int64_t batch, int H,
     int KV, int P, int64_t num_blocks, const T* __restrict__ q_w, const T* __restrict__ k_w,
     float eps, const int64_t* __restrict__ pos, const float* __restrict__ inv_freq, int units_per_wg) {
-  constexpr int E = D / 16, HALF = D / 2;
-  __shared__ float cs[HALF], sn[HALF];
-  const int64_t b = blockIdx.x;
+  constexpr int E = D / 16, HALF = D / 2, PER = kNT / 16;
+  __shared__ __align__(16) float cs[HALF], sn[HALF];
+  // Workgroups are dealt to the 8 XCDs round robin: 16 consecutive tokens, as a rule one
+  // tile's, to one of them, so that its L2 completes the tile's lines before they are written
+  // back (a token's pieces are 8 or 16 bytes of a line).
+  const unsigned bx = blockIdx.x, run = bx & ~127u;
+  const int64_t b = run + 128 <= gridDim.x ? run + (bx % 8) * 16 + bx % 128 / 8 : bx;
   const int c = threadIdx.x & 15;
   const size_t width = (size_t)(H + 2 * KV) * D, plane = (size_t)batch * width;
-  if (threadIdx.x < HALF) {
-    const float p = (float)pos[b], f = inv_freq[threadIdx.x];
-    const float hi = p * f, lo = __builtin_fmaf(p, f, -hi);
-    const float ch = cosf(hi), sh = sinf(hi);
-    cs[threadIdx.x] = ch - sh * lo;
-    sn[threadIdx.x] = sh + ch * lo;
-  }
-  const uint64_t page = (uint64_t)pages[b], slot = (uint64_t)slots[b];
-  float wq[E], wk[E];
-  load_row<T, E>(q_w + E * c, wq);
-  load_row<T, E>(k_w + E * c, wk);
-  __syncthreads();
-  float co[E], si[E];                              // of this lane's dims: y = x cos +- partner sin
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int d = (E * c + i) % HALF;
-    co[i] = cs[d];
-    si[i] = c < 8 ? -sn[d] : sn[d];
-  }
+  // units: the H q heads, then the KV kv heads (k and v)
+  const int u0 = blockIdx.y * units_per_wg, u1 = min(u0 + units_per_wg, H + KV);
   auto sum = [&](int head, float (&x)[E]) {
     const PT* src = part + (size_t)b * width + (size_t)head * D + E * c;
     load_row<PT, E>(src, x);
@@ -172,27 +184,43 @@ __global__ __launch_bounds__(kNT) void qkv_epilogue_kv8_kernel(
       for (int i = 0; i < E; ++i) x[i] += y[i];
     }
   };
-  auto norm_rope = [&](float (&x)[E], const float (&w)[E]) {
+  auto fetch = [&](int un, float (&x)[E], float (&v)[E]) {
+    const int u = min(un, u1 - 1);                 // (lanes without a unit repeat the last)
+    sum(u, x);
+    if (u >= H) sum(u + KV, v);
+  };
+  float x[E], v[E], xn[E], vn[E];
+  int un = u0 + (int)(threadIdx.x >> 4);
+  fetch(un, x, v);
+  const uint64_t page = (uint64_t)pages[b], slot = (uint64_t)slots[b];
+  float wq[E], wk[E];
+  load_row<T, E>(q_w + E * c, wq);
+  load_row<T, E>(k_w + E * c, wk);
+  if (threadIdx.x < HALF) angle(pos[b], inv_freq[threadIdx.x], cs[threadIdx.x], sn[threadIdx.x]);
+  __syncthreads();
+  float co[E], si[E];                              // of this lane's dims: y = x cos +- partner sin
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int d = (E * c) % HALF + i;
+    co[i] = cs[d];
+    si[i] = c < 8 ? -sn[d] : sn[d];
+  }
+  auto norm_rope = [&](float (&y)[E], const float (&w)[E]) {
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) ss += x[i] * x[i];
+    for (int i = 0; i < E; ++i) ss += y[i] * y[i];
     const float inv = 1.0f / sqrtf(row_sum(ss) / (float)D + eps);
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = x[i] * inv * w[i];
+    for (int i = 0; i < E; ++i) y[i] = y[i] * inv * w[i];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float y = __shfl_xor(x[i], 8);
-      x[i] = x[i] * co[i] + y * si[i];
+      const float z = __shfl_xor(y[i], 8);
+      y[i] = y[i] * co[i] + z * si[i];
     }
   };
-  // units: the H q heads, then the KV kv heads (k and v)
-  const int units = H + KV;
-  const int u0 = blockIdx.y * units_per_wg, u1 = min(u0 + units_per_wg, units);
-  for (int ub = u0; ub < u1; ub += kNT / 16) {
-    const int un = ub + (int)(threadIdx.x >> 4);
-    const int u = min(un, u1 - 1);                 // (lanes without a unit repeat the last)
-    float x[E];
-    sum(u, x);
+  for (int ub = u0; ub < u1; ub += PER) {
+    if (ub + PER < u1) fetch(un + PER, xn, vn);
+    const int u = min(un, u1 - 1);
     if (u < H) {
       norm_rope(x, wq);
       if (un < u1) {
@@ -203,8 +231,6 @@ __global__ __launch_bounds__(kNT) void qkv_epilogue_kv8_kernel(
                                                   E * sizeof(T)), o, sizeof(o));
       }
     } else {
-      float v[E];
-      sum(u + KV, v);
       norm_rope(x, wk);
       const int kvh = u - H;
       // a (page, slot) outside the pool is dropped rather than written
@@ -213,8 +239,18 @@ __global__ __launch_bounds__(kNT) void qkv_epilogue_kv8_kernel(
       kv8_store_row<D, std::is_same<T, _Float16>::value>(k_tiles, v_tiles, scales, on ? tile : 0,
                                                          (int)(slot % kKv8Group), on, c, x, v);
     }
+    un += PER;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      x[i] = xn[i];
+      v[i] = vn[i];
+    }
   }
 }
+
+// Token rows from which a workgroup takes all heads of its token (the angles once):
+// enough workgroups for every CU several times over.
+constexpr int64_t kRowsPerWorkgroup = 1024;
 
 int pool_shape(int64_t KV, int64_t D, int64_t P, int64_t num_blocks) {
   if (KV <= 0 || KV > 65535 || D <= 0 || P <= 0 || num_blocks <= 0 || num_blocks > 0x7fffffff)
@@ -265,7 +301,7 @@ int epilogue(const void* part, int64_t nsplit, void* q_out, void* kt, void* vt, 
              int64_t D, int64_t P, int64_t NB, const void* qw, const void* kw, float eps,
              const int64_t* pos, const float* inv_freq, hipStream_t st) {
   const int64_t units = H + KV;
-  const int64_t per = kNT / 16;
+  const int64_t per = batch >= kRowsPerWorkgroup ? units : kNT / 16;
   const dim3 grid((unsigned)batch, (unsigned)((units + per - 1) / per));
   auto kfn = D == 128 ? qkv_epilogue_kv8_kernel<T, PT, 128> : qkv_epilogue_kv8_kernel<T, PT, 64>;
   kfn<<<grid, dim3(kNT), 0, st>>>((const PT*)part, (int)std::max<int64_t>(nsplit, 1), (T*)q_out,

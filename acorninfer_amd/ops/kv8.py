@@ -249,13 +249,24 @@ def qkv_norm_rope_kv8(qkv: torch.Tensor, kv: KV8Pages, pages: torch.Tensor, slot
 
 def kv8_splits(batch: int, kv_heads: int, max_pages: int, page_size: int) -> int:
     """Splits of the cache's length for paged_decode_attention_kv8 over block tables max_pages
-    wide."""
-    groups = max_pages * (page_size // GROUP)
-    pairs = max(1, batch * kv_heads)
-    if groups <= 64 or pairs >= 4 * MI355X_CUS:
+    wide. The kernel runs splits of more than 16 groups of 16 tokens as workgroups of eight waves,
+    of which a CU holds one, and shorter ones as one wave; more than one split takes a second
+    launch (2 to 8 us). Measured on MI355X, 32 / 8 heads, us:
+    - (sequence, kv head) pairs that fill the CUs, or short tables: one split (64 sequences of
+      1024..8192 tokens 110, in 31 splits of one wave 116; one of 333 6.4, in 11 splits 7.3);
+    - else as many as make one round of eight-wave workgroups (one sequence of 131000, 16 / 8
+      heads: 32 splits 47.8, 64 49.8, 24 49.0; 16 of 4000: 2 splits 29.7, 3 33.5, 1 33.1),
+    - but one-wave splits where those would be short (one of 4000: 63 splits 8.9, 16 12.7) or fill
+      three quarters of the CUs or less (12 of 2000..8000: 31 splits 27.2, 2 35.1)."""
+    per = page_size // GROUP
+    groups, pairs = max_pages * per, max(1, batch * kv_heads)
+    if pairs >= MI355X_CUS or groups <= 32 or (groups <= 64 and pairs >= 64):
         return 1
-    unit = max(1, 16 // (page_size // GROUP))
-    return max(1, min(-(-max_pages // unit), 64))
+    S = MI355X_CUS // pairs
+    if groups > 16 * S and 4 * pairs * S > 3 * MI355X_CUS:
+        return S
+    unit = min(16, max(2, -(-groups // 64), -(-pairs * groups // 1024)))
+    return -(-max_pages // -(-unit // per))
 
 
 def kv8_workspace(batch: int, num_heads: int, head_dim: int, num_splits: int, device

@@ -463,39 +463,42 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
   // of tile x / D. K: dims 16 (x % D / 16) .. of token x % 16. V: the E dims of TP tokens
   // (kv8.h). A wave's pieces are of one kind and one tile (D and PCS are multiples of
   // 64), so the block ids are scalar loads. An iteration stages K of the step after V's.
-  u32x4_t stage[PPT];
-  uint32_t code[PPT];
+  struct Piece {
+    u32x4_t v;
+    uint32_t code;
+  };
+  Piece stage[PPT];
   size_t tl[PPT];
   const bool stages = 2 * PCS >= NT || wid * kWave < 2 * PCS;
   auto first = [&](int i) { return i * NT + wid * kWave; };     // the wave's first piece
   auto of_k = [&](int i) { return (i + 1) * NT <= PCS || (i * NT < PCS && first(i) < PCS); };
-  auto find = [&](int i, int step) {
+  auto find = [&](int i, int step) -> size_t {
     const int g = min(2 * step + (first(i) % PCS) / D, glast);
     const unsigned pg = (unsigned)trow[min(g >> gshift, table_stride - 1)];
     const size_t blk = pg < (unsigned)num_blocks ? pg : 0u;
-    tl[i] = ((blk * KV + kvh) << gshift) + (g & ((1 << gshift) - 1));
+    return ((blk * KV + kvh) << gshift) + (g & ((1 << gshift) - 1));
   };
-  auto load = [&](int i) {
+  auto load = [&](int i, size_t tile, Piece& pc_) {
     const int p = first(i) % D + lane;           // piece of the tile
-    const uint8_t* src = (of_k(i) ? k_tiles : v_tiles) + tl[i] * (16 * D);
-    const uint8_t* sb = scales + tl[i] * 32;
-    stage[i] = *(const u32x4_t*)(src + p * 16);
+    const uint8_t* src = (of_k(i) ? k_tiles : v_tiles) + tile * (16 * D);
+    const uint8_t* sb = scales + tile * 32;
+    pc_.v = *(const u32x4_t*)(src + p * 16);
     if (of_k(i)) {
-      code[i] = sb[p % 16];
+      pc_.code = sb[p % 16];
     } else if constexpr (TP == 2) {
-      code[i] = *(const uint16_t*)(sb + 16 + 4 * (p % 64 / 16) + 2 * (p / 64));
+      pc_.code = *(const uint16_t*)(sb + 16 + 4 * (p % 64 / 16) + 2 * (p / 64));
     } else {
-      code[i] = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
+      pc_.code = *(const uint32_t*)(sb + 16 + 4 * (p / 16));
     }
   };
-  auto store = [&](int i, int step, int buf, auto tail) {      // the pieces of `step`
+  auto store = [&](int i, Piece& pc_, int step, int buf, auto tail) {      // the pieces of `step`
     const int p = first(i) % D + lane;
     const int t0 = (first(i) % PCS) / D * kKv8Group;            // the tile's first row
     if (of_k(i)) {
-      const float f = kv8_scale(code[i]);
+      const float f = kv8_scale(pc_.code);
       uint8_t* dst = ks[buf] + (t0 + p % 16) * PITCH + p / 16 * 32;
-      *(u32x4_t*)dst = kv8_cvt8<T>(stage[i][0], stage[i][1], f);
-      *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(stage[i][2], stage[i][3], f);
+      *(u32x4_t*)dst = kv8_cvt8<T>(pc_.v[0], pc_.v[1], f);
+      *(u32x4_t*)(dst + 16) = kv8_cvt8<T>(pc_.v[2], pc_.v[3], f);
     } else {
       const int t = t0 + 4 * (p % 64 / 16) + TP * (p / 64);
       uint8_t* dst = vs[buf] + t * PITCH + p % 16 * (2 * E);
@@ -504,20 +507,20 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
         for (int j = 0; j < TP; ++j)
 #pragma unroll
           for (int w = 0; w < E / 4; ++w)
-            stage[i][E / 4 * j + w] = step * KC + t + j < L ? stage[i][E / 4 * j + w] : 0u;
+            pc_.v[E / 4 * j + w] = step * KC + t + j < L ? pc_.v[E / 4 * j + w] : 0u;
       }
 #pragma unroll
       for (int j = 0; j < TP; ++j) {
-        const float f = kv8_scale_finite(code[i] >> (8 * j) & 0xFFu);
+        const float f = kv8_scale_finite(pc_.code >> (8 * j) & 0xFFu);
         if constexpr (TP == 2)
-          *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(stage[i][2 * j], stage[i][2 * j + 1], f);
+          *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(pc_.v[2 * j], pc_.v[2 * j + 1], f);
         else
           *(u32x2_t*)(dst + j * PITCH) =
-              u32x2_t{kv8_cvt2<T, false>(stage[i][j], f), kv8_cvt2<T, true>(stage[i][j], f)};
+              u32x2_t{kv8_cvt2<T, false>(pc_.v[j], f), kv8_cvt2<T, true>(pc_.v[j], f)};
       }
     }
   };
-  // the step that piece i belongs to in iteration s, and a step's clamp
+  // the step that piece i belongs to in iteration s
   auto step_of = [&](int i, int s) { return of_k(i) ? s + 2 : s; };
 
   float m[QW], nm[QW];                           // nm: -m (0 while m is -inf)
@@ -625,24 +628,32 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     }
   };
 
-  // prologue: K of steps s0 and s0 + 1 staged, the pieces of iteration s0 in flight; as V of
-  // step s0 - 1, which the first iteration multiplies by P = 0, that of s0
-#pragma unroll
-  for (int d = -2; d <= 0; ++d) {
+  // prologue, one round trip to memory: K of steps s0 and s0 + 1 staged, the pieces of
+  // iteration s0 (K of s0 + 2, V of s0) in flight; as V of step s0 - 1, which the first
+  // iteration multiplies by P = 0, that of s0
+  {
+    Piece ka[PPT], kb[PPT];
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
-      if (stages && (d == 0 || of_k(i))) {
-        find(i, step_of(i, s0 + d));
-        load(i);
+      if (stages) {
+        if (of_k(i)) {
+          load(i, find(i, s0), ka[i]);
+          load(i, find(i, s0 + 1), kb[i]);
+        }
+        load(i, find(i, step_of(i, s0)), stage[i]);
       }
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
-      if (stages && of_k(i) == (d < 0))
-        store(i, step_of(i, s0 + d), (of_k(i) ? s0 + d : s0 - 1) & 1, std::true_type{});
+      if (stages) {
+        tl[i] = find(i, step_of(i, s0 + 1));
+        if (of_k(i)) {
+          store(i, ka[i], s0, s0 & 1, std::true_type{});
+          store(i, kb[i], s0 + 1, (s0 + 1) & 1, std::true_type{});
+        } else {
+          store(i, stage[i], s0, (s0 - 1) & 1, std::true_type{});
+        }
+      }
   }
-#pragma unroll
-  for (int i = 0; i < PPT; ++i)
-    if (stages) find(i, step_of(i, s0 + 1));
   __syncthreads();
   read_k(s0);
   scores();
@@ -671,9 +682,9 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
       if (stages) {
-        store(i, step_of(i, s), s & 1, masked);
-        load(i);                                 // of iteration s + 1
-        find(i, step_of(i, s + 2));
+        store(i, stage[i], step_of(i, s), s & 1, masked);
+        load(i, tl[i], stage[i]);                // of iteration s + 1
+        tl[i] = find(i, step_of(i, s + 2));
       }
     // (without this the probabilities' work, next needed in the iteration to come, would sink
     // behind settle's branch, away from the MFMAs)
@@ -790,7 +801,7 @@ int attn_shape(int64_t N, int64_t H, int64_t KV, int64_t D, int64_t P, int64_t n
   if (N < 0 || N > 65535 || H <= 0 || KV <= 0 || KV > 65535 || H % KV != 0 || D <= 0 || P <= 0 ||
       num_blocks <= 0 || num_blocks > 0x7fffffff || table_stride < 1)
     return ACORN_ERR_SHAPE;
-  if ((P & (P - 1)) != 0 || P % kKv8Group != 0 || P > 65536 || table_stride > 0x7fffffff / P - 1)
+  if ((P & (P - 1)) != 0 || P % kKv8Group != 0 || P > 65536 || table_stride > 0x7fffffff / P - 8)
     return ACORN_ERR_SHAPE;
   const int64_t rep = H / KV;
   if ((D != 64 && D != 128) || !(rep == 1 || rep == 2 || rep == 4 || rep == 8))

@@ -57,11 +57,11 @@ __device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum
 // The wave's block ids are fetched one step ahead of their tiles, DEPTH steps
 // of tiles are in flight. Loads are unconditional (wait counts stay static):
 // those past the wave's last group read one line of it.
-// Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 110 us, 5.15
-// TB/s; one of 131000, 16 / 8 heads, 47.8 us, 5.65 TB/s (a large read reaches about
-// 5.5 with the default policy; non-temporal loads, whole lines read once, are worth a
-// tenth here: 119.7 and 53.8 us without). Three steps in flight or four waves per
-// workgroup change nothing; held to 128 registers for four waves per SIMD, 185 us.
+// Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 104 us, 5.4
+// TB/s; one of 131000, 16 / 8 heads, 47.8 us, 5.65 TB/s (a large copy: 4.8). In one
+// sweep, where the first took 111: with default instead of non-temporal loads 120, three
+// steps in flight 111, four waves per workgroup 109 to 117 by splits, 128 registers for four
+// waves per SIMD 185.
 template <typename T, int D, int REP, int NWV, int DEPTH>
 __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ k_tiles,
@@ -850,7 +850,7 @@ extern "C" int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t m
   if (!bytes) return ACORN_ERR_VALUE;
   *bytes = N == 0 || R == 0 || max_nq == 0
                ? 0
-               : prefill_plan(N, R, max_nq, H, KV, D, P, table_stride).ws_bytes;
+               : prefill_plan(N, R, std::min(max_nq, R), H, KV, D, P, table_stride).ws_bytes;
   return ACORN_OK;
 }
 
@@ -868,6 +868,7 @@ extern "C" int acorn_paged_prefill_attention_kv8(
     return ACORN_ERR_VALUE;
   if (!seq_nq && R != N * max_nq) return ACORN_ERR_SHAPE;
   if (!aligned16({q, k_tiles, v_tiles, scales, out, ws})) return ACORN_ERR_VALUE;
+  max_nq = std::min(max_nq, R);                // a bound far above the rows there are costs nothing
   PrefillArgs a{q, k_tiles, v_tiles, scales, tables, seq_row0, seq_pos0, seq_nq, out, N, R, max_nq,
                 H, KV, P, num_blocks, table_stride, scale,
                 prefill_plan(N, R, max_nq, H, KV, D, P, table_stride), (float*)ws,

@@ -357,6 +357,7 @@ extern "C" int acorn_kv8_gather(const void* k_tiles, const void* v_tiles, const 
     return ACORN_ERR_VALUE;
   if (!tiles_ok(k_tiles, v_tiles, scales) || (uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
     return ACORN_ERR_VALUE;
+  max_nq = std::min(max_nq, R);                // a bound far above the rows there are costs nothing
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
     case ACORN_F32: return gather<float>(k_tiles, v_tiles, scales, tables, seq_row0, seq_pos0, seq_nq, k_out, v_out, N, R, max_nq, kv_heads, head_dim, page_size, num_blocks, table_stride, st);

@@ -29,6 +29,7 @@ from typing import NamedTuple
 
 import torch
 
+# (the stream's handle without a Stream object around it: a microsecond of a call's ten)
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from acorninfer_amd._lib import check, dtype_code, lib, ptr, require_gpu
@@ -264,7 +265,7 @@ def kv8_splits(batch: int, kv_heads: int, max_pages: int, page_size: int) -> int
         return 1
     S = MI355X_CUS // pairs
     if groups > 16 * S and 4 * pairs * S > 3 * MI355X_CUS:
-        return S
+        return min(S, max_pages)
     unit = min(16, max(2, -(-groups // 64), -(-pairs * groups // 1024)))
     return -(-max_pages // -(-unit // per))
 

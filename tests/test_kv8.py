@@ -63,6 +63,16 @@ def test_split_rule(batch, kv, pages, P):
     assert 1 <= s <= max(1, pages)
 
 
+def test_split_rule_keeps_to_the_table():
+    """Whole pages of any size, and never more splits than pages."""
+    rule = _kv8().kv8_splits
+    for P in (16, 32, 1024, 65536):
+        for pages in (1, 2, 3, 31, 64, 65, 500, 9000):
+            for batch in (1, 2, 7, 12, 31, 33, 200):
+                for kv in (1, 5, 8):
+                    assert 1 <= rule(batch, kv, pages, P) <= pages, (batch, kv, pages, P)
+
+
 def test_shapes_supported():
     k = _kv8()
     assert k.kv8_supported(128, 16) and k.kv8_supported(64, 64)
@@ -629,6 +639,23 @@ def test_prefill_metadata_past_its_bounds():
             touched = [(int(m[0][k]), int(m[0][k]) + 30) for k in range(3) if k == i]
             if n != i and all(b <= lo or a >= hi for lo, hi in touched):
                 assert torch.equal(out[a:b], good[a:b]), (i, field, value, n)
+
+
+@gpu
+@pytest.mark.parametrize("pre", [0, 1500])
+def test_a_bound_on_the_rows_may_be_any_number(pre):
+    """max_nq far above the rows there are: the same rows, bit for bit, and the same read back."""
+    H, KV, D, P = 32, 8, 128, 16
+    kv, tables, q, meta = _prefill_case(H, KV, D, P, [(pre, 20), (0, 33)], torch.bfloat16, 78)
+    args = (tables.cuda(), *(m.cuda() for m in meta))
+    good = _kv8().paged_prefill_attention_kv8(q.cuda(), kv, *args, len(q), out=torch.zeros_like(q).cuda())
+    for bound in (len(q) + 1, 1 << 20, (1 << 31) - 1):
+        out = torch.zeros_like(q).cuda()
+        assert torch.equal(_kv8().paged_prefill_attention_kv8(q.cuda(), kv, *args, bound, out=out), good)
+    k0, v0 = _kv8().kv8_gather(kv, *args, 33, len(q))
+    k1, v1 = _kv8().kv8_gather(kv, *args, (1 << 31) - 40, len(q))
+    rows = torch.cat([torch.arange(int(a), int(a) + int(n)) for a, n in zip(meta[0], meta[2])]).cuda()
+    assert torch.equal(k0[rows], k1[rows]) and torch.equal(v0[rows], v1[rows])
 
 
 @gpu

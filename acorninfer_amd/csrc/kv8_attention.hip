@@ -49,8 +49,11 @@ __device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum
 //    past REP repeat the last head). Register i of lane (r, c) then holds the
 //    score of head c for token 4 r + i.
 //  * online softmax in that layout, the maximum moved only by scores that
-//    exceed it by more than kMaxSlack; p rounded to T and l the sum of the
-//    rounded values, so that the weights of the mean add up to 1.
+//    exceed it by more than kMaxSlack. In bf16 p goes through the MFMAs as two
+//    terms, p cut to bf16 and the rest, and l sums p itself: as near to 64 bits as
+//    the result's own rounding lets it be, and free beside the loads (with one term
+//    the error of a result is 1.4 times that rounding's). In fp16 p is rounded
+//    once, and l the sum of the rounded values.
 //  * O^T += V^T P^T on v_mfma_f32_16x16x32: B = the p of lane (r, c) as they
 //    stand (tokens 4 r .. 4 r + 3 of both groups); A = V^T, from the E dims of
 //    those tokens that the lane has loaded and converted, transposed by v_perm.
@@ -72,6 +75,7 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
   constexpr int E = D / 16;                    // dims per lane of V = MFMAs per P V
   constexpr int KP = D / 64;                   // 16-byte pieces per lane and tile, K or V
   constexpr int KB = D / 32;                   // q.k MFMAs per group
+  constexpr bool TWO = std::is_same<T, __bf16>::value;
   __shared__ __align__(16) float sacc[NWV == 1 ? 1 : NWV][REP][D];
   __shared__ float sm[NWV][REP], sl[NWV][REP];
 
@@ -177,10 +181,19 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
 #pragma unroll
       for (int j = 0; j < E; ++j) acc[j] *= alpha;
     }
-    u32x4_t pb;
+    u32x4_t pb, pr;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      pb[i] = pack_pair_sum<T>(__builtin_amdgcn_exp2f(x[2 * i] - m), __builtin_amdgcn_exp2f(x[2 * i + 1] - m), l);
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = __builtin_amdgcn_exp2f(x[2 * i] - m), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1] - m);
+      if constexpr (TWO) {
+        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+        pb[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        pr[i] = pack_pair<T>(p0 - __uint_as_float(b0 & 0xffff0000u), p1 - __uint_as_float(b1 & 0xffff0000u));
+        l += p0 + p1;
+      } else {
+        pb[i] = pack_pair_sum<T>(p0, p1, l);
+      }
+    }
     // V: token i of group u, E dims in E / 2 words
     uint32_t vt[2][4][E / 2];
 #pragma unroll
@@ -204,6 +217,7 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
                           __builtin_amdgcn_perm(vt[1][1][j / 2], vt[1][0][j / 2], sel),
                           __builtin_amdgcn_perm(vt[1][3][j / 2], vt[1][2][j / 2], sel)};
       acc[j] = mfma16x16x32<T>(va, pb, acc[j]);
+      if constexpr (TWO) acc[j] = mfma16x16x32<T>(va, pr, acc[j]);
     }
   };
 
@@ -323,6 +337,10 @@ struct DecodeArgs {
 // as eight (the split rule and what it measured: ops/kv8.py).
 constexpr int64_t kOneWaveGroups = 16;
 constexpr int kWaves = 8;
+// LDS that a one-wave workgroup asks for without using it, so that a CU holds eight of
+// them (two per SIMD) and not twelve: 12 sequences of 2000..8000 tokens 29 us against 32,
+// 22 of them 48 against 52; 16, 23 and 26 KB 1 to 2 us slower.
+constexpr size_t kOneWaveLds = 20 * 1024;
 
 template <typename T, int D, int REP>
 int launch_decode(const DecodeArgs& a) {
@@ -331,7 +349,8 @@ int launch_decode(const DecodeArgs& a) {
   float* ws_m = a.ws_ml;
   float* ws_l = a.ws_ml ? a.ws_ml + a.B * a.H * a.S : nullptr;
   auto kfn = one ? kv8_decode_kernel<T, D, REP, 1, 2> : kv8_decode_kernel<T, D, REP, kWaves, 2>;
-  kfn<<<dim3((unsigned)a.KV, (unsigned)a.S, (unsigned)a.B), dim3((one ? 1 : kWaves) * kWave), 0, a.st>>>(
+  kfn<<<dim3((unsigned)a.KV, (unsigned)a.S, (unsigned)a.B), dim3((one ? 1 : kWaves) * kWave),
+        one ? kOneWaveLds : 0, a.st>>>(
       (const T*)a.q, (const uint8_t*)a.kt, (const uint8_t*)a.vt, (const uint8_t*)a.sc, a.tables,
       a.lens, (T*)a.out, a.ws_acc, ws_m, ws_l, (int)a.H, (int)a.KV, (int)a.P, (int)a.num_blocks,
       (int)a.table_stride, (int)a.S, a.scale * kLog2e);

@@ -258,7 +258,7 @@ def kv8_splits(batch: int, kv_heads: int, max_pages: int, page_size: int) -> int
     - else as many as make one round of eight-wave workgroups (one sequence of 131000, 16 / 8
       heads: 32 splits 47.8, 64 49.8, 24 49.0; 16 of 4000: 2 splits 29.7, 3 33.5, 1 33.1),
     - but one-wave splits where those would be short (one of 4000: 63 splits 8.9, 16 12.7) or fill
-      three quarters of the CUs or less (12 of 2000..8000: 31 splits 27.2, 2 35.1)."""
+      three quarters of the CUs or less (12 of 2000..8000: 31 splits 29, 2 36)."""
     per = page_size // GROUP
     groups, pairs = max_pages * per, max(1, batch * kv_heads)
     if pairs >= MI355X_CUS or groups <= 32 or (groups <= 64 and pairs >= 64):

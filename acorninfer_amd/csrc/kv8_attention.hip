@@ -130,7 +130,9 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
       s.vs[u] = *(const uint32_t*)(sb + 16 + 4 * r);
     }
   };
-  float m = -INFINITY, l = 0.f;
+  // m starts at the least finite number: scores of -inf (a product past 32 bits) have no weight
+  // also where a wave begins with them
+  float m = -__FLT_MAX__, l = 0.f;
   f32x4_t acc[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -298,14 +300,14 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
   for (int e = threadIdx.x; e < REP * D; e += NWV * kWave) {
     const int h = e / D, d = e % D;
     // (a wave that saw a NaN score keeps m of its other scores and has l and acc NaN)
-    float M = -INFINITY;
+    float M = sm[0][h];
 #pragma unroll
-    for (int w = 0; w < NWV; ++w) M = fmaxf(M, sm[w][h]);
+    for (int w = 1; w < NWV; ++w) M = fmaxf(M, sm[w][h]);
     float num = 0.f, den = 0.f;
 #pragma unroll
     for (int w = 0; w < NWV; ++w) {
       // a wave without tokens has l = acc = 0
-      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w][h] - M);
+      const float f = __builtin_amdgcn_exp2f(sm[w][h] - M);
       num += f * sacc[w][h][d];
       den += f * sl[w][h];
     }

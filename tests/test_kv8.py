@@ -434,6 +434,35 @@ def test_decode_of_peaked_and_rising_scores(S):
 
 
 @gpu
+@pytest.mark.parametrize("lost", [(0, 64), (0, 470), (300, 600), (40, 41)])
+@pytest.mark.parametrize("S", [1, 3, 40, "prefill"])
+def test_scores_past_32_bits_have_no_weight(S, lost):
+    """Tokens whose products with q pass the least 32-bit number score -inf: the result is that
+    of the others, also where a wave, a split or a run of keys holds nothing else."""
+    H, KV, D, P, L = 8, 2, 128, 16, 600
+    kv, tables, g = _filled([L], KV, D, P, torch.bfloat16, 9)
+    at = torch.arange(*lost)
+    k = torch.zeros(len(at), KV, D)
+    k[:, :, 5] = -3e38
+    v = torch.randn(len(at), KV, D, generator=g)
+    _kv8().kv8_scatter(k.bfloat16().cuda(), v.bfloat16().cuda(), kv, tables[0].long()[at // P].cuda(),
+                       (at % P).cuda())
+    q = torch.randn(1, H, D, generator=g)
+    q[:, :, 5] = 8.0
+    q = q.bfloat16()
+    if S == "prefill":
+        meta = [torch.tensor([x], dtype=torch.int32).cuda() for x in (0, L - 1, 1)]
+        out = _kv8().paged_prefill_attention_kv8(q.cuda(), kv, tables.cuda(), *meta, 1)
+    else:
+        out = _kv8().paged_decode_attention_kv8(q.cuda(), kv, tables.cuda(),
+                                                torch.tensor([L], dtype=torch.int32).cuda(), S)
+    rest = [t for t in range(L) if not lost[0] <= t < lost[1]]
+    k, v = Pool.of(kv, P).values(tables[0], rest)
+    want, mean, big = attend(q[0], k, v)
+    assert ((out[0].cpu().double() - want).abs() <= tolerance(want, mean, big, torch.bfloat16, L)).all()
+
+
+@gpu
 @pytest.mark.parametrize("S", [1, 3, 40])
 def test_decode_of_nan_rows_and_of_no_tokens(S):
     """A NaN row makes its own sequence's heads NaN and nothing else; a sequence without tokens is

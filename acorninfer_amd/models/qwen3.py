@@ -521,6 +521,8 @@ class Qwen3DecodeModel:
             raise NotImplementedError(
                 f"8-bit cache of {cache.dtype} under a model in {self.dtype} with head_dim "
                 f"{cfg.head_dim}, {cfg.num_attention_heads} / {cfg.num_key_value_heads} heads")
+        if any(w.dtype != self.dtype for lw in self.layers for w in (lw.q_norm, lw.k_norm)):
+            raise NotImplementedError(f"8-bit cache: q and k norm weights that are not {self.dtype}")
         return cache.page_size
 
     def step(self, buf: "StepBuffers", k_pool: torch.Tensor, v_pool: torch.Tensor,

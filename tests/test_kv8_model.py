@@ -36,6 +36,22 @@ def test_shapes_and_refusals_without_a_gpu():
         c.scatter_decode([PagedCacheView(c)], 0, k[..., :32], k, torch.tensor([0]), torch.tensor([0]))
 
 
+def test_norm_weights_of_another_type_are_refused():
+    """The qkv epilogue reads q and k norm weights in the activations' type."""
+    from types import SimpleNamespace
+
+    from acorninfer_amd.models.qwen3 import Qwen3DecodeModel
+    cfg = Qwen3Config.qwen3_0_6b().with_layers(2)
+    _, c = _cache(2, cfg.num_key_value_heads, cfg.head_dim, 16, 2, torch.bfloat16, "cpu")
+    w = torch.ones(cfg.head_dim, dtype=torch.bfloat16)
+    model = SimpleNamespace(cfg=cfg, dtype=torch.bfloat16,
+                            layers=[SimpleNamespace(q_norm=w, k_norm=w) for _ in range(2)])
+    assert Qwen3DecodeModel.kv8_page(model, c) == 16
+    model.layers[1].k_norm = w.float()
+    with pytest.raises(NotImplementedError):
+        Qwen3DecodeModel.kv8_page(model, c)
+
+
 # ---- GPU -------------------------------------------------------------------------------------
 
 

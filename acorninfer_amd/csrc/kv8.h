@@ -15,8 +15,9 @@
 // codes 255, bytes 0. So the bytes of v are finite whatever was written, a
 // probability of 0 removes a row that a query must not see, and a query that
 // sees such a row gets NaN through its score.
-// fp16 values above 63456 in magnitude are taken as 63456 (held as 61440): the
-// next number of the grid, 65536, is not an fp16.
+// What is held stays finite when it is read: the largest number is 240 * 2^120
+// (the next of the grid, 2^128, is neither an fp32 nor a bf16), of fp16 rows
+// 240 * 2^8 = 61440 (65536 is not an fp16); greater magnitudes are held as it.
 //
 // Layout. A block holds P tokens (a multiple of 16) in groups of 16; per (block,
 // kv head, group) one K tile and one V tile of 16 D bytes, and 32 bytes of
@@ -41,7 +42,7 @@ typedef uint32_t kv8_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv8_u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kKv8Group = 16;                      // tokens of a tile
-constexpr float kKv8MaxF16 = 63456.f;
+constexpr float kKv8Max = 240.f * 0x1p120f, kKv8MaxF16 = 240.f * 0x1p8f;    // the largest numbers
 
 // Byte of (token t of the group, dim d) in a K tile and in a V tile.
 template <int D>
@@ -109,7 +110,7 @@ __device__ __forceinline__ uint32_t kv8_row_max(uint32_t v) {
 // Writes one (token, kv head) of the cache: the 16 lanes of a row hold E = D / 16
 // dims each of k and of v, dims E c .. . `tile` is the tile's number, t the
 // token in it; `on` false writes nothing (every lane takes part in the row's
-// maxima all the same). SAT: fp16 values.
+// maxima all the same). SAT: an fp16 cache.
 template <int D, bool SAT>
 __device__ __forceinline__ void kv8_store_row(uint8_t* k_tiles, uint8_t* v_tiles, uint8_t* scales,
                                               size_t tile, int t, bool on, int c,
@@ -126,8 +127,10 @@ __device__ __forceinline__ void kv8_store_row(uint8_t* k_tiles, uint8_t* v_tiles
   const bool nan = max(top[0], top[1]) >= 0x7F800000u;
 #pragma unroll
   for (int a = 0; a < 2; ++a) {
-    uint32_t m = top[a];
-    if (SAT) m = min(m, __float_as_uint(kKv8MaxF16));
+    // (a constant: with the limit in registers the qkv epilogue passes 96 of them, which
+    // takes a fifth of its waves and costs 5164 tokens 5 us)
+    constexpr float kMax = SAT ? kKv8MaxF16 : kKv8Max;
+    const uint32_t m = min(top[a], __float_as_uint(kMax));
     // 448 = 1.75 * 2^8
     uint32_t code = (uint32_t)max((int)(m >> 23) - 8 + ((m & 0x7FFFFFu) > 0x600000u ? 1 : 0), 1);
     const float inv = __uint_as_float((254u - code) << 23);      // 2^-e, e + 127 = code <= 247
@@ -136,11 +139,7 @@ __device__ __forceinline__ void kv8_store_row(uint8_t* k_tiles, uint8_t* v_tiles
     for (int i = 0; i < E / 4; ++i) {
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f = x[a][4 * i + j];
-        if (SAT) f = fminf(fmaxf(f, -kKv8MaxF16), kKv8MaxF16);
-        y[j] = f * inv;
-      }
+      for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_fmed3f(x[a][4 * i + j], -kMax, kMax) * inv;
       int b = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
       b = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], b, true);
       w[i] = nan ? 0u : (uint32_t)b;

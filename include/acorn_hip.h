@@ -464,9 +464,10 @@ int acorn_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes);
  *   k: b at (d/16)*256 + t*16 + d%16
  *   v, E = D/16, TP = 16/E: b at (t%4/TP)*1024 + (16*(t/4) + d/E)*16 + (t%TP)*E + d%E
  * A (token, kv head) whose k or v row holds an infinity or NaN is held as NaN (codes
- * 255, bytes 0). Memory of zeros is an empty cache. fp16 magnitudes above 63456 are
- * held as 61440, so that what is read is an fp16; a cache written from another type is
- * read in fp16 only where its values fit. No counterpart in the reference.
+ * 255, bytes 0). Memory of zeros is an empty cache. Magnitudes above 240 * 2^120 are held
+ * as that, written from fp16 those above 61440 = 240 * 2^8, so that what is read in the
+ * type that was written is finite; a cache written from another type is read in fp16 only
+ * where its values fit. No counterpart in the reference.
  *
  * acorn_kv8_scatter: rows k, v of `dtype` (any), row i, head h at k + i*k_row_stride +
  * h*k_head_stride (elements; each D/16 values aligned to their size or 16 bytes), are

@@ -35,8 +35,9 @@ def quantise_row(x: np.ndarray, fp16: bool) -> tuple[np.ndarray, int, bool]:
     """(bytes, code, whether the row is finite) of x [D] in 64 bits."""
     if not np.isfinite(x).all():
         return np.zeros(len(x), np.uint8), 255, False
-    if fp16:
-        x = np.clip(x, -63456.0, 63456.0)
+    # (what is held has to be finite when it is read: in fp16 2^16, else 2^128 is not)
+    top = 61440.0 if fp16 else math.ldexp(240.0, 120)
+    x = np.clip(x, -top, top)
     e = scale_exp(float(np.abs(x).max()))
     y = np.abs(x) * 2.0 ** -e if e > -1000 else x
     hi = np.clip(np.searchsorted(_POS, y), 0, 126)

@@ -2,8 +2,9 @@
 //   acorn_paged_attention_kv8          one new token per sequence, split over
 //                                      the cache's length and joined
 //   acorn_paged_prefill_attention_kv8  packed prompt rows, causal
-// Both turn bytes into bf16 / fp16 (exactly) and use the 16-bit MFMAs with fp32
-// sums. The fp8 MFMAs would take the bytes as they lie, with q in two or three
+// Both turn bytes into bf16 / fp16 and use the 16-bit MFMAs with fp32 sums. The
+// conversion is exact within the type's range: fp16 rounds what lies below 2^-14
+// to steps of 2^-24. The fp8 MFMAs would take the bytes as they lie, with q in two or three
 // e4m3 terms, but add their products to fewer bits: measured against 64 bits
 // 1.6e-5 of the sum of magnitudes for normal numbers, 2.8e-4 where one in
 // sixteen is a hundred times larger, 2e-8 with the bf16 MFMA.
@@ -25,19 +26,6 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   const f2 f = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, t2));
 }
-// ... and their sum added to `sum` after the rounding.
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum) {
-  typedef T t2 __attribute__((ext_vector_type(2)));
-  const uint32_t u = pack_pair<T>(lo, hi);
-  if constexpr (std::is_same<T, __bf16>::value)
-    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, u),
-                                          __builtin_bit_cast(t2, 0x3F803F80u), sum, false);
-  else
-    sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, u), __builtin_bit_cast(t2, 0x3C003C00u),
-                                 sum, false);
-  return u;
-}
 
 // ---------------------------------------------------------------------------
 // Decode. A workgroup of NWV waves serves one (split, kv head, sequence); its
@@ -49,11 +37,12 @@ __device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum
 //    past REP repeat the last head). Register i of lane (r, c) then holds the
 //    score of head c for token 4 r + i.
 //  * online softmax in that layout, the maximum moved only by scores that
-//    exceed it by more than kMaxSlack. In bf16 p goes through the MFMAs as two
-//    terms, p cut to bf16 and the rest, and l sums p itself: as near to 64 bits as
-//    the result's own rounding lets it be, and free beside the loads (with one term
-//    the error of a result is 1.4 times that rounding's). In fp16 p is rounded
-//    once, and l the sum of the rounded values.
+//    exceed it by more than kMaxSlack. p goes through the MFMAs as two bf16 terms, p
+//    cut to bf16 and the rest, and l sums p itself: as near to 64 bits as the
+//    result's own rounding lets it be, and free beside the loads (with one term the
+//    error of a result is 1.4 times that rounding's). V's bytes become bf16 for it, in
+//    fp16 too: exactly, and p has no least step (one fp16 term lost the weight of
+//    tokens 17.5 below the largest score, and half of it at 17).
 //  * O^T += V^T P^T on v_mfma_f32_16x16x32: B = the p of lane (r, c) as they
 //    stand (tokens 4 r .. 4 r + 3 of both groups); A = V^T, from the E dims of
 //    those tokens that the lane has loaded and converted, transposed by v_perm.
@@ -61,7 +50,7 @@ __device__ __forceinline__ uint32_t pack_pair_sum(float lo, float hi, float& sum
 // of tiles are in flight. Loads are unconditional (wait counts stay static):
 // those past the wave's last group read one line of it.
 // Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 104 us, 5.4
-// TB/s; one of 131000, 16 / 8 heads, 47.8 us, 5.65 TB/s (a large copy: 4.8). In one
+// TB/s; one of 131000, 16 / 8 heads, 48.5 us, 5.6 TB/s (a large copy: 4.8). In one
 // sweep, where the first took 111: with default instead of non-temporal loads 120, three
 // steps in flight 111, four waves per workgroup 109 to 117 by splits, 128 registers for four
 // waves per SIMD 185.
@@ -75,7 +64,6 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
   constexpr int E = D / 16;                    // dims per lane of V = MFMAs per P V
   constexpr int KP = D / 64;                   // 16-byte pieces per lane and tile, K or V
   constexpr int KB = D / 32;                   // q.k MFMAs per group
-  constexpr bool TWO = std::is_same<T, __bf16>::value;
   __shared__ __align__(16) float sacc[NWV == 1 ? 1 : NWV][REP][D];
   __shared__ float sm[NWV][REP], sl[NWV][REP];
 
@@ -187,14 +175,11 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float p0 = __builtin_amdgcn_exp2f(x[2 * i] - m), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1] - m);
-      if constexpr (TWO) {
-        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
-        pb[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-        pr[i] = pack_pair<T>(p0 - __uint_as_float(b0 & 0xffff0000u), p1 - __uint_as_float(b1 & 0xffff0000u));
-        l += p0 + p1;
-      } else {
-        pb[i] = pack_pair_sum<T>(p0, p1, l);
-      }
+      const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+      pb[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+      pr[i] = pack_pair<__bf16>(p0 - __uint_as_float(b0 & 0xffff0000u),
+                                p1 - __uint_as_float(b1 & 0xffff0000u));
+      l += p0 + p1;
     }
     // V: token i of group u, E dims in E / 2 words
     uint32_t vt[2][4][E / 2];
@@ -207,8 +192,8 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
 #pragma unroll
         for (int w = 0; w < E / 4; ++w) {
           const int at = E / 4 * i + w;
-          vt[u][i][2 * w] = kv8_cvt2<T, false>(s.v[u][at / 4][at % 4], f[i]);
-          vt[u][i][2 * w + 1] = kv8_cvt2<T, true>(s.v[u][at / 4][at % 4], f[i]);
+          vt[u][i][2 * w] = kv8_cvt2<__bf16, false>(s.v[u][at / 4][at % 4], f[i]);
+          vt[u][i][2 * w + 1] = kv8_cvt2<__bf16, true>(s.v[u][at / 4][at % 4], f[i]);
         }
     }
 #pragma unroll
@@ -218,8 +203,8 @@ __global__ __launch_bounds__(NWV * kWave, 2) void kv8_decode_kernel(
                           __builtin_amdgcn_perm(vt[0][3][j / 2], vt[0][2][j / 2], sel),
                           __builtin_amdgcn_perm(vt[1][1][j / 2], vt[1][0][j / 2], sel),
                           __builtin_amdgcn_perm(vt[1][3][j / 2], vt[1][2][j / 2], sel)};
-      acc[j] = mfma16x16x32<T>(va, pb, acc[j]);
-      if constexpr (TWO) acc[j] = mfma16x16x32<T>(va, pr, acc[j]);
+      acc[j] = mfma16x16x32<__bf16>(va, pb, acc[j]);
+      acc[j] = mfma16x16x32<__bf16>(va, pr, acc[j]);
     }
   };
 

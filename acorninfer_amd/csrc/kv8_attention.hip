@@ -389,6 +389,10 @@ int decode_rep(const DecodeArgs& a) {
 // Masked scores are set to -inf whatever they are, and V bytes are finite, so a row
 // that holds NaN reaches only the queries that see it; V rows past the last key are
 // taken as 0. Steps before the workgroup's first query need no mask.
+// Windows take P in two bf16 terms and V in bf16, in fp16 too, as decode does: a row
+// of a window is as near to 64 bits as the same row through decode (one term 1.4
+// times as far). 8 windows of 5 rows over 1024..8192 tokens 36 -> 39 us in bf16, 37
+// -> 41 in fp16; the sums of P on the VALU instead of by an MFMA of ones: no change.
 // SPLIT, WIN, partials and merge: as in paged_attention.hip. The kv head is the
 // grid's fastest index: workgroups are dealt to the 8 XCDs round robin, so with a
 // multiple of 8 kv heads a head's keys stay in one XCD's L2.
@@ -406,6 +410,8 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
   constexpr int KC = 32;                         // keys per step
   constexpr int WQ = QG * QW * 16;               // query rows per workgroup
   constexpr int PCS = KC / kKv8Group * D;        // 16-byte pieces per step, K or V
+  constexpr bool TWO = WIN;                      // P in two bf16 terms, V in bf16
+  using VT = std::conditional_t<TWO, __bf16, T>;
   constexpr int PPT = (2 * PCS + NT - 1) / NT;   // pieces per thread per step
   static_assert((2 * PCS) % NT == 0 || 2 * PCS < NT, "whole pieces per thread");
   __shared__ __align__(16) uint8_t ks[2][KC * PITCH], vs[2][KC * PITCH];
@@ -519,10 +525,10 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
       for (int j = 0; j < TP; ++j) {
         const float f = kv8_scale_finite(pc_.code >> (8 * j) & 0xFFu);
         if constexpr (TP == 2)
-          *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<T>(pc_.v[2 * j], pc_.v[2 * j + 1], f);
+          *(u32x4_t*)(dst + j * PITCH) = kv8_cvt8<VT>(pc_.v[2 * j], pc_.v[2 * j + 1], f);
         else
           *(u32x2_t*)(dst + j * PITCH) =
-              u32x2_t{kv8_cvt2<T, false>(pc_.v[j], f), kv8_cvt2<T, true>(pc_.v[j], f)};
+              u32x2_t{kv8_cvt2<VT, false>(pc_.v[j], f), kv8_cvt2<VT, true>(pc_.v[j], f)};
       }
     }
   };
@@ -531,8 +537,8 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
 
   float m[QW], nm[QW];                           // nm: -m (0 while m is -inf)
   f32x4_t acc[QW][E], accl[QW], sc[QW][2];
-  u32x4_t va[E], pb[QW];
-  const uint32_t one2 = std::is_same<T, __bf16>::value ? 0x3F803F80u : 0x3C003C00u;
+  u32x4_t va[E], pb[QW], pr[TWO ? QW : 1];       // pr: the second term
+  const uint32_t one2 = std::is_same<VT, __bf16>::value ? 0x3F803F80u : 0x3C003C00u;
   const u32x4_t ones = {one2, one2, one2, one2};
 #pragma unroll
   for (int qw = 0; qw < QW; ++qw) {
@@ -540,18 +546,23 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     nm[qw] = 0.f;
     accl[qw] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     pb[qw] = u32x4_t{0u, 0u, 0u, 0u};
+    if constexpr (TWO) pr[qw] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
     for (int jj = 0; jj < E; ++jj) acc[qw][jj] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   const uint32_t vlane = (uint32_t)((4 * r + (c >> 2)) * PITCH + 8 * (c & 3));
 
-  auto pv = [&]() {
+  auto pv_of = [&](const u32x4_t* p) {
 #pragma unroll
     for (int jj = 0; jj < E; ++jj)
 #pragma unroll
-      for (int qw = 0; qw < QW; ++qw) acc[qw][jj] = mfma16x16x32<T>(va[jj], pb[qw], acc[qw][jj]);
+      for (int qw = 0; qw < QW; ++qw) acc[qw][jj] = mfma16x16x32<VT>(va[jj], p[qw], acc[qw][jj]);
 #pragma unroll
-    for (int qw = 0; qw < QW; ++qw) accl[qw] = mfma16x16x32<T>(ones, pb[qw], accl[qw]);
+    for (int qw = 0; qw < QW; ++qw) accl[qw] = mfma16x16x32<VT>(ones, p[qw], accl[qw]);
+  };
+  auto pv = [&]() {
+    pv_of(pb);
+    if constexpr (TWO) pv_of(pr);
   };
   u32x4_t kf[2][KB];
   auto read_k = [&](int step) {
@@ -669,7 +680,7 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
 
   auto iteration = [&](int s, auto masked) {
     read_k(s + 1);
-    u32x4_t pn[QW];
+    u32x4_t pn[QW], rn[TWO ? QW : 1];
 #pragma unroll
     for (int qw = 0; qw < QW; ++qw)
 #pragma unroll
@@ -678,13 +689,23 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
             __builtin_fmaf(sc[qw][i / 2][2 * (i % 2)], scale_log2, nm[qw]));
         const float p1 = __builtin_amdgcn_exp2f(
             __builtin_fmaf(sc[qw][i / 2][2 * (i % 2) + 1], scale_log2, nm[qw]));
-        pn[qw][i] = pack_pair<T>(p0, p1);
+        if constexpr (TWO) {
+          const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+          pn[qw][i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+          rn[qw][i] = pack_pair<__bf16>(p0 - __uint_as_float(b0 & 0xffff0000u),
+                                        p1 - __uint_as_float(b1 & 0xffff0000u));
+        } else {
+          pn[qw][i] = pack_pair<T>(p0, p1);
+        }
       }
     scores();
     read_v(s - 1);
     pv();
 #pragma unroll
-    for (int qw = 0; qw < QW; ++qw) pb[qw] = pn[qw];
+    for (int qw = 0; qw < QW; ++qw) {
+      pb[qw] = pn[qw];
+      if constexpr (TWO) pr[qw] = rn[qw];
+    }
 #pragma unroll
     for (int i = 0; i < PPT; ++i)
       if (stages) {
@@ -695,7 +716,10 @@ __global__ __launch_bounds__(REP * QG * kWave, 2) void kv8_prefill_kernel(
     // (without this the probabilities' work, next needed in the iteration to come, would sink
     // behind settle's branch, away from the MFMAs)
 #pragma unroll
-    for (int qw = 0; qw < QW; ++qw) asm volatile("" : "+v"(pb[qw]));
+    for (int qw = 0; qw < QW; ++qw) {
+      asm volatile("" : "+v"(pb[qw]));
+      if constexpr (TWO) asm volatile("" : "+v"(pr[qw]));
+    }
     settle(s + 1, masked);
     __syncthreads();
   };

@@ -1,6 +1,6 @@
-"""How near attention over the 8-bit cache is to 64 bits: decode takes the
-probabilities in two bf16 terms, so that only the result's own rounding counts, and loses no weight
-of many tokens far below one (an attention sink)."""
+"""How near attention over the 8-bit cache is to 64 bits: decode and verify windows
+take the probabilities in two bf16 terms, so that only the result's own rounding counts, and lose
+no weight of many tokens far below one (an attention sink)."""
 import pytest
 import torch
 
@@ -27,10 +27,13 @@ def _cache(k, v):
 
 
 def _run(form, q, kv, tab, L):
-    """q [H, D] as the last token of a sequence of L, by decode in n splits."""
-    n = form[1]
-    return _kv8().paged_decode_attention_kv8(q[None].cuda(), kv, tab, torch.full((1,), L, dtype=torch.int32).cuda(),
-                                             n)[0].cpu()
+    """q [H, D] as the last token of a sequence of L: by decode in n splits, or as the last row of a
+    window of n."""
+    kind, n = form
+    lens = torch.full((1,), L, dtype=torch.int32, device="cuda")
+    if kind == "decode":
+        return _kv8().paged_decode_attention_kv8(q[None].cuda(), kv, tab, lens, n)[0].cpu()
+    return _kv8().paged_verify_attention_kv8(q.expand(1, n, *q.shape).cuda(), kv, tab, lens)[0, -1].cpu()
 
 
 def _close(heads, D, dtype, L):
@@ -69,8 +72,10 @@ def test_the_bound_tells_one_term_from_two():
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D,heads,L", [(128, 4, 600), (64, 8, 600), (128, 1, 3000), (128, 8, 34)])
-@pytest.mark.parametrize("form", [("decode", 1), ("decode", 3), ("decode", 64)])
+@pytest.mark.parametrize("form", [("decode", 1), ("decode", 3), ("decode", 64), ("window", 2), ("window", 40)])
 def test_two_terms(form, D, heads, L, dtype):
+    if form[0] == "window":
+        L = max(L, 80)
     q, k, v = _close(heads, D, dtype, L)
     out = _run(form, q, *_cache(k, v), L)
     want, mean, big = attend(q, k.double(), v.double())
@@ -89,21 +94,25 @@ def _random(B, L, H, KV, D, dtype, seed):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,L", [(32, 40), (16, 400), (8, 1600)])
-def test_decode_rows_are_off_by_the_results_rounding(H, L, dtype):
-    """Rows through decode against 64 bits: the error is that of rounding the result to its type,
-    within a percent (20000 outputs and more: the norms are known to within one; what 32 bits and
-    two terms add is below a hundredth of a rounding)."""
-    KV, D, B = 8, 128, 160
+def test_decode_and_window_rows_are_off_by_the_results_rounding(H, L, dtype):
+    """Rows through decode and through windows of five, against 64 bits: the error is that of
+    rounding the result to its type, within a percent (20000 outputs and more: the norms are known
+    to within one; what 32 bits and two terms add is below a hundredth of a rounding)."""
+    KV, D, m, B = 8, 128, 5, 160
     q, k, v = _random(B, L, H, KV, D, dtype, L)
     kv, tab = _cache(k, v)
     pool = Pool.of(kv, P)
     held = pool.values(range(pool.NB), range(L))
-    seen = [L - i % 5 for i in range(B)]
+    seen = [L - (m - 1 - i % m) for i in range(B)]
     exact = torch.stack([attend(x, held[0][:n], held[1][:n])[0] for x, n in zip(q, seen)])
     lens = torch.tensor(seen, dtype=torch.int32, device="cuda")
     rows = _kv8().paged_decode_attention_kv8(q.cuda(), kv, tab.expand(B, -1).contiguous(), lens).cpu()
+    wins = _kv8().paged_verify_attention_kv8(q.view(B // m, m, H, D).cuda(), kv,
+                                             tab.expand(B // m, -1).contiguous(),
+                                             torch.full((B // m,), L, dtype=torch.int32, device="cuda"))
     best = float((exact.to(dtype).double() - exact).norm())
-    assert float((rows.double() - exact).norm()) <= 1.01 * best
+    for name, x in (("decode", rows), ("windows", wins.view(B, H, D).cpu())):
+        assert float((x.double() - exact).norm()) <= 1.01 * best, name
 
 
 SINK_GAPS = (10.0, 16.5, 17.0, 17.5, 20.0, 22.0)
@@ -111,7 +120,7 @@ SINK_GAPS = (10.0, 16.5, 17.0, 17.5, 20.0, 22.0)
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("form", [("decode", 1), ("decode", 16)])
+@pytest.mark.parametrize("form", [("decode", 1), ("decode", 16), ("window", 3), ("window", 40)])
 @pytest.mark.parametrize("at", [0, 2000])
 def test_many_tokens_far_below_one_keep_their_weight(at, form, dtype):
     """One token whose score is `gap` above that of 4000 others, and whose values are 0: the result

@@ -130,12 +130,12 @@ def tolerance(out, mean_abs, big, dtype, L, terms=1):
     """Elementwise bound on |kernel - out|. A score is a sum of D products in 32 bits, its factor
     and the exponential (together under 2^-16 of the sum of magnitudes `big`, plus 2^-20); the
     result is rounded once (u). The weights p: with terms=1 (prompt rows) they are rounded to the
-    type (u each, and their sum with them: 2 u of the mean of |v|), and fp16 weights have
-    no steps finer than 2^-24 (of a largest weight of 1 or more, L of them); with terms=2 (decode,
-    windows) they are two bf16 terms: p cut to 8 bits leaves under 2^-7 of it,
-    rounded to 8 bits itself, half a step of which is 2^-16 of p at most."""
+    type (u each, and their sum with them: 2 u of the mean of |v|), and fp16 weights, held
+    times 2^7, have no steps finer than 2^-24 (of a largest weight of 1 or more, L of them);
+    with terms=2 (decode, windows) they are two bf16 terms: p cut to 8 bits leaves under 2^-7
+    of it, rounded to 8 bits itself, half a step of which is 2^-16 of p at most."""
     u = torch.finfo(dtype).eps / 2
     e = (u if terms == 1 else 2.0 ** -16) + big * 2.0 ** -16 + 2.0 ** -20
-    sub = 2.0 ** -25 * L if dtype == torch.float16 and terms == 1 else 0.0
+    sub = 2.0 ** -32 * L if dtype == torch.float16 and terms == 1 else 0.0
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     return 2 * (e + sub) * mean_abs + u * out.abs() * (1 + 2 ** -6) + tiny

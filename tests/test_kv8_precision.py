@@ -1,6 +1,6 @@
 """How near attention over the 8-bit cache is to 64 bits: decode and verify windows
-take the probabilities in two bf16 terms, so that only the result's own rounding counts, and lose
-no weight of many tokens far below one (an attention sink)."""
+take the probabilities in two bf16 terms, so that only the result's own rounding counts; they and
+prompt rows keep the weight of many tokens far below one (an attention sink)."""
 import pytest
 import torch
 
@@ -27,13 +27,17 @@ def _cache(k, v):
 
 
 def _run(form, q, kv, tab, L):
-    """q [H, D] as the last token of a sequence of L: by decode in n splits, or as the last row of a
-    window of n."""
+    """q [H, D] as the last token of a sequence of L: by decode in n splits, as the last row of a
+    window of n, or as the last of n prompt rows."""
     kind, n = form
     lens = torch.full((1,), L, dtype=torch.int32, device="cuda")
     if kind == "decode":
         return _kv8().paged_decode_attention_kv8(q[None].cuda(), kv, tab, lens, n)[0].cpu()
-    return _kv8().paged_verify_attention_kv8(q.expand(1, n, *q.shape).cuda(), kv, tab, lens)[0, -1].cpu()
+    if kind == "window":
+        return _kv8().paged_verify_attention_kv8(q.expand(1, n, *q.shape).cuda(), kv, tab, lens)[0, -1].cpu()
+    one = torch.ones_like(lens)
+    return _kv8().paged_prefill_attention_kv8(q.expand(n, *q.shape).cuda(), kv, tab, 0 * one, lens - n, n * one,
+                                              n)[-1].cpu()
 
 
 def _close(heads, D, dtype, L):
@@ -115,12 +119,14 @@ def test_decode_and_window_rows_are_off_by_the_results_rounding(H, L, dtype):
         assert float((x.double() - exact).norm()) <= 1.01 * best, name
 
 
+PROMPT_STEP = 2.0 ** -25 * 2.0 ** -7       # half of fp16's least step, of weights held times 2^7
 SINK_GAPS = (10.0, 16.5, 17.0, 17.5, 20.0, 22.0)
 
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("form", [("decode", 1), ("decode", 16), ("window", 3), ("window", 40)])
+@pytest.mark.parametrize("form", [("decode", 1), ("decode", 16), ("window", 3), ("window", 40),
+                                  ("prompt", 1), ("prompt", 70)])
 @pytest.mark.parametrize("at", [0, 2000])
 def test_many_tokens_far_below_one_keep_their_weight(at, form, dtype):
     """One token whose score is `gap` above that of 4000 others, and whose values are 0: the result
@@ -140,6 +146,31 @@ def test_many_tokens_far_below_one_keep_their_weight(at, form, dtype):
         q = q.to(dtype)
         out = _run(form, q, kv, tab, L).double()
         want, mean, big = attend(q, hk, hv)
-        tol = tolerance(want, mean, big, dtype, L, terms=2)
+        tol = tolerance(want, mean, big, dtype, L, terms=1 if form[0] == "prompt" else 2)
+        if form[0] == "prompt" and dtype == torch.float16:
+            tol = tol + PROMPT_STEP * hv.abs().sum(0)          # (each weight, of a sum above 1)
         err = (out - want).abs()
         assert (err <= tol).all(), (SINK_GAPS[first], float((err / tol).max()), float((out / want).mean()))
+
+
+@gpu
+@pytest.mark.parametrize("order", ["rising", "falling"])
+def test_prompt_weights_stay_within_fp16(order):
+    """Scores that rise or fall by less than the maximum's slack from step to step: the largest
+    weights are 2^15, and no sum of them is lost."""
+    L, D, KV, H = 700, 64, 1, 8
+    g = torch.Generator().manual_seed(5)
+    k = torch.zeros(L, KV, D)
+    k[:, 0, 0] = torch.linspace(0, 448, L) if order == "rising" else torch.linspace(448, 0, L)
+    v = torch.randn(L, KV, D, generator=g)
+    kv, tab = _cache(k.half(), v.half())
+    pool = Pool.of(kv, P)
+    hk, hv = pool.values(range(pool.NB), range(L))
+    q = torch.zeros(H, D)
+    q[:, 0] = torch.linspace(0.02, 2.0, H)
+    q = q.half()
+    out = _run(("prompt", 1), q, kv, tab, L).double()
+    want, mean, big = attend(q, hk, hv)
+    err = (out - want).abs()
+    tol = tolerance(want, mean, big, torch.float16, L)
+    assert (err <= tol).all(), float((err / tol).max())

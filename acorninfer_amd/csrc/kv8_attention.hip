@@ -909,6 +909,8 @@ extern "C" int acorn_paged_prefill_attention_kv8(
   if (!q || !k_tiles || !v_tiles || !scales || !tables || !seq_pos0 || !out || !seq_row0 != !seq_nq)
     return ACORN_ERR_VALUE;
   if (!seq_nq && R != N * max_nq) return ACORN_ERR_SHAPE;
+  // (the maxima are those of the scores before the factor, and -inf masks stay so behind it)
+  if (!(scale > 0.f && scale * kLog2e <= __FLT_MAX__)) return ACORN_ERR_VALUE;
   if (!aligned16({q, k_tiles, v_tiles, scales, out, ws})) return ACORN_ERR_VALUE;
   max_nq = std::min(max_nq, R);                // a bound far above the rows there are costs nothing
   PrefillArgs a{q, k_tiles, v_tiles, scales, tables, seq_row0, seq_pos0, seq_nq, out, N, R, max_nq,

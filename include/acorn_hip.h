@@ -525,6 +525,7 @@ int acorn_paged_attention_kv8(const void* q, const void* k_tiles, const void* v_
 /*
  * acorn_paged_prefill_attention_ws over the 8-bit cache (windows included: seq_row0 and
  * seq_nq both NULL). Rows at positions past their table row's pages are not written.
+ * scale is finite and above 0 (ACORN_ERR_VALUE).
  * ws: at least the bytes acorn_paged_prefill_workspace_kv8 reports, or nothing is split.
  */
 int acorn_paged_prefill_attention_kv8(const void* q, const void* k_tiles, const void* v_tiles,

@@ -511,10 +511,17 @@ class Qwen3DecodeModel:
 
     def kv8_page(self, cache) -> int:
         """StepBuffers.kv8_page for steps over `cache`: its page size where it is an 8-bit one
-        (NotImplementedError for a model whose attention it is not built for), else 0."""
+        (NotImplementedError for a model whose attention it is not built for, ValueError for a
+        cache made for another model), else 0."""
         if getattr(cache, "scale_pool", None) is None:
             return 0
         cfg = self.cfg
+        if cache.num_layers < cfg.num_hidden_layers or cache.head_dim != cfg.head_dim or \
+                cache.num_kv_heads != cfg.num_key_value_heads:       # steps would leave its pools
+            raise ValueError(
+                f"8-bit cache of {cache.num_layers} layers, {cache.num_kv_heads} kv heads of "
+                f"{cache.head_dim} under a model of {cfg.num_hidden_layers}, "
+                f"{cfg.num_key_value_heads} of {cfg.head_dim}")
         if cache.dtype != self.dtype or not kv8_attention_supported(
                 self.dtype, cfg.head_dim, cache.page_size, cfg.num_attention_heads,
                 cfg.num_key_value_heads):

@@ -189,8 +189,9 @@ class PagedKVCache:
 
 class PagedKV8Cache(PagedKVCache):
     """The cache in 8 bits: per layer a KV8Pages (`pages[l]`), views of one pool of K tiles, one
-    of V tiles and one of scale codes. `dtype` is the activations' (bf16, or fp16): rows are
-    rounded to it before they are quantised, and what is read back has it."""
+    of V tiles and one of scale codes. `dtype` is the activations' (bf16, or fp16): rows that
+    a view or scatter_* writes are rounded to it before they are quantised (a model's steps quantise
+    from 32 bits), and what is read back has it."""
 
     def _allocate(self) -> None:
         if not kv8_supported(self.head_dim, self.page_size) or \

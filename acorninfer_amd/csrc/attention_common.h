@@ -294,6 +294,8 @@ struct PrefillPlan {
 // run costs its rows' fp32 partials, written and read: small next to a window's
 // keys, about five chunks' time for a full tile, so runs keep kWindowMinRun
 // chunks, kPrefillMinRun, or kPrefillBusyRun once half the CUs have a tile.
+// Everything here was measured with the 16-bit cache's kernel; the 8-bit cache's
+// takes the same plan, of which only single launches were timed.
 // Measured, one split / this rule (us), 32 / 8 heads: 5 rows over 8000 tokens
 // 157 / 27, 64 rows 213 / 39, 150 rows 216 / 63, 520 rows 227 / 150, 800 rows
 // 236 / 193.

@@ -3,11 +3,11 @@
 //                                      the cache's length and joined
 //   acorn_paged_prefill_attention_kv8  packed prompt rows, causal
 // Both turn bytes into bf16 / fp16 and use the 16-bit MFMAs with fp32 sums. The
-// conversion is exact within the type's range: fp16 rounds what lies below 2^-14
-// to steps of 2^-24. The fp8 MFMAs would take the bytes as they lie, with q in two or three
-// e4m3 terms, but add their products to fewer bits: measured against 64 bits
-// 1.6e-5 of the sum of magnitudes for normal numbers, 2.8e-4 where one in
-// sixteen is a hundred times larger, 2e-8 with the bf16 MFMA.
+// conversion is exact within the type's range: fp16 (K, and V of prompt attention)
+// rounds what lies below 2^-14 to steps of 2^-24. The fp8 MFMAs would take the bytes
+// as they lie, with q in two or three e4m3 terms, but add their products to fewer
+// bits: measured against 64 bits 1.6e-5 of the sum of magnitudes for normal numbers,
+// 2.8e-4 where one in sixteen is a hundred times larger, 2e-8 with the bf16 MFMA.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,9 +49,9 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
 // The wave's block ids are fetched one step ahead of their tiles, DEPTH steps
 // of tiles are in flight. Loads are unconditional (wait counts stay static):
 // those past the wave's last group read one line of it.
-// Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 104 us, 5.4
-// TB/s; one of 131000, 16 / 8 heads, 48.5 us, 5.6 TB/s (a large copy: 4.8). In one
-// sweep, where the first took 111: with default instead of non-temporal loads 120, three
+// Bound by memory: 64 sequences of 1024..8192 tokens, 32 / 8 heads, 105 us, 5.4
+// TB/s; one of 131000, 16 / 8 heads, 48.7 us, 5.5 TB/s (a large copy: 4.8). In one
+// sweep, where the first took 111 (another card): with default instead of non-temporal loads 120, three
 // steps in flight 111, four waves per workgroup 109 to 117 by splits, 128 registers for four
 // waves per SIMD 185.
 template <typename T, int D, int REP, int NWV, int DEPTH>
@@ -380,11 +380,11 @@ int decode_rep(const DecodeArgs& a) {
 // steps' work without dependences between them, the probabilities of step s, the score
 // MFMAs of step s + 1 and the P V MFMAs of step s - 1, while K of step s + 2 and V of
 // step s move from registers into LDS. K and V have two LDS buffers each, with one
-// barrier per step. 8192 causal tokens, 32 / 8 heads: 521 us (1055 TFLOP/s; a large
-// library product reaches 1208); the steps' parts one after another 772; P V of step
-// s - 1 ahead of the scores, V held in registers over the barrier, 569. Fixed orders
-// of MFMA and VALU instructions (scheduling groups) and wave priorities around
-// the MFMAs were slower than the compiler's order, 530 to 600.
+// barrier per step. 8192 causal tokens, 32 / 8 heads: 510 to 540 us on different cards
+// (1.08 to 1.02 PFLOP/s; a large library product reaches 1.21). Where it took 521: the
+// steps' parts one after another 772; P V of step s - 1 ahead of the scores, V held in
+// registers over the barrier, 569; fixed orders of MFMA and VALU instructions
+// (scheduling groups) and wave priorities around the MFMAs 530 to 600.
 //
 // P is rounded to T once (a second term would double the P V MFMAs, which already take
 // as long as the VALU work), and the sum of a query's P is that of the rounded values. In

@@ -252,13 +252,18 @@ def kv8_splits(batch: int, kv_heads: int, max_pages: int, page_size: int) -> int
     """Splits of the cache's length for paged_decode_attention_kv8 over block tables max_pages
     wide. The kernel runs splits of more than 16 groups of 16 tokens as workgroups of eight waves,
     of which a CU holds one, and shorter ones as one wave; more than one split takes a second
-    launch (2 to 8 us). Measured on MI355X, 32 / 8 heads, us:
+    launch (2 to 8 us). Measured on MI355X, 32 / 8 heads, tables as wide as the longest sequence,
+    us, each line from one sweep (figures of other cards and runs differ by some 5%):
     - (sequence, kv head) pairs that fill the CUs, or short tables: one split (64 sequences of
       1024..8192 tokens 110, in 31 splits of one wave 116; one of 333 6.4, in 11 splits 7.3);
     - else as many as make one round of eight-wave workgroups (one sequence of 131000, 16 / 8
       heads: 32 splits 47.8, 64 49.8, 24 49.0; 16 of 4000: 2 splits 29.7, 3 33.5, 1 33.1),
     - but one-wave splits where those would be short (one of 4000: 63 splits 8.9, 16 12.7) or fill
-      three quarters of the CUs or less (12 of 2000..8000: 31 splits 29, 2 36)."""
+      three quarters of the CUs or less (12 of 2000..8000: 31 splits 29, 2 36).
+    The rule sees the table's width and not the lengths: splits grow with the table, and a sequence
+    much longer than the others gets no more of them. 8 sequences of 2000..8000 take 22 us under a
+    table of 7456 tokens and 48 under one of 131072; one of 100000 among 31 of 500..1500 takes 497
+    (16-bit cache 167), where num_splits of the caller's choice may do better."""
     per = page_size // GROUP
     groups, pairs = max_pages * per, max(1, batch * kv_heads)
     if pairs >= MI355X_CUS or groups <= 32 or (groups <= 64 and pairs >= 64):

@@ -16,6 +16,9 @@ from pathlib import Path
 
 import torch
 
+# (the stream's handle without a Stream object around it: a microsecond of a call's ten)
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
+
 LIB_PATH = Path(os.environ.get(
     "ACORN_HIP_LIB", Path(__file__).resolve().parent / "_lib" / "libacorn_hip.so"))
 
@@ -87,6 +90,14 @@ _SIGNATURES = {
                                           _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32,
                                           _vp, _i64, _vp],
     "acorn_paged_prefill_workspace_kv8": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
+    "acorn_beam_select": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
+                          _vp],
+    "acorn_beam_select_workspace": [_i64, _i64, _i64, _i64, _i32, _vp],
+    "acorn_beam_advance": [_vp] * 24 + [_i64] * 5 + [ctypes.c_double, _i32, _i64, _vp],
+    "acorn_beam_reorder": [_vp] * 6 + [_i64] * 9 + [_vp],
+    "acorn_beam_trace": [_vp] * 5 + [_i64] * 5 + [_vp],
+    "acorn_block_tables": [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "acorn_slot_map": [_vp] * 9 + [_i64] * 4 + [_vp],
     "acorn_kv_scatter": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32,
                          _vp],
 }
@@ -159,3 +170,28 @@ def require_gpu(*tensors: torch.Tensor | None) -> None:
         if t is not None and t.device.type != "cuda":
             raise ValueError(
                 f"acorninfer_amd operators run only on the GPU (got a {t.device} tensor)")
+
+
+def one_device(first: torch.Tensor, *tensors: torch.Tensor) -> int:
+    """The index of the one GPU that holds the tensors: a kernel launches on one device's stream
+    and reaches every tensor by its pointer."""
+    dev = first.get_device()
+    for t in tensors:
+        if t.get_device() != dev:
+            require_gpu(first, *tensors)
+            raise AssertionError(f"tensors on {first.device} and {t.device}")
+    if dev < 0:
+        require_gpu(first)
+    return dev
+
+
+def launch(name: str, dev: int, *args) -> None:
+    """Launch on the current stream of device `dev`, with that device current."""
+    fn = getattr(lib(), "acorn_" + name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        check(rc, name)

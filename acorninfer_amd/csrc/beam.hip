@@ -1,0 +1,391 @@
+// Between two steps of a beam search, after its selection (beam_select.hip):
+//   acorn_beam_advance  the next beams and the finished hypotheses of every group
+//   acorn_beam_reorder  block tables and partly filled pages follow the beams
+//   acorn_beam_trace    hypotheses out of the logs of tokens and parents
+// All are short: a few hundred bytes, or copies of a page per layer, behind a chain of
+// dependent loads.
+#include <algorithm>
+
+#include "common.h"
+
+using namespace acorn;
+
+namespace {
+
+constexpr int kMaxBeams = 32, kMaxK = 64;
+
+__device__ __forceinline__ uint64_t lanes_below(int lane) { return (1ull << lane) - 1; }
+
+struct BeamFields {
+  float* scores;         // [G, W]
+  int32_t* length;       // [G]
+  int32_t* done;         // [G]
+  int64_t* ids;          // [G, W]
+  int32_t* position;     // [G, W]
+  int32_t* parents;      // [G, W]
+  float* fin_scores;     // [G, W]
+  int32_t* fin_length;
+  int32_t* fin_beam;
+  int32_t* fin_token;
+};
+
+// One wave per group, a candidate to a lane; a group's old state is in registers before any of the
+// new one is written, so that both may be the same memory.
+__global__ __launch_bounds__(kWave) void beam_advance_kernel(
+    const BeamFields in, const BeamFields out, int32_t* token_log, int32_t* parent_log,
+    const float* cand_score, const int32_t* cand_beam, const int64_t* cand_token,
+    const int64_t* ends, int G, int W, int K, int T, int n_ends, double alpha, int early,
+    int64_t pad) {
+  const int g = blockIdx.x, lane = threadIdx.x;
+  const size_t gw = (size_t)g * W;
+  const bool beam = lane < W, cand = lane < K;
+  const int l = beam ? lane : 0;
+  const int t = in.length[g], old_done = in.done[g];
+  const float score = in.scores[gw + l];
+  const int position = in.position[gw + l];
+  const float fin_score = in.fin_scores[gw + l];
+  const int fin_length = in.fin_length[gw + l], fin_beam = in.fin_beam[gw + l],
+            fin_token = in.fin_token[gw + l];
+  const size_t ck = (size_t)g * K + (cand ? lane : 0);
+  const float cs = cand_score[ck];
+  const int cb = cand_beam[ck];
+  const int64_t ct = cand_token[ck];
+  bool end = false;
+  for (int i = 0; i < n_ends; ++i) end |= ct == ends[i];
+  __syncthreads();
+
+  if (old_done != 0 || t < 0 || t >= T) {                      // it stays as it is
+    if (beam) {
+      out.scores[gw + lane] = score;
+      out.ids[gw + lane] = pad;
+      out.position[gw + lane] = position;
+      out.parents[gw + lane] = lane;
+      out.fin_scores[gw + lane] = fin_score;
+      out.fin_length[gw + lane] = fin_length;
+      out.fin_beam[gw + lane] = fin_beam;
+      out.fin_token[gw + lane] = fin_token;
+    }
+    if (lane == 0) {
+      out.length[g] = t;
+      out.done[g] = old_done;
+    }
+    return;
+  }
+
+  // the next beams: the first W candidates that go on
+  const bool valid = cand && cs > -INFINITY && cb >= 0 && cb < W;
+  const bool goes = valid && !end;
+  const uint64_t gm = __ballot(goes);
+  const int slot = __popcll(gm & lanes_below(lane)), live = min(__popcll(gm), W);
+  const size_t log = ((size_t)t * G + g) * W;
+  auto put = [&](int i, float s, int64_t id, int parent) {
+    out.scores[gw + i] = s;
+    out.ids[gw + i] = id;
+    out.parents[gw + i] = parent;
+    token_log[log + i] = (int32_t)id;
+    parent_log[log + i] = parent;
+  };
+  if (goes && slot < W) put(slot, cs, ct, cb);
+  if (beam && lane >= live) put(lane, -INFINITY, pad, lane);
+  const float best = gm ? __shfl(cs, __ffsll((unsigned long long)gm) - 1) : -INFINITY;
+
+  // the finished: the best W of those there were (lanes 0 .. W - 1, sorted) and those that end
+  // now (lanes W .. 2 W - 1: candidates 0 .. W - 1), of equal ones the lower lane
+  const double power = pow((double)(t + 1), alpha);
+  const int from = lane >= W ? lane - W : 0;
+  const bool took = __shfl((int)(valid && end), from) && lane >= W && lane < 2 * W;
+  const float fresh = (float)((double)__shfl(cs, from) / power);
+  const int fresh_beam = __shfl(cb, from), fresh_token = (int)__shfl((long long)ct, from);
+  const float fs = beam ? fin_score : took ? fresh : -INFINITY;
+  const int fl = beam ? fin_length : took ? t + 1 : 0;
+  const int fb = beam ? fin_beam : took ? fresh_beam : 0;
+  const int ft = beam ? fin_token : took ? fresh_token : 0;
+  int rank = 0;
+  for (int j = 0; j < 2 * W; ++j) {
+    const float o = __shfl(fs, j);
+    rank += o > fs || (o == fs && j < lane);
+  }
+  const bool kept = lane < 2 * W && rank < W;
+  if (kept) {
+    out.fin_scores[gw + rank] = fs;
+    out.fin_length[gw + rank] = fl;
+    out.fin_beam[gw + rank] = fb;
+    out.fin_token[gw + rank] = ft;
+  }
+  const uint64_t last = __ballot(kept && rank == W - 1);
+  const int ll = __ffsll((unsigned long long)last) - 1;
+  const float worst = __shfl(fs, max(ll, 0));
+  const bool full = last && __shfl(fl, max(ll, 0)) > 0;
+  if (beam) out.position[gw + lane] = position + 1;
+  if (lane == 0) {
+    const float reach = (float)((double)best / power);
+    const bool stop = best == -INFINITY || t + 1 >= T || (full && (early || worst >= reach));
+    out.length[g] = t + 1;
+    out.done[g] = stop;
+  }
+}
+
+// ---- the cache follows the beams --------------------------------------------------------------
+// At n cached tokens the pages before column c = n / P are full: a beam's row takes its parent's,
+// shared from now on. Column c is a page of the beam's own, filled by n % P tokens: the first
+// child of a beam takes its page over, every further child a page of a beam without children, in
+// order, with a copy of the tokens. So every page stays with one beam of its group, sources are
+// pages that nothing is written to, and no page is needed that the group has not.
+
+// Of lane l < W: the page that the next beam l holds at column c, and the one its tokens are in.
+struct Plan {
+  int to, from;
+};
+__device__ __forceinline__ Plan plan_pages(int parent, int page, int W, int lane) {
+  bool first = lane < W, child = false;
+  for (int j = 0; j < W; ++j) {
+    const int pj = __shfl(parent, j);
+    first &= !(j < lane && pj == parent);
+    child |= pj == lane;
+  }
+  const uint64_t more = __ballot(lane < W && !first), spare = __ballot(lane < W && !child);
+  const int from = __shfl(page, parent);
+  // the r-th further child takes the page of the r-th beam without children
+  const int r = __popcll(more & lanes_below(lane));
+  uint64_t rest = spare;
+  for (int i = 0; i < r; ++i) rest &= rest - 1;
+  const int owner = rest ? __ffsll((unsigned long long)rest) - 1 : 0;
+  const int other = __shfl(page, owner);
+  return {first ? from : other, from};
+}
+
+__device__ __forceinline__ int parent_of(const int32_t* parents, size_t gw, int W, int lane) {
+  const int l = lane < W ? lane : 0;
+  const int p = parents[gw + l];
+  return p >= 0 && p < W ? p : l;              // (a parent that there is not: the beam itself)
+}
+
+// A pool [layers, num_blocks, page_bytes]; a page is `segs` runs of `stride` bytes, of which the
+// tokens' first bytes are copied: `unit` for every `group` tokens or part of them.
+struct Pool {
+  uint8_t* base;
+  int64_t page_bytes;
+  int segs, stride, unit, group;
+};
+struct Pools {
+  Pool p[3];
+};
+
+constexpr int kCopyNT = 256;
+typedef uint32_t bm_u32x4 __attribute__((ext_vector_type(4)));
+
+__global__ __launch_bounds__(kCopyNT) void beam_copy_kernel(
+    const Pools pools, const int32_t* __restrict__ tables, const int32_t* __restrict__ lens,
+    const int32_t* __restrict__ parents, int W, int P, int64_t num_blocks, int width) {
+  const int child = blockIdx.y, g = child / W, layer = blockIdx.x;
+  const int lane = threadIdx.x % kWave;
+  const size_t gw = (size_t)g * W;
+  const int n = lens[gw], fill = n % P, c = n / P;
+  if (n <= 0 || fill == 0 || c >= width) return;
+  const int parent = parent_of(parents, gw, W, lane);
+  const int page = tables[(gw + (lane < W ? lane : 0)) * width + c];
+  const Plan plan = plan_pages(parent, page, W, lane);
+  const int w = child % W;
+  const int64_t to = __shfl(plan.to, w), from = __shfl(plan.from, w);
+  if (to == from || to < 0 || from < 0 || to >= num_blocks || from >= num_blocks) return;
+  const Pool pool = pools.p[blockIdx.z];
+  const size_t base = (size_t)layer * num_blocks * pool.page_bytes;
+  const uint8_t* src = pool.base + base + from * pool.page_bytes;
+  uint8_t* dst = pool.base + base + to * pool.page_bytes;
+  const int per = (fill + pool.group - 1) / pool.group * pool.unit / 16;   // 16-byte pieces of a run
+  const int total = per * pool.segs;
+  for (int i = threadIdx.x; i < total; i += kCopyNT) {
+    const int64_t at = (int64_t)(i / per) * pool.stride + (int64_t)(i % per) * 16;
+    *(bm_u32x4*)(dst + at) = *(const bm_u32x4*)(src + at);
+  }
+}
+
+// A thread per column, which reads the group's entries of it before it writes them.
+__global__ __launch_bounds__(256) void beam_tables_kernel(int32_t* tables, const int32_t* lens,
+                                                          const int32_t* parents, int W, int P,
+                                                          int width) {
+  __shared__ int32_t held[kMaxBeams][256];
+  __shared__ int32_t par[kMaxBeams], taken[kMaxBeams];
+  const int g = blockIdx.y, lane = threadIdx.x;
+  const size_t gw = (size_t)g * W;
+  const int n = max(lens[gw], 0), fill = n % P, c = n / P;
+  if ((int64_t)blockIdx.x * 256 > c) return;                   // columns of the future
+  if (lane < kWave) {
+    const int parent = parent_of(parents, gw, W, lane);
+    const int page = c < width ? tables[(gw + (lane < W ? lane : 0)) * width + c] : 0;
+    const Plan plan = plan_pages(parent, page, W, lane);
+    if (lane < W) {
+      par[lane] = parent;
+      taken[lane] = fill ? plan.to : page;
+    }
+  }
+  __syncthreads();
+  const int64_t column = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (column >= width || column > c) return;
+  int32_t* t = tables + gw * width + column;
+  if (column == c) {
+    for (int w = 0; w < W; ++w) t[(size_t)w * width] = taken[w];
+    return;
+  }
+  for (int w = 0; w < W; ++w) held[w][threadIdx.x] = t[(size_t)w * width];
+  for (int w = 0; w < W; ++w)
+    if (par[w] != w) t[(size_t)w * width] = held[par[w]][threadIdx.x];
+}
+
+// ---- hypotheses -------------------------------------------------------------------------------
+// out[g, m, t] = tokens[t, g, b_t] for t < steps[g, m], where b_{steps - 1} = beams[g, m] and
+// b_{t - 1} = parents[t, g, b_t]; `pad` behind. A walk of T dependent steps: each wave takes a
+// piece of the steps, follows every beam through it (a map of W beams), the maps of the pieces
+// are chained, and each wave then walks its piece again with the beams that reach it.
+constexpr int kTraceWaves = 16;
+
+__global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
+    const int32_t* __restrict__ tokens, const int32_t* __restrict__ parents,
+    const int32_t* __restrict__ steps, const int32_t* __restrict__ beams,
+    int64_t* __restrict__ out, int T, int G, int W, int M, int64_t pad) {
+  __shared__ int map[kTraceWaves][kMaxBeams];      // beam at a piece's end -> before its first step
+  __shared__ int part[kWave];                      // the same for a walk that starts in a piece
+  const int g = blockIdx.x, lane = threadIdx.x % kWave, wid = threadIdx.x / kWave;
+  const int m = blockIdx.y * kWave + lane;
+  const bool hyp = m < M;
+  const int per = (T + kTraceWaves - 1) / kTraceWaves;
+  const int a = min(wid * per, T), b = min(a + per, T);
+  const int start = hyp ? min(steps[(size_t)g * M + m], T) - 1 : -1;
+  const int beam0 = hyp ? beams[(size_t)g * M + m] : -1;
+  auto inside = [&](int x) { return x >= 0 && x < W ? x : -1; };      // -1 ends a walk
+  auto hop = [&](int row, int cur) {
+    const int next = __shfl(row, cur < 0 ? 0 : cur);
+    return cur < 0 ? -1 : inside(next);
+  };
+  const int l = lane < W ? lane : 0;
+  int all = lane < W ? lane : -1, mine = -1;
+  const bool here = hyp && start >= a && start < b;
+  for (int t = b - 1; t >= a; --t) {
+    const int row = parents[((size_t)t * G + g) * W + l];
+    if (here && t == start) mine = inside(beam0);
+    all = hop(row, all);
+    mine = hop(row, mine);
+  }
+  if (lane < W) map[wid][lane] = all;
+  if (here) part[lane] = mine;
+  __syncthreads();
+  // the beam at this piece's end (or at the walk's start in it)
+  int cur = -1;
+  if (hyp && start >= b) {
+    const int piece = start / per;
+    cur = part[lane];
+    for (int i = piece - 1; i > wid; --i) cur = cur < 0 ? -1 : map[i][cur];
+  }
+  int64_t* o = out + ((size_t)g * M + (hyp ? m : 0)) * T;
+  for (int t = b - 1; t >= a; --t) {
+    const size_t at = ((size_t)t * G + g) * W + l;
+    const int row = parents[at], token = tokens[at];
+    if (here && t == start) cur = inside(beam0);
+    const int tok = __shfl(token, cur < 0 ? 0 : cur);
+    if (hyp) o[t] = cur < 0 ? pad : (int64_t)tok;
+    cur = hop(row, cur);
+  }
+}
+
+}  // namespace
+
+extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t* done,
+                                  const int32_t* position, const float* fin_scores,
+                                  const int32_t* fin_length, const int32_t* fin_beam,
+                                  const int32_t* fin_token, float* out_scores, int32_t* out_length,
+                                  int32_t* out_done, int64_t* out_ids, int32_t* out_position,
+                                  int32_t* out_parents, float* out_fin_scores,
+                                  int32_t* out_fin_length, int32_t* out_fin_beam,
+                                  int32_t* out_fin_token, int32_t* token_log, int32_t* parent_log,
+                                  const float* cand_score, const int32_t* cand_beam,
+                                  const int64_t* cand_token, const int64_t* ends, int64_t groups,
+                                  int64_t beams, int64_t k, int64_t steps, int64_t n_ends,
+                                  double length_penalty, int early_stopping, int64_t pad,
+                                  void* stream) {
+  if (groups < 0 || groups > 0x7fffffff || beams < 1 || k < 1 || steps < 1 || steps > 0x7fffffff ||
+      n_ends < 0 || n_ends > 0x7fffffff)
+    return ACORN_ERR_SHAPE;
+  if (beams > kMaxBeams || k > kMaxK) return ACORN_ERR_UNSUPPORTED;
+  if (groups == 0) return ACORN_OK;
+  const void* all[] = {scores, length, done, position, fin_scores, fin_length, fin_beam, fin_token,
+                       out_scores, out_length, out_done, out_ids, out_position, out_parents,
+                       out_fin_scores, out_fin_length, out_fin_beam, out_fin_token, token_log,
+                       parent_log, cand_score, cand_beam, cand_token};
+  for (const void* p : all)
+    if (!p) return ACORN_ERR_VALUE;
+  if ((n_ends && !ends) || !(length_penalty > -INFINITY && length_penalty < INFINITY))
+    return ACORN_ERR_VALUE;
+  const BeamFields in = {(float*)scores, (int32_t*)length, (int32_t*)done, nullptr,
+                         (int32_t*)position, nullptr, (float*)fin_scores, (int32_t*)fin_length,
+                         (int32_t*)fin_beam, (int32_t*)fin_token};
+  const BeamFields out = {out_scores, out_length, out_done, out_ids, out_position, out_parents,
+                          out_fin_scores, out_fin_length, out_fin_beam, out_fin_token};
+  beam_advance_kernel<<<dim3((unsigned)groups), dim3(kWave), 0, (hipStream_t)stream>>>(
+      in, out, token_log, parent_log, cand_score, cand_beam, cand_token, ends, (int)groups,
+      (int)beams, (int)k, (int)steps, (int)n_ends, length_penalty, early_stopping, pad);
+  ACORN_LAUNCH_CHECK();
+  return ACORN_OK;
+}
+
+extern "C" int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, int32_t* tables,
+                                  const int32_t* lens, const int32_t* parents, int64_t groups,
+                                  int64_t beams, int64_t table_stride, int64_t layers,
+                                  int64_t num_blocks, int64_t page_size, int64_t kv_heads,
+                                  int64_t head_dim, int64_t elem_size, void* stream) {
+  if (groups < 0 || groups > 65535 || beams < 1 || table_stride < 1 || layers < 1 || num_blocks < 1 ||
+      num_blocks > 0x7fffffff || page_size < 1 || page_size > 65536 || kv_heads < 1 ||
+      kv_heads > 65535 || head_dim < 1 || head_dim > 65536 || table_stride > 0x7fffffff / page_size)
+    return ACORN_ERR_SHAPE;
+  if (beams > kMaxBeams) return ACORN_ERR_UNSUPPORTED;
+  if (groups * beams > 65535 || layers > 0x7fffffff) return ACORN_ERR_SHAPE;
+  const bool tiles = scale_pool != nullptr;
+  if (tiles && (page_size % 16 || elem_size != 1)) return ACORN_ERR_SHAPE;
+  if (!tiles && elem_size != 2 && elem_size != 4) return ACORN_ERR_DTYPE;
+  const int64_t row = kv_heads * head_dim * elem_size;         // a token's bytes
+  if (row % 16 || row * page_size > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
+  if (groups == 0) return ACORN_OK;
+  if (!k_pool || !v_pool || !tables || !lens || !parents) return ACORN_ERR_VALUE;
+  if ((uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16 || (uintptr_t)scale_pool % 16)
+    return ACORN_ERR_VALUE;
+  Pools pools = {};
+  const int64_t pb = row * page_size;
+  if (tiles) {
+    const int per = (int)(page_size * head_dim);
+    pools.p[0] = {(uint8_t*)k_pool, pb, (int)kv_heads, per, (int)(16 * head_dim), 16};
+    pools.p[1] = {(uint8_t*)v_pool, pb, (int)kv_heads, per, (int)(16 * head_dim), 16};
+    pools.p[2] = {(uint8_t*)scale_pool, kv_heads * page_size * 2, (int)kv_heads,
+                  (int)(page_size * 2), 32, 16};
+  } else {
+    pools.p[0] = {(uint8_t*)k_pool, pb, 1, 0, (int)row, 1};
+    pools.p[1] = {(uint8_t*)v_pool, pb, 1, 0, (int)row, 1};
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (beams > 1) {
+    beam_copy_kernel<<<dim3((unsigned)layers, (unsigned)(groups * beams), tiles ? 3 : 2),
+                       dim3(kCopyNT), 0, st>>>(pools, tables, lens, parents, (int)beams,
+                                               (int)page_size, num_blocks, (int)table_stride);
+    ACORN_LAUNCH_CHECK();
+    beam_tables_kernel<<<dim3((unsigned)((table_stride + 255) / 256), (unsigned)groups), dim3(256),
+                         0, st>>>(tables, lens, parents, (int)beams, (int)page_size,
+                                  (int)table_stride);
+    ACORN_LAUNCH_CHECK();
+  }
+  return ACORN_OK;
+}
+
+extern "C" int acorn_beam_trace(const int32_t* tokens, const int32_t* parents,
+                                const int32_t* steps, const int32_t* beams, int64_t* out,
+                                int64_t T, int64_t groups, int64_t W, int64_t M, int64_t pad,
+                                void* stream) {
+  if (T < 0 || T > 0x7fffffff - 64 || groups < 0 || groups > 0x7fffffff || W < 1 || M < 0 ||
+      M > 65535 * (int64_t)kWave)
+    return ACORN_ERR_SHAPE;
+  if (W > kMaxBeams) return ACORN_ERR_UNSUPPORTED;
+  if (T == 0 || groups == 0 || M == 0) return ACORN_OK;
+  if (!tokens || !parents || !steps || !beams || !out) return ACORN_ERR_VALUE;
+  beam_trace_kernel<<<dim3((unsigned)groups, (unsigned)((M + kWave - 1) / kWave)),
+                      dim3(kTraceWaves * kWave), 0, (hipStream_t)stream>>>(
+      tokens, parents, steps, beams, out, (int)T, (int)groups, (int)W, (int)M, pad);
+  ACORN_LAUNCH_CHECK();
+  return ACORN_OK;
+}

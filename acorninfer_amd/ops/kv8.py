@@ -29,10 +29,7 @@ from typing import NamedTuple
 
 import torch
 
-# (the stream's handle without a Stream object around it: a microsecond of a call's ten)
-from torch._C import _cuda_getCurrentRawStream as _raw_stream
-
-from acorninfer_amd._lib import check, dtype_code, lib, ptr, require_gpu
+from acorninfer_amd._lib import check, dtype_code, launch as _call, lib, one_device as _device, ptr
 
 GROUP = 16               # tokens of a tile
 MI355X_CUS = 256
@@ -97,31 +94,6 @@ def _pool(kv: KV8Pages) -> tuple[int, int, int, int]:
     assert k.dtype is v.dtype is s.dtype is torch.uint8 and k.is_contiguous() and \
         v.is_contiguous() and s.is_contiguous(), "pages are contiguous uint8"
     return NB, KV, n // GROUP, G * GROUP
-
-
-def _device(first: torch.Tensor, *tensors: torch.Tensor) -> int:
-    """The index of the one GPU that holds the tensors: a kernel launches on one device's stream
-    and reaches every tensor by its pointer."""
-    dev = first.get_device()
-    for t in tensors:
-        if t.get_device() != dev:
-            require_gpu(first, *tensors)
-            raise AssertionError(f"tensors on {first.device} and {t.device}")
-    if dev < 0:
-        require_gpu(first)
-    return dev
-
-
-def _call(name: str, dev: int, *args) -> None:
-    """Launch on the current stream of device `dev`, with that device current."""
-    fn = getattr(lib(), "acorn_" + name)
-    if torch.cuda.current_device() == dev:
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
-    if rc:
-        check(rc, name)
 
 
 def _check_targets(pages: torch.Tensor, slots: torch.Tensor, rows: int) -> None:

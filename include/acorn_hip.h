@@ -539,6 +539,103 @@ int acorn_paged_prefill_attention_kv8(const void* q, const void* k_tiles, const 
 int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t max_nq, int64_t H, int64_t KV,
                                       int64_t D, int64_t P, int64_t table_stride, int64_t* bytes);
 
+/*
+ * Beam search. G groups (requests) of W beams (1 to 32). No counterpart in the reference.
+ *
+ * acorn_beam_select: the k (1 to 64) best continuations of every group by
+ *   s(w, v) = scores[g, w] + x[w, v] - ln sum_u exp(x[w, u]),
+ * x [G*W, vocab] rows of `dtype`, row_stride elements apart, compared in 64 bits. In falling
+ * order of s, equal ones by beam and then token: out_score [G, k] (s rounded to fp32), out_beam,
+ * out_token. -inf logits are banned tokens, beams of score -inf have only continuations of -inf
+ * and their rows are not read. status [G*W]: 1 for a beam whose score or row holds NaN or +inf
+ * (it counts as one of score -inf), else 0. ws: 8-byte aligned, at least the bytes
+ * acorn_beam_select_workspace reports; contents need not be set, calls that overlap need
+ * workspaces of their own. Deterministic.
+ */
+int acorn_beam_select(const void* logits, int64_t row_stride, const float* scores, int64_t groups,
+                      int64_t beams, int64_t vocab, int64_t k, float* out_score,
+                      int32_t* out_beam, int64_t* out_token, int32_t* status, void* ws,
+                      int64_t ws_bytes, int dtype, void* stream);
+/* *bytes = workspace of acorn_beam_select. No GPU access. */
+int acorn_beam_select_workspace(int64_t groups, int64_t beams, int64_t vocab, int64_t k, int dtype,
+                                int64_t* bytes);
+
+/*
+ * One step of a group's bookkeeping, from its candidates cand_* [G, k] (k <= 64) in falling
+ * order. State per group: length (tokens of the answer so far), done; per beam [G, W]: scores
+ * (sums of log-probabilities), ids and parents (the newest token, and the beam it continues),
+ * position (of the newest token); and the group's W best finished hypotheses in falling order
+ * of s / n^length_penalty: fin_scores (-inf: none), fin_length n (0: none), fin_beam and fin_token
+ * (the last token, and the beam of step n - 2 that it continues). Logs [steps, G, W].
+ * A group that is done, or has `steps` tokens, stays: ids = pad, parents[w] = w, the rest as it
+ * was. Else, with t = length:
+ *   the first W candidates that are above -inf and do not end (token in ends[n_ends]) become the
+ *   beams, their tokens and parents row t of the logs; beams that are left get score -inf, pad, w;
+ *   those among the first W candidates that end join the finished (of equal scores older ones first);
+ *   length and position grow by 1; the group is done where no beam is left, t + 1 == steps, or
+ *   there are W finished and (early_stopping, or the worst is no worse than the best beam's
+ *   score / (t + 1)^length_penalty).
+ * out_* may be the same memory as the state they replace.
+ */
+int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t* done,
+                       const int32_t* position, const float* fin_scores,
+                       const int32_t* fin_length, const int32_t* fin_beam,
+                       const int32_t* fin_token, float* out_scores, int32_t* out_length,
+                       int32_t* out_done, int64_t* out_ids, int32_t* out_position,
+                       int32_t* out_parents, float* out_fin_scores, int32_t* out_fin_length,
+                       int32_t* out_fin_beam, int32_t* out_fin_token, int32_t* token_log,
+                       int32_t* parent_log, const float* cand_score, const int32_t* cand_beam,
+                       const int64_t* cand_token, const int64_t* ends, int64_t groups,
+                       int64_t beams, int64_t k, int64_t steps, int64_t n_ends,
+                       double length_penalty, int early_stopping, int64_t pad, void* stream);
+
+/*
+ * The cache follows the beams: beam w of a group continues beam parents[g, w] (outside [0, W):
+ * itself), with n = lens[g, 0] tokens in the cache. Columns of tables [G*W, table_stride] before
+ * c = n / P become the parent's; where n % P tokens fill a page in part, column c (pages of the
+ * group's beams that differ from one another) is dealt out again: the first child of a beam takes
+ * its page, every further child the page of a beam without children (in order), into which the
+ * tokens are copied, in every layer. Columns behind stay. k_pool, v_pool [layers, num_blocks, P,
+ * KV, D] of elem_size 2 or 4; with scale_pool the 8-bit cache's pools (elem_size 1, layers of the
+ * arrays above), of which tiles that hold a token are copied whole. KV*D*elem_size is a multiple
+ * of 16, pools are 16-byte aligned. A page outside the pool is not copied.
+ */
+int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, int32_t* tables,
+                       const int32_t* lens, const int32_t* parents, int64_t groups, int64_t beams,
+                       int64_t table_stride, int64_t layers, int64_t num_blocks,
+                       int64_t page_size, int64_t kv_heads, int64_t head_dim, int64_t elem_size,
+                       void* stream);
+
+/*
+ * Hypotheses out of the logs tokens, parents [T, G, W]: out[g, m, t] (int64 [G, M, T]) =
+ * tokens[t, g, b_t] for t < steps[g, m], with b of the last step beams[g, m] and
+ * b_{t-1} = parents[t, g, b_t]; pad behind, and before a beam outside [0, W).
+ */
+int acorn_beam_trace(const int32_t* tokens, const int32_t* parents, const int32_t* steps,
+                     const int32_t* beams, int64_t* out, int64_t T, int64_t groups, int64_t W,
+                     int64_t M, int64_t pad, void* stream);
+
+/*
+ * Block tables from lengths: request n holds ceil(lengths[n] / P) blocks (P a power of two, none
+ * for lengths below 1), the next ones of the list blocks[n_blocks]; tables [N, width] get the
+ * first `width` of each, and pad behind them and where the list has ended.
+ */
+int acorn_block_tables(const int32_t* blocks, int64_t n_blocks, const int32_t* lengths,
+                       int32_t* tables, int64_t N, int64_t width, int64_t page_size, int pad,
+                       void* stream);
+
+/*
+ * The slot map of packed rows: request n brings counts[n] rows (none below 1), tokens starts[n]
+ * .. of it. Row r of the packing, token p of request n: seq = n, positions = p, pages =
+ * tables[n, p / P] (-1 past the table's width or for p < 0: the cache's writers skip it), slots =
+ * p % P, lens = p + 1. row0 [N]: each request's first row. Rows from R on have no place, rows
+ * that no request brings stay as they were.
+ */
+int acorn_slot_map(const int32_t* tables, const int32_t* starts, const int32_t* counts,
+                   int32_t* seq, int64_t* positions, int64_t* pages, int64_t* slots, int32_t* lens,
+                   int32_t* row0, int64_t N, int64_t R, int64_t width, int64_t page_size,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

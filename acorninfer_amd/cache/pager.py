@@ -31,6 +31,7 @@ from __future__ import annotations
 import torch
 
 from acorninfer_amd._lib import check, dtype_code, lib, ptr, stream_ptr
+from acorninfer_amd.ops.beam import beam_reorder
 from acorninfer_amd.ops.kv8 import (GROUP, KV8Pages, kv8_gather, kv8_scatter, kv8_supported)
 
 
@@ -144,6 +145,10 @@ class PagedKVCache:
         self.k_pages[layer_idx][rows, slots] = k.to(self.dtype)
         self.v_pages[layer_idx][rows, slots] = v.to(self.dtype)
 
+    def reorder_beams(self, tables: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor) -> None:
+        """The pages follow the beams of a search, in all layers (ops.beam.beam_reorder)."""
+        beam_reorder(self.k_pool, self.v_pool, tables, lens, parents, scale_pool=self.scale_pool)
+
     def scatter_decode(self, views: list["PagedCacheView"], layer_idx: int, k: torch.Tensor,
                        v: torch.Tensor, pages: torch.Tensor, slots: torch.Tensor) -> None:
         """Decode-step batched write (pager.py:87-113): k_pages[l][pages[b], slots[b]] =
@@ -255,6 +260,10 @@ class PagedCacheView:
                              device=c.device, dtype=torch.long)
         c._put(layer_idx, rows, slots, k_new[0].permute(1, 0, 2), v_new[0].permute(1, 0, 2))
         self._lens[layer_idx] = base + s
+
+    def ensure_room(self, n: int) -> None:
+        """`reserve` without the list: room for n more tokens after layer 0's length."""
+        self._grow_to((self.seq_len + n + self.cache.page_size - 1) // self.cache.page_size)
 
     def reserve(self, n: int) -> list[tuple[int, int]]:
         """Make room for n more tokens after layer 0's length; return each

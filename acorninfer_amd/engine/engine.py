@@ -22,6 +22,7 @@ import torch
 
 from acorninfer_amd.cache.pager import (BlockAllocator, PagedCacheView, PagedKV8Cache,
                                         PagedKVCache)
+from acorninfer_amd.engine.beam import BeamSearch, Hypothesis
 from acorninfer_amd.engine.graph_runner import BUCKETS, DecodeGraphRunner
 from acorninfer_amd.engine.scheduler import Scheduler
 from acorninfer_amd.engine.sequence import RequestStatus, Sequence
@@ -74,6 +75,8 @@ class Engine:
         self._views: dict[int, PagedCacheView] = {}
         self._next_id = 0
         self._gen = torch.Generator(device=model.device).manual_seed(seed + 1)
+        self._capture = capture
+        self._searches: dict[tuple, BeamSearch] = {}
 
     def submit(self, prompt_ids: list[int], sampling: SamplingParams, *, max_tokens: int,
                eos_ids: frozenset[int] | None = None) -> int:
@@ -168,6 +171,21 @@ class Engine:
             seq.stop_reason = reason
             seq.status = RequestStatus.FINISHED
         outputs.append(TokenOutput(seq.seq_id, token_id, reason is not None, reason))
+
+    def beam_search(self, prompts: list[list[int]], *, beams: int, max_tokens: int,
+                    length_penalty: float = 1.0, early_stopping: bool = False,
+                    eos_ids: frozenset[int] | None = None) -> list[list[Hypothesis]]:
+        """The best answers of every prompt by beam search (engine/beam.py), run to its end between
+        two steps on this engine's cache. Requests in flight keep their blocks; BlockExhausted
+        where too few are free, and nothing has changed then."""
+        key = (beams, max_tokens, length_penalty, early_stopping,
+               frozenset(QWEN3_EOS_IDS if eos_ids is None else eos_ids))
+        if key not in self._searches:
+            self._searches[key] = BeamSearch(
+                self.model, self.cache, self.allocator, beams=beams, max_tokens=max_tokens,
+                max_model_len=self.max_model_len, eos_ids=key[-1], length_penalty=length_penalty,
+                early_stopping=early_stopping, capture=self._capture)
+        return self._searches[key].search(prompts)
 
     def drop(self, seq_id: int) -> None:
         """Forget a finished sequence's record (the caller consumed its output)."""

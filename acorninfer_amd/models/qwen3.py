@@ -43,6 +43,7 @@ from acorninfer_amd._lib import (BF16, WFMT_BF16, WFMT_BF16B, WFMT_W4, WFMT_W4B,
 from acorninfer_amd.config import Qwen3Config
 from acorninfer_amd.ops.kv8 import kv8_attention_supported, kv8_splits, prefill_workspace_kv8
 from acorninfer_amd.ops.paged_attention import prefill_supported, prefill_workspace
+from acorninfer_amd.ops.request_maps import block_tables, slot_map
 from acorninfer_amd.quant import quantize as Q
 from acorninfer_amd.sampler import sample_workspace
 
@@ -536,8 +537,11 @@ class Qwen3DecodeModel:
              num_blocks: int, page_size: int, *, fused_attn: bool = True,
              head_rows: torch.Tensor | None = None,
              segments: "PrefillSegments | None" = None,
-             scale_pool: torch.Tensor | None = None) -> torch.Tensor | None:
+             scale_pool: torch.Tensor | None = None, sample: bool = True) -> torch.Tensor | None:
         """Launch one decode step on the current stream.
+
+        sample=False ends with buf.logits: the caller chooses the next tokens
+        (buf.next_ids, buf.logprob and buf.status are not written).
 
         scale_pool: the pools are an 8-bit cache's (PagedKV8Cache); the qkv
         epilogue then quantises the new k/v (acorn_qkv_epilogue_kv8) and
@@ -725,6 +729,8 @@ class Qwen3DecodeModel:
             return out
         self.lm_head.launch(buf.normed, B, buf.cfgs["lm_head"], out=buf.logits,
                             part=buf.ws_lm, stream=st)
+        if not sample:
+            return None
         # next token: greedy rows (temperature 0) take the argmax, the others
         # temperature -> top-k -> top-p -> inverse-CDF draw of their uniform
         check(L.acorn_sample_split(ptr(buf.logits), B, cfg.vocab_size, dtype_code(buf.logits),
@@ -1033,28 +1039,22 @@ class Qwen3DecodeModel:
         cfg = self.cfg
         tiled = self.tiled_prefill and prefill_supported(
             self.dtype, cfg.head_dim, P, cfg.num_attention_heads, cfg.num_key_value_heads)
-        targets = [v.reserve(n) for v, n in zip(views, chunk_lens)]
+        for v, n in zip(views, chunk_lens):
+            v.ensure_room(n)
+        dev = self.device
+        # one copy to the device: every view's blocks, then tokens its table holds | starts | rows
         W = max(len(v.table) for v in views)
-        ids, pos, pages, slots, lens, tabs = [], [], [], [], [], []
-        for i, (v, s, n) in enumerate(zip(views, starts, chunk_lens)):
-            ids.append(input_ids[i, :n].to(torch.int64).cpu())
-            pos += list(range(s, s + n))
-            pages += [p for p, _ in targets[i]]
-            slots += [q for _, q in targets[i]]
-            lens += list(range(s + 1, s + n + 1))
-            row = torch.zeros(W, dtype=torch.int32)
-            row[:len(v.table)] = torch.tensor(v.table, dtype=torch.int32)
-            tabs.append(row)
-        R = len(pos)
-        ids_all = torch.cat(ids)
-        pos_all = torch.tensor(pos, dtype=torch.int64)
-        pages_all = torch.tensor(pages, dtype=torch.int64)
-        slots_all = torch.tensor(slots, dtype=torch.int64)
-        lens_all = torch.tensor(lens, dtype=torch.int32)
-        seq_tabs = torch.stack(tabs)                                  # [N, W]
+        R = sum(chunk_lens)
+        meta = torch.tensor([b for v in views for b in v.table] +
+                            [len(v.table) * P for v in views] + list(starts) + list(chunk_lens),
+                            dtype=torch.int32).to(dev)
+        blocks, (held, first_pos, counts) = meta[:-3 * N], meta[-3 * N:].view(3, N)
+        seq_tabs = block_tables(blocks, held, P, W)                   # [N, W]
+        rows = slot_map(seq_tabs, first_pos, counts, P, R)
+        ids_all = torch.cat([input_ids[i, :n] for i, n in enumerate(chunk_lens)]).to(
+            device=dev, dtype=torch.int64)
         first = torch.tensor([0] + list(chunk_lens), dtype=torch.int64).cumsum(0)
         last = first[1:] - 1
-        dev = self.device
         # Rows run in blocks of at most EXTEND_MAX_ROWS, in order: a block's
         # layer-l attention reads the k/v that earlier blocks wrote at layer l,
         # so this is chunked prefill over the packed rows.
@@ -1083,18 +1083,15 @@ class Qwen3DecodeModel:
                                                        kv8_page=kv8_page))
             buf = self._extend_buf[1]
             buf.ids.copy_(ids_all[r0:r1])
-            buf.positions.copy_(pos_all[r0:r1])
-            buf.pages.copy_(pages_all[r0:r1])
-            buf.slots.copy_(slots_all[r0:r1])
+            buf.positions.copy_(rows.positions[r0:r1])
+            buf.pages.copy_(rows.pages[r0:r1])
+            buf.slots.copy_(rows.slots[r0:r1])
             segs = None
             if tiled:
                 segs = PrefillSegments.for_rows(first, starts, seq_tabs, r0, r1, dev)
             else:
-                buf.lens.copy_(lens_all[r0:r1])
-                for i in range(N):                 # each sequence's table on its rows
-                    a, b = max(int(first[i]), r0), min(int(first[i + 1]), r1)
-                    if a < b:
-                        buf.tables[a - r0:b - r0].copy_(seq_tabs[i].expand(b - a, W))
+                buf.lens.copy_(rows.lens[r0:r1])
+                torch.index_select(seq_tabs, 0, rows.seq[r0:r1], out=buf.tables)
             heads = last[(last >= r0) & (last < r1)] - r0
             outs.append(self.step(buf, cache.k_pool, cache.v_pool, cache.num_blocks, P,
                                   fused_attn=False, head_rows=heads.to(dev), segments=segs,
@@ -1122,7 +1119,8 @@ class PrefillSegments:
     def for_rows(cls, first: torch.Tensor, starts: list[int], seq_tabs: torch.Tensor,
                  r0: int, r1: int, device) -> "PrefillSegments":
         """Rows [r0, r1) of a packing where sequence i holds rows
-        first[i] .. first[i + 1] - 1 from KV position starts[i]."""
+        first[i] .. first[i + 1] - 1 from KV position starts[i], with block
+        table seq_tabs[i] (on the device)."""
         sel, row0, pos0, nq = [], [], [], []
         for i in range(len(starts)):
             a, b = max(int(first[i]), r0), min(int(first[i + 1]), r1)
@@ -1131,11 +1129,9 @@ class PrefillSegments:
                 row0.append(a - r0)
                 pos0.append(starts[i] + a - int(first[i]))
                 nq.append(b - a)
-        meta = torch.tensor([row0, pos0, nq], dtype=torch.int32)
-        blob = torch.cat([meta.reshape(-1), seq_tabs[sel].reshape(-1)]).to(device)
-        n = len(sel)
-        return cls(blob[3 * n:].view(n, seq_tabs.shape[1]), blob[0:n], blob[n:2 * n],
-                   blob[2 * n:3 * n], n, max(nq))
+        meta = torch.tensor([row0, pos0, nq], dtype=torch.int32).to(device)
+        # (every sequence has rows, so those of a run of rows follow one another)
+        return cls(seq_tabs[sel[0]:sel[-1] + 1], meta[0], meta[1], meta[2], len(sel), max(nq))
 
 
 def _dense_linear(w: torch.Tensor, dtype: torch.dtype) -> QLinear:

@@ -46,17 +46,6 @@ template <> __device__ __forceinline__ float vec_elem<float>(const bs_u32x4& w, 
   return __uint_as_float(w[e]);
 }
 
-// The vector without its element 0.
-template <typename T>
-__device__ __forceinline__ void drop_elem(bs_u32x4& w) {
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = w[i] >> 16 | (i < 3 ? w[i + 1] << 16 : 0u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) w[i] = w[i + 1];
-  }
-}
 // A vector as the compiler has not seen it: what it made of it before is not kept in registers.
 __device__ __forceinline__ void forget(bs_u32x4& w) { asm volatile("" : "+v"(w)); }
 
@@ -284,19 +273,18 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     const float floor = unorder32((uint32_t)(least >> 32));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const bool any = vmax[u] >= floor;
-      if (__ballot(any) == 0) continue;
+      if (__ballot(vmax[u] >= floor) == 0) continue;
       forget(x[u]);
-      bs_u32x4 w = x[u];
-      uint32_t i = (at0 + u * kPartNT) * E;
-#pragma unroll 1
-      for (int e = 0; e < E; ++e, ++i) {
-        const u64 key = key_of(vec_elem<T>(w, 0), i);
-        if (any && key >= least) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kHeld) held[at] = key;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = vec_elem<T>(x[u], e);
+        if (f >= floor) {
+          const u64 key = key_of(f, (at0 + u * kPartNT) * E + e);
+          if (key >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kHeld) held[at] = key;
+          }
         }
-        drop_elem<T>(w);
       }
     }
     __syncthreads();

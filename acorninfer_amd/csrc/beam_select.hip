@@ -3,13 +3,13 @@
 //   s(w, v) = score[w] + x[w, v] - ln sum_u exp(x[w, u]),
 // sorted, equal ones in order of w and then v.
 //
-// Two launches. beam_part_kernel reads the logits once: a workgroup holds a piece of one
-// row in registers and leaves the piece's maximum, its sum of exponentials and its k
-// largest logits. Within a row the order of s is the order of x, so a piece needs
-// neither the row's sum nor the beam's score. beam_join_kernel, one workgroup per
-// group, joins a row's pieces, then the rows, by s in 64 bits: beams are compared
-// through sums over the whole vocabulary, and 32 bits of s (2^-20 at 10) would tie
-// or turn round what the logits tell apart.
+// Two launches. beam_part_kernel reads the logits once: a workgroup takes a piece of one
+// row and leaves the piece's maximum, its sum of exponentials and its k largest logits,
+// sorted. Within a row the order of s is the order of x, so a piece needs neither the
+// row's sum nor the beam's score. beam_join_kernel, one workgroup per group, joins a
+// row's pieces, then the rows, by s in 64 bits: beams are compared through sums over the
+// whole vocabulary, and 32 bits of s (2^-20 at 10) would tie or turn round what the
+// logits tell apart.
 //
 // A value's key is its order-preserving image in 32 bits, then ~token: keys differ
 // from one another, the larger is the better, and the k largest do not depend on
@@ -29,7 +29,8 @@ typedef uint32_t bs_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPartNT = 256, kPartWaves = kPartNT / kWave;
 constexpr int kMaxBeams = 32, kMaxK = 64;
-constexpr int kHeld = 1024;                    // candidates of a piece that are kept before they are sorted
+constexpr int kHeld = 256;                     // a wave's candidates that are kept until they are sorted
+constexpr int kQueue = 5 * kWave;              // a wave's vectors that may hold candidates
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHuge = 1e6f;                   // to here x log2 e as a float is off by less than 1 / 8
 constexpr uint32_t kLowest = 0x007FFFFFu;      // order32 of -inf
@@ -45,6 +46,7 @@ template <> __device__ __forceinline__ float vec_elem<_Float16>(const bs_u32x4& 
 template <> __device__ __forceinline__ float vec_elem<float>(const bs_u32x4& w, int e) {
   return __uint_as_float(w[e]);
 }
+
 
 // A vector as the compiler has not seen it: what it made of it before is not kept in registers.
 __device__ __forceinline__ void forget(bs_u32x4& w) { asm volatile("" : "+v"(w)); }
@@ -68,7 +70,10 @@ __device__ __forceinline__ u64 key_of(float x, uint32_t token) {
   return (u64)order32(x) << 32 | (uint32_t)~token;
 }
 
-// ---- lists across a wave ----------------------------------------------------------------------
+// ---- across a wave ----------------------------------------------------------------------------
+// (What runs once is kept short: a launch finds the instruction caches cold, and code that is jumped
+// to costs a trip to memory for every line.)
+
 // The value of lane ^ D, D a power of two, without the LDS: DPP within rows of 16, else the
 // swaps of rows and halves (of a value with itself: the even and the odd rows' in every lane).
 template <int D>
@@ -104,29 +109,18 @@ __device__ __forceinline__ u64 read_lane(u64 v, int lane) {
   return (u64)read_lane((uint32_t)(v >> 32), lane) << 32 | read_lane((uint32_t)v, lane);
 }
 
-// An entry of a group's list: s as a key, then its place (beam * 64 + rank in the beam's list): the
-// larger key first, of equal ones the lower place.
-struct Entry {
-  u64 key;
-  uint32_t place;
-};
-template <int D>
-__device__ __forceinline__ Entry lane_xor(const Entry& e, int lane) {
-  return {lane_xor<D>(e.key, lane), lane_xor<D>(e.place, lane)};
-}
-__device__ __forceinline__ bool before(uint32_t a, uint32_t b) { return a > b; }
-__device__ __forceinline__ bool before(u64 a, u64 b) { return a > b; }
-__device__ __forceinline__ bool before(const Entry& a, const Entry& b) {
-  return a.key > b.key || (a.key == b.key && a.place < b.place);
+__device__ __forceinline__ int lanes_before(u64 mask) {        // set bits below this lane's
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
 // One step of a bitonic network over the wave: of lanes that differ by D, the first keeps the
-// better value where `falls`, the worse where not.
+// larger value where `falls`, the smaller where not.
 template <int D, typename U>
-__device__ __forceinline__ U exchange(const U& v, int lane, bool falls) {
+__device__ __forceinline__ U exchange(U v, int lane, bool falls) {
   const U o = lane_xor<D>(v, lane);
-  const bool better = ((lane & D) == 0) == falls;
-  return before(o, v) == better ? o : v;
+  const bool larger = ((lane & D) == 0) == falls;
+  return (o > v) == larger ? o : v;
 }
 template <int D, typename U>
 __device__ __forceinline__ U exchanges(U v, int lane, bool falls) {
@@ -134,23 +128,25 @@ __device__ __forceinline__ U exchanges(U v, int lane, bool falls) {
   if constexpr (D > 1) v = exchanges<D / 2>(v, lane, falls);
   return v;
 }
-// The lanes' values in falling order, or in rising order.
-template <bool FALLS, typename U>
+// The lanes' values in rising order.
+template <typename U>
 __device__ __forceinline__ U sort_wave(U v, int lane) {
-  v = exchanges<1>(v, lane, ((lane & 2) == 0) == FALLS);
-  v = exchanges<2>(v, lane, ((lane & 4) == 0) == FALLS);
-  v = exchanges<4>(v, lane, ((lane & 8) == 0) == FALLS);
-  v = exchanges<8>(v, lane, ((lane & 16) == 0) == FALLS);
-  v = exchanges<16>(v, lane, ((lane & 32) == 0) == FALLS);
-  return exchanges<32>(v, lane, FALLS);
+  v = exchanges<1>(v, lane, (lane & 2) != 0);
+  v = exchanges<2>(v, lane, (lane & 4) != 0);
+  v = exchanges<4>(v, lane, (lane & 8) != 0);
+  v = exchanges<8>(v, lane, (lane & 16) != 0);
+  v = exchanges<16>(v, lane, (lane & 32) != 0);
+  return exchanges<32>(v, lane, false);
 }
 // The 64 best of a falling list and a rising one, falling.
 template <typename U>
-__device__ __forceinline__ U merge_wave(const U& top, const U& other, int lane) {
-  return exchanges<32>(before(other, top) ? other : top, lane, true);
+__device__ __forceinline__ U merge_wave(U top, U other, int lane) {
+  return exchanges<32>(max(top, other), lane, true);
 }
 
 // The sum, or another fold, over the wave, in every lane.
+__device__ __forceinline__ uint32_t from_bits(uint32_t v, uint32_t) { return v; }
+__device__ __forceinline__ uint32_t bits_of(uint32_t v) { return v; }
 __device__ __forceinline__ float from_bits(uint32_t v, float) { return __uint_as_float(v); }
 __device__ __forceinline__ double from_bits(u64 v, double) { return __builtin_bit_cast(double, v); }
 __device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v); }
@@ -165,23 +161,32 @@ __device__ __forceinline__ F over_lanes(F v, int lane, Op op) {
 // ---- pieces -----------------------------------------------------------------------------------
 // A row in vectors of 16 bytes from its first element, whatever that one's alignment (the loads
 // are by element): what a lane adds up, and in which order, depends on the row's values alone, so
-// that equal rows have equal sums. Piece i takes vectors i * NV * kPartNT .. , NV to a lane.
+// that equal rows have equal sums. Piece i takes vectors i * NV * kPartNT .. , NV to a lane, all
+// of them on their way before the first is worked off.
 //
-// The k largest: at least k values of the piece reach the k-th largest of the lanes' own maxima,
-// few more do as a rule, and these are gathered in LDS and sorted by one wave. Where more than
-// kHeld reach it (values in order, or many alike), the k-th of those that were gathered takes its
-// place: keys are different, so each time the gathered ones but k drop out.
+// Candidates. `least`, which at least k values of the piece reach and few more do as a rule, comes
+// from the lanes' maxima: the k-th largest of a wave's, or what k / 4 of each wave's reach. Vectors
+// whose maximum reaches it (some 30 of a piece at k = 16) are queued in LDS and looked at one to a
+// lane, and what is found is sorted by one wave. Where a wave finds more than kHeld (values in
+// order, or many alike), the k-th largest of those that were held takes its place: keys are
+// different, so each time the ones held but k drop out.
+struct Piece {
+  float m, s;                                                  // the maximum, sum exp(x - m)
+};
+
 template <typename T, int NV>
 __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     const T* __restrict__ logits, int64_t row_stride, const float* __restrict__ scores, int V,
-    int k, u64* __restrict__ lists, float2* __restrict__ sums) {
+    int k, u64* __restrict__ lists, Piece* __restrict__ pieces) {
 #pragma clang fp contract(off)
   constexpr int E = 16 / sizeof(T);
-  __shared__ u64 held[kHeld];
-  __shared__ uint32_t maxima[kPartWaves][kWave];
+  __shared__ u64 held[kPartWaves][kHeld];
+  __shared__ bs_u32x4 queue[kPartWaves][kQueue];
+  __shared__ uint32_t first[kPartWaves][kQueue];               // their first tokens
   __shared__ float wave_m[kPartWaves], wave_s[kPartWaves];
+  __shared__ uint32_t some[kPartWaves], most[kPartWaves];
+  __shared__ int found[kPartWaves];
   __shared__ u64 limit;
-  __shared__ int count;
   const int row = blockIdx.y, piece = blockIdx.x, C = gridDim.x;
   const float score = scores[row];
   if (!(score > -INFINITY && score < INFINITY)) return;        // no such beam: nothing is read
@@ -201,23 +206,26 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     for (int u = 0; u < NV; ++u)
       __builtin_memcpy(&x[u], base + min((uint32_t)(tid + u * kPartNT) * 16u, last), 16);
   }
-  if (p0 + NV * kPartNT > full) {                              // the row ends in this piece
+  // the row's last elements, and nothing behind them
+  auto ending = [&](int j) {
     T r[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) r[e] = (T)-INFINITY;
-    bs_u32x4 none, rest;
-    __builtin_memcpy(&none, r, 16);
 #pragma unroll
     for (int e = 0; e < E - 1; ++e)
-      if (e < V % E) r[e] = p[(int64_t)full * E + e];
-    __builtin_memcpy(&rest, r, 16);
+      if (j == full && e < V % E) r[e] = p[(int64_t)full * E + e];
+    bs_u32x4 w;
+    __builtin_memcpy(&w, r, 16);
+    return w;
+  };
+  if (p0 + NV * kPartNT > full) {                              // the row ends in this piece
+    const bs_u32x4 none = ending(full + 1), rest = ending(full);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int j = p0 + tid + u * kPartNT;
       x[u] = j < full ? x[u] : j == full ? rest : none;
     }
   }
-  if (tid == 0) count = 0;
 
   // The lane's maximum m and s = sum exp(x - m), as powers of 2 of x log2 e - R, R the running
   // maximum's x log2 e as a float, so that one fma with one rounding makes the exponent. NaN and
@@ -247,69 +255,98 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     const float ref = m == -INFINITY ? 0.f : m;
     s = 0.f;
 #pragma unroll
-    for (int u = 0; u < NV; ++u)
+    for (int u = 0; u < NV; ++u) {
+      forget(x[u]);
 #pragma unroll
       for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((vec_elem<T>(x[u], e) - ref) * kLog2e);
+    }
   }
-  const uint32_t sorted = sort_wave<true>(order32(m), lane);
-  maxima[wid][lane] = sorted;
-  const float mw = unorder32(read_lane(sorted, 0)), refw = mw == -INFINITY ? 0.f : mw;
+
+  const uint32_t rising = sort_wave(order32(m), lane);
+  const float mw = unorder32(read_lane(rising, kWave - 1)), refw = mw == -INFINITY ? 0.f : mw;
   const float sw = over_lanes(s * __builtin_amdgcn_exp2f((m - refw) * kLog2e), lane,
                               [](float a, float b) { return a + b; });
   if (lane == 0) {
     wave_m[wid] = mw;
     wave_s[wid] = sw;
+    some[wid] = read_lane(rising, kWave - (k + kPartWaves - 1) / kPartWaves);
+    most[wid] = read_lane(rising, kWave - k);
   }
   __syncthreads();
-  uint32_t all = maxima[0][lane];
-#pragma unroll
-  for (int w = 1; w < kPartWaves; ++w) all = merge_wave(all, maxima[w][kWave - 1 - lane], lane);
-  u64 least = (u64)max(read_lane(all, k - 1), kLowest + 1) << 32;
+  u64 least = (u64)max(max(min(min(some[0], some[1]), min(some[2], some[3])),
+                           max(max(most[0], most[1]), max(most[2], most[3]))), kLowest + 1) << 32;
 
-  u64 top = 0;
+  const int64_t at = (int64_t)row * C + piece;
   for (;;) {
-    int at0 = p0 + tid;
-    asm volatile("" : "+v"(at0));
     const float floor = unorder32((uint32_t)(least >> 32));
+    int n = 0;                                                 // found by this wave
+    uint32_t todo = (uint32_t)((1ull << NV) - 1);              // its vectors (a bit for each of a lane's)
+    while (todo) {
+      int q = 0;                                               // queued
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      if (__ballot(vmax[u] >= floor) == 0) continue;
-      forget(x[u]);
+      for (int u = 0; u < NV; ++u) {
+        if (NV * kWave > kQueue && (!(todo >> u & 1) || q > kQueue - kWave)) continue;
+        todo &= ~(1u << u);
+        const bool any = vmax[u] >= floor;
+        const u64 mask = __ballot(any);
+        if (mask == 0) continue;
+        if (any) {
+          const int i = q + lanes_before(mask);
+          queue[wid][i] = x[u];
+          first[wid][i] = (uint32_t)(p0 + tid + u * kPartNT) * E;
+        }
+        q += __popcll(mask);
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (int i = lane; i < (q + kWave - 1) / kWave * kWave; i += kWave) {
+        const bs_u32x4 w = queue[wid][min(i, kQueue - 1)];
+        const uint32_t token = first[wid][min(i, kQueue - 1)];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float f = vec_elem<T>(x[u], e);
-        if (f >= floor) {
-          const u64 key = key_of(f, (at0 + u * kPartNT) * E + e);
-          if (key >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kHeld) held[at] = key;
-          }
+        for (int e = 0; e < E; ++e) {
+          const u64 key = key_of(vec_elem<T>(w, e), token + e);
+          const bool in = i < q && key >= least;
+          const u64 mask = __ballot(in);
+          const int to = n + lanes_before(mask);
+          if (in && to < kHeld) held[wid][to] = key;
+          n += __popcll(mask);
         }
       }
+      __builtin_amdgcn_wave_barrier();
     }
+    if (lane == 0) found[wid] = n;
     __syncthreads();
-    const int n = count;
-    if (wid == 0) {
-      top = 0;
-      for (int i = 0; i < min(n, kHeld); i += kWave) {
-        const u64 v = i + lane < min(n, kHeld) ? held[i + lane] : 0;
-        if (__ballot(v > read_lane(top, k - 1)) == 0) continue;
-        top = i == 0 ? sort_wave<true>(v, lane) : merge_wave(top, sort_wave<false>(v, lane), lane);
-      }
-      if (lane == 0) {
-        limit = read_lane(top, k - 1);
-        count = 0;
-      }
+    int end[kPartWaves];                                       // of the waves' candidates in a row
+    bool more = false;
+#pragma unroll
+    for (int w = 0; w < kPartWaves; ++w) {
+      more |= found[w] > kHeld;
+      end[w] = (w ? end[w - 1] : 0) + min(found[w], kHeld);
     }
-    if (n <= kHeld) break;
+    u64 top = 0;
+    if (wid == 0) {
+#pragma unroll 1
+      for (int i = 0; i < end[kPartWaves - 1]; i += kWave) {
+        const int j = i + lane;
+        int w = 0, from = j;
+#pragma unroll
+        for (int c = 0; c < kPartWaves - 1; ++c)
+          if (j >= end[c]) w = c + 1, from = j - end[c];
+        const u64 v = j < end[kPartWaves - 1] ? held[w][from] : 0;
+        if (__ballot(v > read_lane(top, k - 1)) == 0) continue;
+        top = merge_wave(top, sort_wave(v, lane), lane);
+      }
+      if (lane == 0) limit = read_lane(top, k - 1);
+    }
+    if (!more) {
+      if (wid == 0 && lane < k) lists[at * k + lane] = top;
+      break;
+    }
     __syncthreads();
     least = limit;
-    __syncthreads();                                           // (count is 0 for all)
+    __syncthreads();                                           // (before found is written again)
   }
-  if (wid != 0) return;
-  const int64_t at = (int64_t)row * C + piece;
-  if (lane < k) lists[at * k + lane] = top;
-  if (lane == 0) {
+  if (tid == kPartNT - 1) {
     float M = wave_m[0], S = wave_s[0];
 #pragma unroll
     for (int w = 1; w < kPartWaves; ++w) {
@@ -318,32 +355,35 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
           wave_s[w] * __builtin_amdgcn_exp2f((wave_m[w] - r) * kLog2e);
       M = n;
     }
-    sums[at] = make_float2(M, S);
+    pieces[at] = Piece{M, S};
   }
 }
 
 // ---- the join ---------------------------------------------------------------------------------
-constexpr int kJoinWaves = 16, kAhead = 4;
+constexpr int kJoinWaves = 16;
+constexpr int kAhead = 4;                      // loads of a lane in flight
+constexpr int kSide = 4;                       // rows that are searched side by side
 
-// A wave per row: the sum of its pieces, and its k best out of their lists. Then wave 0 takes the
-// group's best of the rows'.
+// A wave per row: the sum of its pieces, and its k best out of their lists, sorted. An entry's
+// place in the group's list is its place in its row's and the numbers of entries before it in
+// the other rows', found by halving.
 __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
-    const u64* __restrict__ lists, const float2* __restrict__ sums,
+    const u64* __restrict__ lists, const Piece* __restrict__ pieces,
     const float* __restrict__ scores, int W, int V, int k, int C, float* __restrict__ out_score,
     int32_t* __restrict__ out_beam, int64_t* __restrict__ out_token, int32_t* __restrict__ status) {
-  __shared__ uint32_t tokens[kMaxBeams][kWave];
-  __shared__ u64 keys[kMaxBeams][kWave];
+  __shared__ uint32_t tokens[kMaxBeams][kMaxK];
+  __shared__ u64 keys[kMaxBeams][kMaxK];                       // s, 0: no entry
   __shared__ u64 reach[kJoinWaves][(kAhead + 1) * kWave];      // of a row's entries, those that may count
   const int g = blockIdx.x, lane = threadIdx.x % kWave, wid = threadIdx.x / kWave;
   const int waves = blockDim.x / kWave;
   for (int w = wid; w < W; w += waves) {
     const int64_t row = (int64_t)g * W + w;
-    const float score = scores[row];
-    // (the first loads together: what they find of a row that was not read is not used)
-    const float2* sp = sums + row * C;
+    const Piece* pc = pieces + row * C;
     const u64* lp = lists + row * C * k;
     const int total = C * k;
-    const float2 ms0 = sp[min(lane, C - 1)];
+    const float score = scores[row];
+    // (the first loads together: what they find of a row that was not read is not used)
+    const Piece b = pc[min(lane, C - 1)];
     const uint32_t head = (uint32_t)(lp[(int64_t)min(lane, C - 1) * k] >> 32);
     u64 ahead[kAhead];
 #pragma unroll
@@ -352,14 +392,14 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     double ref = 0.0, log_sum = 0.0;           // ln sum exp(x) = ref + log_sum
     u64 top = 0;
     if (live) {
-      float M = lane < C ? ms0.x : -INFINITY;
-      for (int c = lane + kWave; c < C; c += kWave) M = fmaxf(M, sp[c].x);
+      float M = lane < C ? b.m : -INFINITY;
+      for (int c = lane + kWave; c < C; c += kWave) M = fmaxf(M, pc[c].m);
       M = over_lanes(M, lane, [](float a, float b) { return fmaxf(a, b); });
       ref = M == -INFINITY ? 0.0 : (double)M;
       double S = 0.0;
       for (int c = lane; c < C; c += kWave) {
-        const float2 ms = c < kWave ? ms0 : sp[c];
-        S += (double)ms.y * exp2(((double)ms.x - ref) * (double)kLog2e);
+        const Piece e = c < kWave ? b : pc[c];
+        S += (double)e.s * exp2(((double)e.m - ref) * (double)kLog2e);
       }
       S = over_lanes(S, lane, [](double a, double b) { return a + b; });
       if (!(S == S)) bad = true;
@@ -369,69 +409,84 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     }
     if (live) {
       // lists begin with their largest: at least k entries reach the k-th of (the first 64 of) those
-      const uint32_t reaches = sort_wave<true>(lane < C ? head : 0u, lane);
-      const u64 least = max((u64)read_lane(reaches, k - 1) << 32, (u64)1);
+      const uint32_t reaches = C < k ? 0u : read_lane(sort_wave(lane < C ? head : 0u, lane), kWave - k);
+      const u64 least = max((u64)reaches << 32, (u64)1);
       u64* buf = reach[wid];
       int n = 0;
-      auto flush = [&]() {
-        __builtin_amdgcn_wave_barrier();
-        n -= kWave;
-        const u64 v = n + lane >= 0 ? buf[n + lane] : 0;
-        n = max(n, 0);
-        __builtin_amdgcn_wave_barrier();
-        top = merge_wave(top, sort_wave<false>(v, lane), lane);
-      };
+#pragma unroll 1
       for (int i0 = 0; i0 < total; i0 += kAhead * kWave) {
+        const bool rest = i0 + kAhead * kWave >= total;
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
           const int i = i0 + a * kWave + lane;
           const bool in = i < total && ahead[a] >= least;
           const u64 mask = __ballot(in);
-          if (in) buf[n + __popcll(mask & ((1ull << lane) - 1))] = ahead[a];
+          if (in) buf[n + lanes_before(mask)] = ahead[a];
           n += __popcll(mask);
           ahead[a] = lp[min(i + kAhead * kWave, total - 1)];
         }
-        while (n >= kWave) flush();
+#pragma unroll 1
+        while (n >= kWave || (n > 0 && rest)) {                // 64 of them into the list
+          __builtin_amdgcn_wave_barrier();
+          n -= kWave;
+          const u64 e = n + lane >= 0 ? buf[n + lane] : 0;
+          top = merge_wave(top, sort_wave(e, lane), lane);
+          __builtin_amdgcn_wave_barrier();
+        }
       }
-      if (n > 0) flush();
     }
-    // behind the row's tokens above -inf (all of them are in the list, if there are fewer than k):
-    // the lowest others, at -inf
-    const uint32_t token = ~(uint32_t)top;
-    const int have = live ? __popcll(__ballot(top != 0)) : 0;
+    const int have = live ? min(__popcll(__ballot(top != 0)), k) : 0;
+    uint32_t token = ~(uint32_t)top;
     u64 key = 0;
-    uint32_t shown = token;
-    if (lane < have) {
+    if (lane < have)
       // (x - ref first: where logits are of the type's lowest value, their sum would swallow log_sum)
       key = order64((double)score + (((double)unorder32((uint32_t)(top >> 32)) - ref) - log_sum));
-    } else {
-      key = order64(-INFINITY);
-      shown = lane - have;
+    if (lane < k) {
+      keys[w][lane] = key;
+      tokens[w][lane] = token;
     }
-    if (have > 0 && have < min(k, V)) {
-      const uint32_t rising = sort_wave<false>(lane < have ? token : 0xFFFFFFFFu, lane);
-      for (int i = 0; i < have; ++i) shown += lane >= have && read_lane(rising, i) <= shown;
+    __builtin_amdgcn_wave_barrier();
+    if (lane >= have && lane < k) {
+      // behind the row's tokens above -inf (all of them are here, if they are fewer than k): the
+      // lowest others, at -inf: past as many as lie at or below them
+      token = lane - have;
+      for (bool moved = have > 0; moved;) {
+        uint32_t t = lane - have;
+        for (int j = 0; j < have; ++j) t += tokens[w][j] <= token;
+        moved = t != token;
+        token = t;
+      }
+      keys[w][lane] = lane < V ? order64(-INFINITY) : 0;
+      tokens[w][lane] = token;
     }
-    keys[w][lane] = lane < min(k, V) ? key : 0;
-    tokens[w][lane] = shown;
     if (lane == 0) status[row] = bad;
   }
   __syncthreads();
-  if (wid != 0) return;
-  Entry best = {0, 0xFFFFFFFFu};
-  for (int i = 0; i < W * k; i += kWave) {
-    const int at = i + lane, w = at / k, r = at % k;
-    const bool on = at < W * k;
-    Entry e = {on ? keys[w][r] : 0, on ? (uint32_t)(w * kWave + r) : 0xFFFFFFFFu};
-    const Entry last = {read_lane(best.key, k - 1), read_lane(best.place, k - 1)};
-    if (__ballot(before(e, last)) == 0) continue;
-    best = i == 0 ? sort_wave<true>(e, lane) : merge_wave(best, sort_wave<false>(e, lane), lane);
-  }
-  if (lane < k) {
-    const int64_t o = (int64_t)g * k + lane;
-    out_score[o] = (float)unorder64(best.key);
-    out_beam[o] = (int32_t)(best.place / kWave);
-    out_token[o] = (int64_t)tokens[best.place / kWave][best.place % kWave];
+  const int half = 1 << (31 - __builtin_clz(k));               // the largest power of 2 in k
+  for (int w = wid; w < W; w += waves) {
+    const u64 key = lane < k ? keys[w][lane] : 0;
+    int place = key ? 0 : k;
+#pragma unroll 1
+    for (int o0 = 0; o0 < W; o0 += kSide) {
+      if (__ballot(place < k) == 0) break;
+      int before[kSide] = {};                                  // entries of row o that come before
+      for (int step = half; step > 0; step >>= 1) {
+#pragma unroll
+        for (int i = 0; i < kSide; ++i) {
+          const int o = min(o0 + i, W - 1);
+          const u64 other = before[i] + step <= k ? keys[o][before[i] + step - 1] : 0;
+          if (other > key || (other == key && o < w && other)) before[i] += step;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kSide; ++i) place += o0 + i == w ? lane : o0 + i < W ? before[i] : 0;
+    }
+    if (place < k) {
+      const int64_t at = (int64_t)g * k + place;
+      out_score[at] = (float)unorder64(key);
+      out_beam[at] = w;
+      out_token[at] = (int64_t)tokens[w][lane];
+    }
   }
 }
 
@@ -461,15 +516,13 @@ int elem_size(int dtype) { return dtype == ACORN_F32 ? 4 : 2; }
 
 template <typename T>
 void part(const void* logits, int64_t rs, const float* scores, int64_t rows, int64_t V, int64_t k,
-          Pieces pc, void* ws, hipStream_t st) {
-  u64* lists = (u64*)ws;
-  float2* sums = (float2*)(lists + rows * pc.count * k);
+          Pieces pc, u64* lists, Piece* pieces, hipStream_t st) {
   auto kfn = pc.nv == 2   ? beam_part_kernel<T, 2>
              : pc.nv == 5  ? beam_part_kernel<T, 5>
              : pc.nv == 10 ? beam_part_kernel<T, 10>
                            : beam_part_kernel<T, 20>;
-  kfn<<<dim3(pc.count, (unsigned)rows), dim3(kPartNT), 0, st>>>((const T*)logits, rs, scores, (int)V,
-                                                                (int)k, lists, sums);
+  kfn<<<dim3(pc.count, (unsigned)rows), dim3(kPartNT), 0, st>>>(
+      (const T*)logits, rs, scores, (int)V, (int)k, lists, pieces);
 }
 
 }  // namespace
@@ -482,7 +535,8 @@ extern "C" int acorn_beam_select_workspace(int64_t groups, int64_t beams, int64_
   if (rc != ACORN_OK) return rc;
   if (dtype != ACORN_F32 && dtype != ACORN_F16 && dtype != ACORN_BF16) return ACORN_ERR_DTYPE;
   const int64_t rows = groups * beams;
-  *bytes = rows * pieces_of(rows, vocab, elem_size(dtype)).count * (k + 1) * 8;
+  *bytes = rows * pieces_of(rows, vocab, elem_size(dtype)).count *
+           (k * (int64_t)sizeof(u64) + (int64_t)sizeof(Piece));
   return ACORN_OK;
 }
 
@@ -497,22 +551,22 @@ extern "C" int acorn_beam_select(const void* logits, int64_t row_stride, const f
   if (groups == 0) return ACORN_OK;
   if (!logits || !scores || !out_score || !out_beam || !out_token || !status || !ws)
     return ACORN_ERR_VALUE;
-  if (row_stride < 0 || ws_bytes < need || (uintptr_t)ws % 8 ||
+  if (row_stride < 0 || ws_bytes < need || (uintptr_t)ws % 16 ||
       (uintptr_t)logits % (unsigned)elem_size(dtype))
     return ACORN_ERR_VALUE;
   hipStream_t st = (hipStream_t)stream;
   const int64_t rows = groups * beams;
   const Pieces pc = pieces_of(rows, vocab, elem_size(dtype));
-  if (dtype == ACORN_F32) part<float>(logits, row_stride, scores, rows, vocab, k, pc, ws, st);
-  if (dtype == ACORN_F16) part<_Float16>(logits, row_stride, scores, rows, vocab, k, pc, ws, st);
-  if (dtype == ACORN_BF16) part<__bf16>(logits, row_stride, scores, rows, vocab, k, pc, ws, st);
+  Piece* pieces = (Piece*)ws;
+  u64* lists = (u64*)(pieces + rows * pc.count);
+  if (dtype == ACORN_F32) part<float>(logits, row_stride, scores, rows, vocab, k, pc, lists, pieces, st);
+  if (dtype == ACORN_F16) part<_Float16>(logits, row_stride, scores, rows, vocab, k, pc, lists, pieces, st);
+  if (dtype == ACORN_BF16) part<__bf16>(logits, row_stride, scores, rows, vocab, k, pc, lists, pieces, st);
   ACORN_LAUNCH_CHECK();
-  const u64* lists = (const u64*)ws;
-  const float2* sums = (const float2*)(lists + rows * pc.count * k);
   const unsigned waves = (unsigned)std::min<int64_t>(beams, kJoinWaves);
   beam_join_kernel<<<dim3((unsigned)groups), dim3(waves * kWave), 0, st>>>(
-      lists, sums, scores, (int)beams, (int)vocab, (int)k, pc.count, out_score, out_beam, out_token,
-      status);
+      lists, pieces, scores, (int)beams, (int)vocab, (int)k, pc.count, out_score, out_beam,
+      out_token, status);
   ACORN_LAUNCH_CHECK();
   return ACORN_OK;
 }

@@ -157,7 +157,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
     else:
         assert workspace.get_device() == dev and workspace.is_contiguous() and \
             workspace.numel() * workspace.element_size() >= need and \
-            workspace.data_ptr() % 8 == 0, "workspace: beam_select_workspace of the same sizes"
+            workspace.data_ptr() % 16 == 0, "workspace: beam_select_workspace of the same sizes"
     launch("beam_select", dev, logits.data_ptr(), logits.stride(0), scores.data_ptr(), G, W, V, k,
            out.score.data_ptr(), out.beam.data_ptr(), out.token.data_ptr(), out.status.data_ptr(),
            workspace.data_ptr(), workspace.numel() * workspace.element_size(), code)

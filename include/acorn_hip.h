@@ -548,7 +548,7 @@ int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t max_nq, int6
  * order of s, equal ones by beam and then token: out_score [G, k] (s rounded to fp32), out_beam,
  * out_token. -inf logits are banned tokens, beams of score -inf have only continuations of -inf
  * and their rows are not read. status [G*W]: 1 for a beam whose score or row holds NaN or +inf
- * (it counts as one of score -inf), else 0. ws: 8-byte aligned, at least the bytes
+ * (it counts as one of score -inf), else 0. ws: 16-byte aligned, at least the bytes
  * acorn_beam_select_workspace reports; contents need not be set, calls that overlap need
  * workspaces of their own. Deterministic.
  */

@@ -226,7 +226,8 @@ def _hold(x, scores, k, out=None):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("G,W,V,k", [(1, 1, 1, 1), (1, 1, 5, 5), (2, 3, 7, 21), (3, 4, 1000, 8),
                                      (1, 32, 77, 64), (2, 5, 4097, 15), (5, 2, 8193, 1),
-                                     (1, 4, 32768, 12), (70, 3, 517, 6)])
+                                     (1, 4, 32768, 12), (70, 3, 517, 6), (130, 4, 20003, 8),
+                                     (300, 4, 6001, 8)])
 def test_select(dtype, G, W, V, k):
     x, s = _logits(G * W, V, dtype, G + V)
     _hold(x, s.view(G, W), k)
@@ -274,6 +275,18 @@ def test_select_of_ordered_and_equal_logits(dtype, shape):
            "two": (i % 2).float(), "zeros": torch.where(i % 3 == 0, -0.0, 0.0)}[shape].to(dtype)
     x = torch.stack([row, row, row])
     _hold(x, torch.tensor([[-1.0, -1.0, -2.5]]), k)
+
+
+@gpu
+@pytest.mark.parametrize("shape", ["equal", "rising"])
+@pytest.mark.parametrize("G,W,V", [(300, 4, 6001), (130, 4, 20003)])
+def test_select_of_ordered_and_equal_logits_in_many_rows(shape, G, W, V):
+    """Long pieces, whose candidates do not fit where they are held."""
+    i = torch.arange(V)
+    row = (torch.full((V,), 1.5) if shape == "equal" else i / 100.0).to(torch.bfloat16)
+    x = row.expand(G * W, V)
+    s = -torch.arange(G * W).view(G, W) / 64.0
+    _hold(x, s, 33)
 
 
 @gpu

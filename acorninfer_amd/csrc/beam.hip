@@ -160,76 +160,111 @@ __device__ __forceinline__ int parent_of(const int32_t* parents, size_t gw, int 
   return p >= 0 && p < W ? p : l;              // (a parent that there is not: the beam itself)
 }
 
-// A pool [layers, num_blocks, page_bytes]; a page is `segs` runs of `stride` bytes, of which the
-// tokens' first bytes are copied: `unit` for every `group` tokens or part of them.
-struct Pool {
-  uint8_t* base;
-  int64_t page_bytes;
-  int segs, stride, unit, group;
-};
+// The pools: pages of `bytes`, [layers, num_blocks] of them. Of a page whose first `fill` tokens are
+// to be copied these are its first fill * row bytes (tokens one after another), or with `tiles` the
+// groups of 16 tokens that hold one: of each kv head's P / 16 groups of 2^shift pieces of 16 bytes
+// the first ones. An 8-bit cache's scale codes (2 pieces to a group) go with its V tiles.
 struct Pools {
-  Pool p[3];
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* scales;                                             // or none: no tiles
+  int64_t bytes, num_blocks;
+  int row, shift;
 };
 
-constexpr int kCopyNT = 256;
+constexpr int kCopyNT = 256, kCopyUnroll = 4;
+constexpr int64_t kCopyParts = 2048;                           // workgroups that a copy is divided into, if it has the units
+constexpr int kCopyUnit = kCopyNT * kCopyUnroll;               // pieces of 16 bytes that are on their way together
 typedef uint32_t bm_u32x4 __attribute__((ext_vector_type(4)));
 
+// A workgroup per (layer and pool, group, part of the group's copies): every wave works the plan out,
+// and the units of all copies are dealt to the parts, so that no workgroup is there for a beam that
+// needs no copy. 16 x 4 beams through 36 layers, 24 pages of half 32 KB in each: 12.8 us with a
+// workgroup per beam, layer and pool; as it is, see kCopyParts.
 __global__ __launch_bounds__(kCopyNT) void beam_copy_kernel(
     const Pools pools, const int32_t* __restrict__ tables, const int32_t* __restrict__ lens,
-    const int32_t* __restrict__ parents, int W, int P, int64_t num_blocks, int width) {
-  const int child = blockIdx.y, g = child / W, layer = blockIdx.x;
+    const int32_t* __restrict__ parents, int W, int P, int width) {
+  const int g = blockIdx.y, layer = blockIdx.x >> 1;
+  const bool second = blockIdx.x & 1;
   const int lane = threadIdx.x % kWave;
   const size_t gw = (size_t)g * W;
   const int n = lens[gw], fill = n % P, c = n / P;
-  if (n <= 0 || fill == 0 || c >= width) return;
   const int parent = parent_of(parents, gw, W, lane);
+  if (n <= 0 || fill == 0 || c >= width) return;
   const int page = tables[(gw + (lane < W ? lane : 0)) * width + c];
   const Plan plan = plan_pages(parent, page, W, lane);
-  const int w = child % W;
-  const int64_t to = __shfl(plan.to, w), from = __shfl(plan.from, w);
-  if (to == from || to < 0 || from < 0 || to >= num_blocks || from >= num_blocks) return;
-  const Pool pool = pools.p[blockIdx.z];
-  const size_t base = (size_t)layer * num_blocks * pool.page_bytes;
-  const uint8_t* src = pool.base + base + from * pool.page_bytes;
-  uint8_t* dst = pool.base + base + to * pool.page_bytes;
-  const int per = (fill + pool.group - 1) / pool.group * pool.unit / 16;   // 16-byte pieces of a run
-  const int total = per * pool.segs;
-  for (int i = threadIdx.x; i < total; i += kCopyNT) {
-    const int64_t at = (int64_t)(i / per) * pool.stride + (int64_t)(i % per) * 16;
-    *(bm_u32x4*)(dst + at) = *(const bm_u32x4*)(src + at);
+  const bool copy = lane < W && plan.to != plan.from && (uint32_t)plan.to < (uint32_t)pools.num_blocks &&
+                    (uint32_t)plan.from < (uint32_t)pools.num_blocks;
+  const uint64_t copies = __ballot(copy);
+  const int rank = __popcll(copies & lanes_below(lane));
+  const bool tiles = pools.scales != nullptr;
+  const int groups = (fill + 15) / 16, of = P / 16;
+  const int pieces = (int)((tiles ? pools.bytes : (int64_t)fill * pools.row) / 16);
+  const int units = (pieces + kCopyUnit - 1) / kCopyUnit;
+  uint8_t* pool = (second ? pools.v : pools.k) + (size_t)layer * pools.num_blocks * pools.bytes;
+  for (int i = blockIdx.z; i < __popcll(copies) * units; i += gridDim.z) {
+    const int from_lane = __ffsll((unsigned long long)__ballot(copy && rank == i / units)) - 1;
+    const int64_t to = __builtin_amdgcn_readlane(plan.to, from_lane);
+    const int64_t from = __builtin_amdgcn_readlane(plan.from, from_lane);
+    const bm_u32x4* src = (const bm_u32x4*)(pool + from * pools.bytes);
+    bm_u32x4* dst = (bm_u32x4*)(pool + to * pools.bytes);
+    const int first = i % units * kCopyUnit + threadIdx.x;
+    bm_u32x4 x[kCopyUnroll];
+    bool on[kCopyUnroll];
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u) {
+      const int at = first + u * kCopyNT;
+      on[u] = at < pieces && (!tiles || (at >> pools.shift & (of - 1)) < groups);
+      x[u] = src[on[u] ? at : 0];
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u)
+      if (on[u]) dst[first + u * kCopyNT] = x[u];
+    if (tiles && second && i % units == 0) {                   // the page's scale codes
+      const int64_t codes = (pools.bytes >> pools.shift) * 2;  // 32 bytes to a group
+      uint8_t* sc = pools.scales + (size_t)layer * pools.num_blocks * codes;
+      for (int at = threadIdx.x; at < codes / 16; at += kCopyNT)
+        if ((at >> 1 & (of - 1)) < groups)
+          ((bm_u32x4*)(sc + to * codes))[at] = ((const bm_u32x4*)(sc + from * codes))[at];
+    }
   }
 }
 
-// A thread per column, which reads the group's entries of it before it writes them.
-__global__ __launch_bounds__(256) void beam_tables_kernel(int32_t* tables, const int32_t* lens,
-                                                          const int32_t* parents, int W, int P,
-                                                          int width) {
-  __shared__ int32_t held[kMaxBeams][256];
+// A thread per column, which reads the group's entries of it before it writes them; the plan comes
+// out of the column that these hold.
+constexpr int kTableNT = 256;
+
+__global__ __launch_bounds__(kTableNT) void beam_tables_kernel(int32_t* tables, const int32_t* lens,
+                                                               const int32_t* parents, int W, int P,
+                                                               int width) {
+  __shared__ int32_t held[kMaxBeams][kTableNT];
   __shared__ int32_t par[kMaxBeams], taken[kMaxBeams];
-  const int g = blockIdx.y, lane = threadIdx.x;
+  const int g = blockIdx.y, lane = threadIdx.x % kWave;
   const size_t gw = (size_t)g * W;
+  const int c0 = blockIdx.x * kTableNT, column = c0 + threadIdx.x;
+  int32_t* t = tables + gw * width + min(column, width - 1);
   const int n = max(lens[gw], 0), fill = n % P, c = n / P;
-  if ((int64_t)blockIdx.x * 256 > c) return;                   // columns of the future
-  if (lane < kWave) {
-    const int parent = parent_of(parents, gw, W, lane);
-    const int page = c < width ? tables[(gw + (lane < W ? lane : 0)) * width + c] : 0;
+  const int parent = parent_of(parents, gw, W, lane);
+  for (int w = 0; w < W; ++w) held[w][threadIdx.x] = t[(size_t)w * width];
+  if (c0 > c) return;                                          // columns of the future
+  __syncthreads();
+  if (threadIdx.x < kWave) {
+    const bool here = fill && c < width && c < c0 + kTableNT;
+    const int page = held[lane < W ? lane : 0][here ? c - c0 : 0];
     const Plan plan = plan_pages(parent, page, W, lane);
     if (lane < W) {
       par[lane] = parent;
-      taken[lane] = fill ? plan.to : page;
+      taken[lane] = plan.to;
     }
   }
   __syncthreads();
-  const int64_t column = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (column >= width || column > c) return;
-  int32_t* t = tables + gw * width + column;
-  if (column == c) {
-    for (int w = 0; w < W; ++w) t[(size_t)w * width] = taken[w];
-    return;
+  if (column >= width || column > c || (column == c && !fill)) return;
+  for (int w = 0; w < W; ++w) {
+    if (column == c)
+      t[(size_t)w * width] = taken[w];
+    else if (par[w] != w)
+      t[(size_t)w * width] = held[par[w]][threadIdx.x];
   }
-  for (int w = 0; w < W; ++w) held[w][threadIdx.x] = t[(size_t)w * width];
-  for (int w = 0; w < W; ++w)
-    if (par[w] != w) t[(size_t)w * width] = held[par[w]][threadIdx.x];
 }
 
 // ---- hypotheses -------------------------------------------------------------------------------
@@ -337,9 +372,10 @@ extern "C" int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, 
       kv_heads > 65535 || head_dim < 1 || head_dim > 65536 || table_stride > 0x7fffffff / page_size)
     return ACORN_ERR_SHAPE;
   if (beams > kMaxBeams) return ACORN_ERR_UNSUPPORTED;
-  if (groups * beams > 65535 || layers > 0x7fffffff) return ACORN_ERR_SHAPE;
+  if (groups * beams > 65535 || layers > 0x3fffffff) return ACORN_ERR_SHAPE;
   const bool tiles = scale_pool != nullptr;
-  if (tiles && (page_size % 16 || elem_size != 1)) return ACORN_ERR_SHAPE;
+  if (tiles && (page_size % 16 || (page_size & (page_size - 1)) || elem_size != 1)) return ACORN_ERR_SHAPE;
+  if (tiles && head_dim != 64 && head_dim != 128) return ACORN_ERR_UNSUPPORTED;
   if (!tiles && elem_size != 2 && elem_size != 4) return ACORN_ERR_DTYPE;
   const int64_t row = kv_heads * head_dim * elem_size;         // a token's bytes
   if (row % 16 || row * page_size > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
@@ -347,29 +383,20 @@ extern "C" int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, 
   if (!k_pool || !v_pool || !tables || !lens || !parents) return ACORN_ERR_VALUE;
   if ((uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16 || (uintptr_t)scale_pool % 16)
     return ACORN_ERR_VALUE;
-  Pools pools = {};
-  const int64_t pb = row * page_size;
-  if (tiles) {
-    const int per = (int)(page_size * head_dim);
-    pools.p[0] = {(uint8_t*)k_pool, pb, (int)kv_heads, per, (int)(16 * head_dim), 16};
-    pools.p[1] = {(uint8_t*)v_pool, pb, (int)kv_heads, per, (int)(16 * head_dim), 16};
-    pools.p[2] = {(uint8_t*)scale_pool, kv_heads * page_size * 2, (int)kv_heads,
-                  (int)(page_size * 2), 32, 16};
-  } else {
-    pools.p[0] = {(uint8_t*)k_pool, pb, 1, 0, (int)row, 1};
-    pools.p[1] = {(uint8_t*)v_pool, pb, 1, 0, (int)row, 1};
-  }
+  if (beams == 1) return ACORN_OK;
+  const Pools pools = {(uint8_t*)k_pool, (uint8_t*)v_pool, (uint8_t*)scale_pool, row * page_size,
+                       num_blocks, (int)row, tiles ? __builtin_ctzll((unsigned long long)head_dim) : 0};
+  const int64_t most = (beams - 1) * ((pools.bytes / 16 + kCopyUnit - 1) / kCopyUnit);
+  const int64_t parts = std::max<int64_t>(1, std::min(most, kCopyParts / (2 * layers * groups)));
   hipStream_t st = (hipStream_t)stream;
-  if (beams > 1) {
-    beam_copy_kernel<<<dim3((unsigned)layers, (unsigned)(groups * beams), tiles ? 3 : 2),
-                       dim3(kCopyNT), 0, st>>>(pools, tables, lens, parents, (int)beams,
-                                               (int)page_size, num_blocks, (int)table_stride);
-    ACORN_LAUNCH_CHECK();
-    beam_tables_kernel<<<dim3((unsigned)((table_stride + 255) / 256), (unsigned)groups), dim3(256),
-                         0, st>>>(tables, lens, parents, (int)beams, (int)page_size,
-                                  (int)table_stride);
-    ACORN_LAUNCH_CHECK();
-  }
+  beam_copy_kernel<<<dim3((unsigned)(2 * layers), (unsigned)groups, (unsigned)parts), dim3(kCopyNT), 0,
+                     st>>>(pools, tables, lens, parents, (int)beams, (int)page_size,
+                           (int)table_stride);
+  ACORN_LAUNCH_CHECK();
+  beam_tables_kernel<<<dim3((unsigned)((table_stride + kTableNT - 1) / kTableNT), (unsigned)groups),
+                       dim3(kTableNT), 0, st>>>(tables, lens, parents, (int)beams, (int)page_size,
+                                                (int)table_stride);
+  ACORN_LAUNCH_CHECK();
   return ACORN_OK;
 }
 

@@ -269,56 +269,118 @@ __global__ __launch_bounds__(kTableNT) void beam_tables_kernel(int32_t* tables, 
 
 // ---- hypotheses -------------------------------------------------------------------------------
 // out[g, m, t] = tokens[t, g, b_t] for t < steps[g, m], where b_{steps - 1} = beams[g, m] and
-// b_{t - 1} = parents[t, g, b_t]; `pad` behind. A walk of T dependent steps: each wave takes a
-// piece of the steps, follows every beam through it (a map of W beams), the maps of the pieces
-// are chained, and each wave then walks its piece again with the beams that reach it.
+// b_{t - 1} = parents[t, g, b_t]; `pad` behind. T dependent steps, taken side by side: a wave's lanes
+// are 64 / B stretches of L steps by B beams (B a power of 2, W of them used), 16 waves hold the T
+// steps of a group. Every stretch is walked from each beam at its end: a map of beams. A
+// hypothesis's beam at a stretch's end comes out of the maps of the stretches behind it (those
+// of a wave composed by doubling), and the stretch is walked once more from there with the tokens.
+// 16 groups of 8 beams, 2048 steps: 16 dependent steps, 16 more with the tokens.
 constexpr int kTraceWaves = 16;
+constexpr int kTile = 16;                          // steps whose rows are loaded together
 
 __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
     const int32_t* __restrict__ tokens, const int32_t* __restrict__ parents,
     const int32_t* __restrict__ steps, const int32_t* __restrict__ beams,
-    int64_t* __restrict__ out, int T, int G, int W, int M, int64_t pad) {
-  __shared__ int map[kTraceWaves][kMaxBeams];      // beam at a piece's end -> before its first step
-  __shared__ int part[kWave];                      // the same for a walk that starts in a piece
+    int64_t* __restrict__ out, int T, int G, int W, int M, int L, int shift, int64_t pad) {
+  // beam at a stretch's end -> before its first step; and through the wave's stretches behind it too
+  __shared__ int8_t one[kTraceWaves * kWave], rest[kTraceWaves * kWave];
+  __shared__ int8_t part[kMaxBeams];               // a hypothesis's beam before the stretch it ends in
+  __shared__ int64_t stage[kTraceWaves][kWave][kTile + 1];
   const int g = blockIdx.x, lane = threadIdx.x % kWave, wid = threadIdx.x / kWave;
-  const int m = blockIdx.y * kWave + lane;
-  const bool hyp = m < M;
-  const int per = (T + kTraceWaves - 1) / kTraceWaves;
-  const int a = min(wid * per, T), b = min(a + per, T);
-  const int start = hyp ? min(steps[(size_t)g * M + m], T) - 1 : -1;
-  const int beam0 = hyp ? beams[(size_t)g * M + m] : -1;
+  const int B = 1 << shift, S = kWave >> shift, j = lane >> shift, h = lane & (B - 1);
+  const int own = lane - h;                        // the first lane of the stretch
+  const int q = wid * S + j;                       // the stretch, steps a .. e - 1
+  const int a = min((int64_t)q * L, (int64_t)T), e = min(a + L, T);
   auto inside = [&](int x) { return x >= 0 && x < W ? x : -1; };      // -1 ends a walk
+  auto at = [&](int v, int beam) { return __shfl(v, own + max(beam, 0)); };
   auto hop = [&](int row, int cur) {
-    const int next = __shfl(row, cur < 0 ? 0 : cur);
+    const int next = at(row, cur);
     return cur < 0 ? -1 : inside(next);
   };
-  const int l = lane < W ? lane : 0;
-  int all = lane < W ? lane : -1, mine = -1;
-  const bool here = hyp && start >= a && start < b;
-  for (int t = b - 1; t >= a; --t) {
-    const int row = parents[((size_t)t * G + g) * W + l];
-    if (here && t == start) mine = inside(beam0);
-    all = hop(row, all);
-    mine = hop(row, mine);
-  }
-  if (lane < W) map[wid][lane] = all;
-  if (here) part[lane] = mine;
-  __syncthreads();
-  // the beam at this piece's end (or at the walk's start in it)
-  int cur = -1;
-  if (hyp && start >= b) {
-    const int piece = start / per;
-    cur = part[lane];
-    for (int i = piece - 1; i > wid; --i) cur = cur < 0 ? -1 : map[i][cur];
-  }
-  int64_t* o = out + ((size_t)g * M + (hyp ? m : 0)) * T;
-  for (int t = b - 1; t >= a; --t) {
-    const size_t at = ((size_t)t * G + g) * W + l;
-    const int row = parents[at], token = tokens[at];
-    if (here && t == start) cur = inside(beam0);
-    const int tok = __shfl(token, cur < 0 ? 0 : cur);
-    if (hyp) o[t] = cur < 0 ? pad : (int64_t)tok;
-    cur = hop(row, cur);
+  // steps a + L - kTile (i + 1) .. of every stretch, one beam to a lane
+  auto load = [&](const int32_t* from, int i, int (&x)[kTile]) {
+#pragma unroll
+    for (int o = 0; o < kTile; ++o) {
+      const int t = min(max(a + L - kTile * (i + 1) + o, 0), T - 1);
+      x[o] = from[((size_t)t * G + g) * W + min(h, W - 1)];
+    }
+  };
+  const int tiles = (L + kTile - 1) / kTile;
+  int all = h < W ? h : -1;
+  for (int h0 = 0; h0 < M; h0 += B) {
+    const int m = h0 + h;
+    const bool hyp = m < M;
+    const int last = hyp ? min(steps[(size_t)g * M + m], T) - 1 : -1;
+    const int beam = hyp ? inside(beams[(size_t)g * M + m]) : -1;
+    const int ends = last >= 0 ? last / L : -1;    // the stretch it ends in
+    int mine = -1;
+    const bool some = __ballot(q == ends) != 0;    // a hypothesis ends in one of the wave's stretches
+    for (int i = 0; i < ((int64_t)wid * S * L < T && (h0 == 0 || some) ? tiles : 0); ++i) {
+      int row[kTile];
+      load(parents, i, row);
+#pragma unroll
+      for (int o = kTile - 1; o >= 0; --o) {
+        if (kTile * (i + 1) - o > L) break;        // (before every stretch)
+        const int t = a + L - kTile * (i + 1) + o;
+        if (h0 == 0) {
+          const int x = hop(row[o], all);
+          if (t < e) all = x;
+        }
+        if (some) {
+          if (t == last) mine = beam;              // (q == ends there)
+          const int y = hop(row[o], mine);
+          if (t < e) mine = y;
+        }
+      }
+    }
+    if (h0 == 0) {
+      one[threadIdx.x] = (int8_t)all;
+      for (int d = 1; d < S; d <<= 1) {            // this stretch after the d behind it
+        const int v = __shfl(all, (lane + d * B) % kWave), x = at(all, v);
+        if (j + d < S) all = v < 0 ? -1 : x;
+      }
+      rest[threadIdx.x] = (int8_t)all;
+    }
+    if (q == ends) part[h] = (int8_t)mine;
+    __syncthreads();
+    // the beam at this stretch's end
+    int cur = -1;
+    if (ends > q) {
+      cur = part[h];
+      auto follow = [&](const int8_t* map, int stretch) { cur = cur < 0 ? -1 : map[stretch * B + cur]; };
+      const int w = ends / S, from = w == wid ? q + 1 : w * S;
+      for (int i = ends - 1; i >= from; --i) follow(one, i);
+      if (w != wid) {
+        for (int i = w - 1; i > wid; --i) follow(rest, i * S);
+        if (j + 1 < S) follow(rest, q + 1);
+      }
+    }
+    __syncthreads();                               // (part is written again)
+    for (int i = 0; i < ((int64_t)wid * S * L < T ? tiles : 0); ++i) {  // (a wave may have no steps)
+      int row[kTile], token[kTile];
+      load(parents, i, row);
+      load(tokens, i, token);
+#pragma unroll
+      for (int o = kTile - 1; o >= 0; --o) {
+        if (kTile * (i + 1) - o > L) break;
+        const int t = a + L - kTile * (i + 1) + o;
+        if (t == last) cur = beam;
+        const int tok = at(token[o], cur);
+        stage[wid][lane][o] = cur < 0 || t > last ? pad : (int64_t)tok;
+        const int next = hop(row[o], cur);
+        if (t < e && t <= last) cur = next;
+      }
+      __builtin_amdgcn_wave_barrier();
+      // kTile tokens of a lane side by side
+      for (int r = 0; r < kWave * kTile; r += kWave) {
+        const int of = (r + lane) / kTile, o = lane % kTile;
+        const int a_of = min((int64_t)(wid * S + (of >> shift)) * L, (int64_t)T);
+        const int t = a_of + L - kTile * (i + 1) + o, m_of = h0 + (of & (B - 1));
+        if (m_of < M && t >= a_of && t < min(a_of + L, T))
+          out[((size_t)g * M + m_of) * T + t] = stage[wid][of][o];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
@@ -405,14 +467,17 @@ extern "C" int acorn_beam_trace(const int32_t* tokens, const int32_t* parents,
                                 int64_t T, int64_t groups, int64_t W, int64_t M, int64_t pad,
                                 void* stream) {
   if (T < 0 || T > 0x7fffffff - 64 || groups < 0 || groups > 0x7fffffff || W < 1 || M < 0 ||
-      M > 65535 * (int64_t)kWave)
+      M > 0x7fffffff - kMaxBeams)
     return ACORN_ERR_SHAPE;
   if (W > kMaxBeams) return ACORN_ERR_UNSUPPORTED;
   if (T == 0 || groups == 0 || M == 0) return ACORN_OK;
   if (!tokens || !parents || !steps || !beams || !out) return ACORN_ERR_VALUE;
-  beam_trace_kernel<<<dim3((unsigned)groups, (unsigned)((M + kWave - 1) / kWave)),
-                      dim3(kTraceWaves * kWave), 0, (hipStream_t)stream>>>(
-      tokens, parents, steps, beams, out, (int)T, (int)groups, (int)W, (int)M, pad);
+  int shift = 0;
+  while ((1 << shift) < W) ++shift;
+  const int64_t stretches = (int64_t)kTraceWaves * (kWave >> shift);
+  beam_trace_kernel<<<dim3((unsigned)groups), dim3(kTraceWaves * kWave), 0, (hipStream_t)stream>>>(
+      tokens, parents, steps, beams, out, (int)T, (int)groups, (int)W, (int)M,
+      (int)((T + stretches - 1) / stretches), shift, pad);
   ACORN_LAUNCH_CHECK();
   return ACORN_OK;
 }

@@ -176,10 +176,10 @@ def one_device(first: torch.Tensor, *tensors: torch.Tensor) -> int:
     """The index of the one GPU that holds the tensors: a kernel launches on one device's stream
     and reaches every tensor by its pointer."""
     dev = first.get_device()
-    for t in tensors:
-        if t.get_device() != dev:
+    for d in map(torch.Tensor.get_device, tensors):
+        if d != dev:
             require_gpu(first, *tensors)
-            raise AssertionError(f"tensors on {first.device} and {t.device}")
+            raise AssertionError(f"tensors on {sorted({str(t.device) for t in (first, *tensors)})}")
     if dev < 0:
         require_gpu(first)
     return dev

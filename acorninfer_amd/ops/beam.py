@@ -140,11 +140,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
         logits = logits.contiguous()
     if out is None:
         dev = one_device(logits, scores)
-        i32 = torch.empty(G * (2 * k + W), dtype=torch.int32, device=logits.device)
-        out = BeamCandidates(i32[:G * k].view(torch.float32).view(G, k),
-                             i32[G * k:2 * G * k].view(G, k),
-                             torch.empty((G, k), dtype=torch.int64, device=logits.device),
-                             i32[2 * G * k:])
+        out = BeamCandidates(scores.new_empty((G, k)), scores.new_empty((G, k), dtype=torch.int32),
+                             scores.new_empty((G, k), dtype=torch.int64),
+                             scores.new_empty((G * W,), dtype=torch.int32))
     else:
         for name, dtype in (("score", torch.float32), ("beam", torch.int32), ("token", torch.int64)):
             _check(getattr(out, name), "out." + name, (G, k), dtype)
@@ -164,16 +162,26 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
     return out
 
 
+# (a state is twelve tensors, and a call looks at two of them: what is as it should be is passed in
+# one expression, and only what is not is looked at field by field)
 def _check_state(s: BeamState, name: str, G: int, W: int) -> None:
-    T = s.token_log.shape[0] if s.token_log.dim() == 3 else 0
+    scores, length, done, ids, position, parents, tlog, plog, fs, fl, fb, ft = s
+    gw, g, log, i32, f32 = (G, W), (G,), (s.token_log.shape[0], G, W), torch.int32, torch.float32
+    if scores.dtype is f32 is fs.dtype and ids.dtype is torch.int64 and length.dtype is i32 and \
+            done.dtype is i32 and position.dtype is i32 and parents.dtype is i32 and \
+            tlog.dtype is i32 and plog.dtype is i32 and fl.dtype is i32 and fb.dtype is i32 and \
+            ft.dtype is i32 and scores.shape == gw == fs.shape == ids.shape == position.shape == \
+            parents.shape == fl.shape == fb.shape == ft.shape and length.shape == g == done.shape and \
+            tlog.shape == log == plog.shape and log[0] >= 1 and scores.is_contiguous() and \
+            length.is_contiguous() and done.is_contiguous() and ids.is_contiguous() and \
+            position.is_contiguous() and parents.is_contiguous() and tlog.is_contiguous() and \
+            plog.is_contiguous() and fs.is_contiguous() and fl.is_contiguous() and \
+            fb.is_contiguous() and ft.is_contiguous():
+        return
     for field, t, dtype in zip(BeamState._fields, s, _STATE_DTYPES):
-        if field in ("length", "done"):
-            shape = (G,)
-        else:
-            shape = (T, G, W) if field.endswith("_log") else (G, W)
-        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-            _check(t, f"{name}.{field}", shape, dtype)
-    assert T >= 1, "logs are [steps, G, W]"
+        shape = g if field in ("length", "done") else log if field.endswith("_log") else gw
+        _check(t, f"{name}.{field}", shape, dtype)
+    raise AssertionError("logs are [steps, G, W], of at least one step")
 
 
 def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Tensor, *,
@@ -188,7 +196,8 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
     Groups that are done stay (ids `pad`, every beam its own parent). k = W * (E + 1) candidates
     are always enough for W beams; beams that get none have score -inf. Returns `out` (a state of
     the same sizes; by default `state`, in place), whose logs are written in place."""
-    assert state.scores.dim() == 2, "scores are [G, W]"
+    assert state.scores.dim() == 2 and state.token_log.dim() == 3, \
+        "scores are [G, W], logs [steps, G, W]"
     G, W = state.scores.shape
     out = state if out is None else out
     _check_state(state, "state", G, W)
@@ -213,7 +222,7 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
                                   f"{MAX_CANDIDATES}")
     dev = one_device(*state, score, beam, token, end_ids, *(() if out is state else out))
     s, o = state, out
-    launch("beam_advance", dev, *(t.data_ptr() for t in (
+    launch("beam_advance", dev, *map(torch.Tensor.data_ptr, (
         s.scores, s.length, s.done, s.position, s.fin_scores, s.fin_length, s.fin_beam, s.fin_token,
         o.scores, o.length, o.done, o.ids, o.position, o.parents, o.fin_scores, o.fin_length,
         o.fin_beam, o.fin_token, o.token_log, o.parent_log, score, beam, token, end_ids)),

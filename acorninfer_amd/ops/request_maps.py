@@ -54,7 +54,7 @@ def block_tables(blocks: torch.Tensor, lengths: torch.Tensor, page_size: int, wi
     N = lengths.shape[0]
     if out is None:
         dev = one_device(blocks, lengths)
-        out = torch.empty((N, width), dtype=torch.int32, device=lengths.device)
+        out = lengths.new_empty((N, width))
     else:
         assert out.dtype is torch.int32 and out.shape == (N, width) and out.is_contiguous(), \
             f"out is contiguous int32 {[N, width]}"
@@ -80,9 +80,8 @@ def slot_map(tables: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, p
     assert R >= 0 and (W >= 1 or N == 0), "tables hold at least one page per request"
     if out is None:
         dev = one_device(tables, starts, counts)
-        wide = torch.empty((3, R), dtype=torch.int64, device=tables.device)
-        slim = torch.empty(2 * R + N, dtype=torch.int32, device=tables.device)
-        out = SlotMap(slim[:R], *wide, slim[R:2 * R], slim[2 * R:])
+        seq, lens, row0 = tables.new_empty((2 * R + N,)).split((R, R, N))
+        out = SlotMap(seq, *tables.new_empty((3, R), dtype=torch.int64).unbind(), lens, row0)
     else:
         for name, t, dtype in zip(SlotMap._fields, out, _MAP_DTYPES):
             n = N if name == "row0" else R

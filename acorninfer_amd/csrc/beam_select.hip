@@ -230,7 +230,9 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
   // The lane's maximum m and s = sum exp(x - m), as powers of 2 of x log2 e - R, R the running
   // maximum's x log2 e as a float, so that one fma with one rounding makes the exponent. NaN and
   // +inf reach s as NaN, -inf adds nothing.
-  float m = -INFINITY, s = 0.f, R = -kHuge * kLog2e;
+  // Beside a token that has nearly all of the probability the others are below half a unit in the
+  // last place of s one by one: what an addition of a vector's sum rounds off is kept in `lost`.
+  float m = -INFINITY, s = 0.f, lost = 0.f, R = -kHuge * kLog2e;
   float vmax[NV];
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
@@ -241,16 +243,21 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     vmax[u] = vm;
     m = fmaxf(m, vm);
     const float Rn = fmaxf(m, -kHuge) * kLog2e;
-    s *= __builtin_amdgcn_exp2f(R - Rn);
+    const float scale = __builtin_amdgcn_exp2f(R - Rn);
     R = Rn;
+    float t = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      s += __builtin_amdgcn_exp2f(__builtin_fmaf(vec_elem<T>(x[u], e), kLog2e, -R));
+      t += __builtin_amdgcn_exp2f(__builtin_fmaf(vec_elem<T>(x[u], e), kLog2e, -R));
+    s *= scale;
+    const float sum = s + t;
+    lost = lost * scale + (t - (sum - s));         // (exact where s >= t, as it soon is)
+    s = sum;
     // (a vector is worked off while the ones behind it are on their way; its sum stays here)
-    asm volatile("" : "+v"(s));
+    asm volatile("" : "+v"(s), "+v"(lost));
     __builtin_amdgcn_sched_barrier(0);
   }
-  s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(fmaxf(m, -kHuge), kLog2e, -R));
+  s = (s + lost) * __builtin_amdgcn_exp2f(-__builtin_fmaf(fmaxf(m, -kHuge), kLog2e, -R));
   if (__ballot(fabsf(m) >= kHuge && m > -INFINITY) != 0) {     // (x log2 e is too coarse there)
     const float ref = m == -INFINITY ? 0.f : m;
     s = 0.f;
@@ -404,7 +411,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
       S = over_lanes(S, lane, [](double a, double b) { return a + b; });
       if (!(S == S)) bad = true;
       live = !bad && M > -INFINITY;
-      // (the pieces' exponentials are powers of 2 of x * kLog2e, which as a float is 1.3e-8 off)
+      // (the pieces' exponentials are powers of 2 of x * kLog2e, which as a float is 1.3e-8 off: what
+      // is left of that is 1.3e-8 times the row's entropy, 1e-7)
       log_sum = log2(S) / (double)kLog2e;
     }
     if (live) {

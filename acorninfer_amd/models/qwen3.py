@@ -506,9 +506,12 @@ class Qwen3DecodeModel:
     def buffers(self, batch: int, max_pages: int, num_splits: int | None = None,
                 tilings: dict | None = None, *, prefill: bool = False,
                 kv8_page: int = 0) -> "StepBuffers":
-        return StepBuffers(self, batch, max_pages, num_splits,
-                           tilings if tilings is not None else self.tilings.get(batch),
-                           prefill=prefill, kv8_page=kv8_page)
+        # (ordinary tensors, whoever asks: forward_extend keeps its buffers, and what an engine's
+        # step made in inference mode could not be written outside it)
+        with torch.inference_mode(False):
+            return StepBuffers(self, batch, max_pages, num_splits,
+                               tilings if tilings is not None else self.tilings.get(batch),
+                               prefill=prefill, kv8_page=kv8_page)
 
     def kv8_page(self, cache) -> int:
         """StepBuffers.kv8_page for steps over `cache`: its page size where it is an 8-bit one

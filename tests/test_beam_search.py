@@ -182,6 +182,32 @@ def test_an_engine_searches_between_its_steps():
 
 
 @gpu
+def test_a_prefill_after_a_search_reuses_its_buffers():
+    """The model keeps the last prefill's buffers: a search's, which runs in inference mode, can be
+    written outside it, and the other way round."""
+    from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, random_state_dict
+    sd = random_state_dict(SMALL, seed=7, std=0.02, dtype=torch.bfloat16)
+    model = Qwen3DecodeModel.from_state_dict(SMALL, sd, device="cuda")
+    search, alloc = _search(model, 60, beams=2, max_tokens=3, max_model_len=64, eos_ids={1})
+    prompt = list(range(50, 61))
+
+    def prefill():
+        view = PagedCacheView(search.cache)
+        out = model.forward_prefill_batch(torch.tensor([prompt]).cuda(), [view], real_lens=[len(prompt)])
+        for block in view.table:
+            alloc.free(block)
+        return out
+
+    first = search.search([prompt])
+    kept = model._extend_buf[1]
+    logits = prefill()
+    assert model._extend_buf[1] is kept
+    assert search.search([prompt]) == first and model._extend_buf[1] is kept
+    assert torch.equal(prefill(), logits)
+    alloc.assert_balanced()
+
+
+@gpu
 def test_broken_logits_end_a_search():
     from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, random_state_dict
     sd = random_state_dict(TINY, seed=3, std=0.25, dtype=torch.float32)

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
   // this lane's vectors are p0 + tid + u * kPartNT; those past the row's whole ones read the last
   // of these
   const uint8_t* base = (const uint8_t*)(p + (int64_t)min(p0, max(full - 1, 0)) * E);
-  const uint32_t last = (uint32_t)max(full - 1 - p0, 0) * 16u;
+  const uint32_t last = (uint32_t)min(max(full - 1 - p0, 0), NV * kPartNT) * 16u;
   bs_u32x4 x[NV];
 #pragma unroll
   for (int u = 0; u < NV; ++u) x[u] = bs_u32x4{0u, 0u, 0u, 0u};

@@ -165,7 +165,8 @@ class BeamSearch:
         views = [PagedCacheView(self.cache) for _ in prompts]
         try:
             flat, room = self._reserve(lens, views, own, steps)
-            return self._search(prompts, lens, views, flat, room, steps)
+            with torch.cuda.device(self.device):
+                return self._search(prompts, lens, views, flat, room, steps)
         finally:
             for block in own + [b for v in views for b in v.table]:
                 self.allocator.free(block)

@@ -178,14 +178,18 @@ class Engine:
         """The best answers of every prompt by beam search (engine/beam.py), run to its end between
         two steps on this engine's cache. Requests in flight keep their blocks; BlockExhausted
         where too few are free, and nothing has changed then."""
-        key = (beams, max_tokens, length_penalty, early_stopping,
+        if max_tokens < 1:
+            raise ValueError("max_tokens must be >= 1")
+        # (searches of similar lengths share their buffers and captured steps)
+        most = min(max(16, 1 << (max_tokens - 1).bit_length()), max(max_tokens, self.max_model_len))
+        key = (beams, most, length_penalty, early_stopping,
                frozenset(QWEN3_EOS_IDS if eos_ids is None else eos_ids))
         if key not in self._searches:
             self._searches[key] = BeamSearch(
-                self.model, self.cache, self.allocator, beams=beams, max_tokens=max_tokens,
+                self.model, self.cache, self.allocator, beams=beams, max_tokens=most,
                 max_model_len=self.max_model_len, eos_ids=key[-1], length_penalty=length_penalty,
                 early_stopping=early_stopping, capture=self._capture)
-        return self._searches[key].search(prompts)
+        return self._searches[key].search(prompts, max_tokens=max_tokens)
 
     def drop(self, seq_id: int) -> None:
         """Forget a finished sequence's record (the caller consumed its output)."""

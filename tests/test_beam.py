@@ -176,7 +176,7 @@ def test_entries_refuse_without_a_gpu():
     assert select(G=40000) == _lib.ERR_SHAPE
     assert select(dtype=3) == _lib.ERR_DTYPE
     assert select(x=None) == select(ws=None) == select(ws_bytes=8) == select(stride=-1) == \
-        select(x=p + 1) == select(ws=p + 4) == _lib.ERR_VALUE
+        select(x=p + 1) == select(ws=p + 8) == _lib.ERR_VALUE
     assert select(G=0) == 0
     def advance(G=1, W=2, k=4, T=3, E=1, alpha=1.0, first=p):
         return L.acorn_beam_advance(first, *[p] * 23, G, W, k, T, E, alpha, 0, 0, None)
@@ -189,6 +189,8 @@ def test_entries_refuse_without_a_gpu():
     assert reorder(ts=0) == reorder(layers=0) == reorder(P=0) == reorder(G=70000) == _lib.ERR_SHAPE
     assert reorder(W=33) == reorder(KV=1, D=4) == _lib.ERR_UNSUPPORTED
     assert reorder(esz=1) == _lib.ERR_DTYPE and reorder(scales=p) == _lib.ERR_SHAPE
+    assert reorder(esz=1, scales=p, P=48) == reorder(esz=1, scales=p, P=8) == _lib.ERR_SHAPE
+    assert reorder(esz=1, scales=p, D=32) == _lib.ERR_UNSUPPORTED
     assert reorder(k=None) == reorder(k=p + 8) == reorder(esz=1, scales=p + 8) == _lib.ERR_VALUE
     def trace(T=4, G=1, W=2, M=2, x=p):
         return L.acorn_beam_trace(x, p, p, p, p, T, G, W, M, 0, None)

@@ -506,7 +506,7 @@ struct Pieces {
 Pieces pieces_of(int64_t rows, int64_t V, int elem) {
   const int64_t e = 16 / elem, vectors = (V + e - 1) / e;
   Pieces pc = {0, 0};
-  for (int nv : {2, 5, 10, 20}) {
+  for (int nv : {2, 5, 10, 19}) {
     pc = {(int)((vectors + nv * kPartNT - 1) / (nv * kPartNT)), nv};
     if (pc.count * rows <= 1024) break;
   }
@@ -528,7 +528,7 @@ void part(const void* logits, int64_t rs, const float* scores, int64_t rows, int
   auto kfn = pc.nv == 2   ? beam_part_kernel<T, 2>
              : pc.nv == 5  ? beam_part_kernel<T, 5>
              : pc.nv == 10 ? beam_part_kernel<T, 10>
-                           : beam_part_kernel<T, 20>;
+                           : beam_part_kernel<T, 19>;
   kfn<<<dim3(pc.count, (unsigned)rows), dim3(kPartNT), 0, st>>>(
       (const T*)logits, rs, scores, (int)V, (int)k, lists, pieces);
 }

@@ -16,8 +16,8 @@
 // the order they are met in. Tokens at -inf are no candidates here: the join puts
 // them behind the others where a row has too few.
 //
-// Rows of 151936 in bf16, from a graph: 1 row 10 us, 4 rows 11, 64 rows 16, 256 rows 26 (78 MB:
-// 3.0 TB/s), 1024 rows 77 (4.0 TB/s). Few rows are latency: two launches, each with a chain of
+// Rows of 151936 in bf16, from a graph: 1 row 9.4 us, 4 rows 10.9, 64 rows 15.6, 256 rows 25 (78 MB:
+// 3.1 TB/s), 1024 rows 72 (4.4 TB/s). Few rows are latency: two launches, each with a chain of
 // loads, a sort and a join. Of the 19 us of 256 rows' pieces the loads alone take 11.7 (from the
 // last cache; 13.5 from memory), with the sums 13.5; the rest comes behind the loads in all
 // workgroups at once: queue 2.9, look 1, sort 1.5, write 1.5. Many rows are bound by VALU work
@@ -375,11 +375,34 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
 // ---- the join ---------------------------------------------------------------------------------
 constexpr int kJoinWaves = 16;
 constexpr int kAhead = 4;                      // loads of a lane in flight
-constexpr int kSide = 4;                       // rows that are searched side by side
 
-// A wave per row: the sum of its pieces, and its k best out of their lists, sorted. An entry's
-// place in the group's list is its place in its row's and the numbers of entries before it in
-// the other rows', found by halving.
+// An entry of the group's list: s as a key, then its place (beam * 64 + rank in the beam's list): the
+// larger key first, of equal ones the lower place.
+struct Entry {
+  u64 key;
+  uint32_t place;
+};
+__device__ __forceinline__ bool comes_before(const Entry& a, const Entry& b) {
+  return a.key > b.key || (a.key == b.key && a.place < b.place);
+}
+__device__ __forceinline__ Entry entry_of(const u64 (*keys)[kMaxK], int w, int k, int i) {
+  return i < k ? Entry{keys[w][i], (uint32_t)(w * kWave + i)} : Entry{0, 0xFFFFFFFFu};
+}
+template <int D = 32>
+__device__ __forceinline__ Entry exchange_entries(const Entry& v, int lane) {
+  const Entry o = {lane_xor<D>(v.key, lane), lane_xor<D>(v.place, lane)};
+  const Entry r = comes_before(o, v) == ((lane & D) == 0) ? o : v;
+  if constexpr (D > 1) return exchange_entries<D / 2>(r, lane);
+  return r;
+}
+// The 64 first of a list in order and one in the opposite order, in order.
+__device__ __forceinline__ Entry merge_entries(const Entry& a, const Entry& b, int lane) {
+  return exchange_entries(comes_before(b, a) ? b : a, lane);
+}
+
+// A wave per row (or two): the sum of its pieces, and its k best out of their lists, sorted; then the
+// rows' lists are merged pair by pair. (Finding every entry's place by halving in the other rows'
+// lists is W^2 log k reads of LDS: as fast for 4 beams, 1 us more for 8, 11 more for 32.)
 __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     const u64* __restrict__ lists, const Piece* __restrict__ pieces,
     const float* __restrict__ scores, int W, int V, int k, int C, float* __restrict__ out_score,
@@ -387,6 +410,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
   __shared__ uint32_t tokens[kMaxBeams][kMaxK];
   __shared__ u64 keys[kMaxBeams][kMaxK];                       // s, 0: no entry
   __shared__ u64 reach[kJoinWaves][(kAhead + 1) * kWave];      // of a row's entries, those that may count
+  __shared__ u64 pair_key[kJoinWaves][kWave];
+  __shared__ uint32_t pair_place[kJoinWaves][kWave];
   const int g = blockIdx.x, lane = threadIdx.x % kWave, wid = threadIdx.x / kWave;
   const int waves = blockDim.x / kWave;
   for (int w = wid; w < W; w += waves) {
@@ -476,39 +501,31 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     if (lane == 0) status[row] = bad;
   }
   __syncthreads();
-  const int half = 1 << (31 - __builtin_clz(k));               // the largest power of 2 in k
-  for (int w = wid; w < W; w += waves) {
-    const u64 key = lane < k ? keys[w][lane] : 0;
-    int place = key ? 0 : k;
-#pragma unroll 1
-    for (int o0 = 0; o0 < W; o0 += kSide) {
-      if (__ballot(place < k) == 0) break;
-      int before[kSide] = {};                                  // entries of row o that come before
-      for (int step = half; step > 0; step >>= 1) {
-#pragma unroll
-        for (int i = 0; i < kSide; ++i) {
-          const int o = min(o0 + i, W - 1);
-          const u64 other = before[i] + step <= k ? keys[o][before[i] + step - 1] : 0;
-          if (other > key || (other == key && o < w && other)) before[i] += step;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kSide; ++i) place += o0 + i == w ? lane : o0 + i < W ? before[i] : 0;
-    }
-    if (place < k) {
-      const int64_t at = (int64_t)g * k + place;
-      out_score[at] = (float)unorder64(key);
-      out_beam[at] = w;
-      out_token[at] = (int64_t)tokens[w][lane];
-    }
+  // the waves' lists pair by pair
+  Entry best = entry_of(keys, wid, k, lane);
+  if (wid + waves < W) best = merge_entries(best, entry_of(keys, wid + waves, k, kWave - 1 - lane), lane);
+  for (int half = waves > 1 ? 1 << (31 - __builtin_clz(waves - 1)) : 0; half > 0; half >>= 1) {
+    pair_key[wid][lane] = best.key;
+    pair_place[wid][lane] = best.place;
+    __syncthreads();
+    if (wid < half && wid + half < waves)
+      best = merge_entries(best, Entry{pair_key[wid + half][kWave - 1 - lane],
+                                       pair_place[wid + half][kWave - 1 - lane]}, lane);
+    __syncthreads();
+  }
+  if (wid == 0 && lane < k) {
+    const int64_t at = (int64_t)g * k + lane;
+    out_score[at] = (float)unorder64(best.key);
+    out_beam[at] = (int32_t)(best.place / kWave);
+    out_token[at] = (int64_t)tokens[best.place / kWave][best.place % kWave];
   }
 }
 
 // Vectors of a lane and pieces of a row: the shortest pieces with which a batch has no more
 // workgroups than the chip has places for them (four to a CU), so that it runs in one round, each
-// with one sort. 16 / 32 / 128 / 256 rows of 151936: 12.6 / 12.7 / 18.6 / 24 us; with up to 512
-// workgroups 11.7 / 12.8 / 19.3 / 25.4, with up to 2048 12.6 / 15.5 / 20.5 / 25.0. 19 vectors is
-// the most that 128 registers hold beside their maxima (20 spill: 27.4 against 26.3 us at k = 16).
+// with one sort. 16 / 32 / 128 / 256 rows of 151936, 4 beams: 12.4 / 12.5 / 18.6 / 24.5 us; with up
+// to 512 workgroups 11.7 / 12.8 / 19.3 / 25.4, with up to 2048 12.6 / 15.5 / 20.5 / 25.0. 19 vectors
+// is the most that 128 registers hold beside their maxima (20 spill: 1 us more for 256 rows).
 struct Pieces {
   int count, nv;
 };

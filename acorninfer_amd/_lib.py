@@ -18,6 +18,7 @@ import torch
 
 # (the stream's handle without a Stream object around it: a microsecond of a call's ten)
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch._C import _cuda_getDevice as _current_device
 
 LIB_PATH = Path(os.environ.get(
     "ACORN_HIP_LIB", Path(__file__).resolve().parent / "_lib" / "libacorn_hip.so"))
@@ -103,6 +104,7 @@ _SIGNATURES = {
 }
 
 _lib = None
+_entries: dict = {}             # of `launch`, by name
 
 
 class AcornError(RuntimeError):
@@ -187,8 +189,10 @@ def one_device(first: torch.Tensor, *tensors: torch.Tensor) -> int:
 
 def launch(name: str, dev: int, *args) -> None:
     """Launch on the current stream of device `dev`, with that device current."""
-    fn = getattr(lib(), "acorn_" + name)
-    if torch.cuda.current_device() == dev:
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), "acorn_" + name)
+    if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):

@@ -316,7 +316,7 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
   for (int h0 = 0; h0 < M; h0 += B) {
     const int m = h0 + h;
     const bool hyp = m < M;
-    const int last = hyp ? min(steps[(size_t)g * M + m], T) - 1 : -1;
+    const int last = hyp ? min(max(steps[(size_t)g * M + m], 0), T) - 1 : -1;
     const int beam = hyp ? inside(beams[(size_t)g * M + m]) : -1;
     const int ends = last >= 0 ? last / L : -1;    // the stretch it ends in
     int mine = -1;
@@ -472,7 +472,7 @@ extern "C" int acorn_beam_trace(const int32_t* tokens, const int32_t* parents,
                                 const int32_t* steps, const int32_t* beams, int64_t* out,
                                 int64_t T, int64_t groups, int64_t W, int64_t M, int64_t pad,
                                 void* stream) {
-  if (T < 0 || T > 0x7fffffff - 64 || groups < 0 || groups > 0x7fffffff || W < 1 || M < 0 ||
+  if (T < 0 || T > 0x3fffffff || groups < 0 || groups > 0x7fffffff || W < 1 || M < 0 ||
       M > 0x7fffffff - kMaxBeams)
     return ACORN_ERR_SHAPE;
   if (W > kMaxBeams) return ACORN_ERR_UNSUPPORTED;

@@ -543,3 +543,19 @@ def test_trace_of_logs_with_a_beam_that_there_is_not():
     got = _beam().beam_trace(tokens.cuda(), parents.cuda(), steps.cuda(), beams.cuda(), pad=-1)
     assert torch.equal(got.cpu(), ref.trace_ref(tokens, parents, steps, beams, pad=-1))
     assert got[0, 0, :7].tolist() == [-1] * 7 and got[0, 0, 7:].min() >= 0
+
+
+@gpu
+@pytest.mark.parametrize("least", [-2**31, -2**31 + 1, -1])
+def test_trace_of_a_length_far_below_zero(least):
+    tokens = torch.arange(80).view(40, 1, 2).int()
+    parents = torch.zeros(40, 1, 2, dtype=torch.int32)
+    steps, beams = torch.tensor([[least, 40]]).int(), torch.tensor([[1, 1]]).int()
+    got = _beam().beam_trace(tokens.cuda(), parents.cuda(), steps.cuda(), beams.cuda(), pad=-1)
+    assert torch.equal(got.cpu(), ref.trace_ref(tokens, parents, steps, beams, pad=-1))
+
+
+def test_trace_refuses_logs_past_its_whole_numbers():
+    from acorninfer_amd import _lib
+    L, p = _lib.lib(), 64
+    assert L.acorn_beam_trace(p, p, p, p, p, 2**30, 1, 1, 1, 0, None) == _lib.ERR_SHAPE

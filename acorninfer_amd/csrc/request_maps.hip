@@ -39,7 +39,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red, int64_t* 
 }
 
 __device__ __forceinline__ int64_t pages_for(int32_t length, int shift) {
-  return length > 0 ? ((int64_t)length + (1 << shift) - 1) >> shift : 0;
+  return length > 0 ? ((int64_t)length + (1ll << shift) - 1) >> shift : 0;
 }
 
 // `rows` table rows to a workgroup, a part of their columns.
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kNT) void slot_map_kernel(
 }
 
 int shift_of(int64_t page_size) {
-  if (page_size < 1 || page_size > 65536 || (page_size & (page_size - 1))) return -1;
+  if (page_size < 1 || page_size > (1 << 30) || (page_size & (page_size - 1))) return -1;
   return __builtin_ctzll((unsigned long long)page_size);
 }
 
@@ -131,7 +131,7 @@ extern "C" int acorn_block_tables(const int32_t* blocks, int64_t n_blocks, const
                                   int32_t* tables, int64_t N, int64_t width, int64_t page_size,
                                   int pad, void* stream) {
   const int shift = shift_of(page_size);
-  if (shift < 0 || N < 0 || N > 0x7fffffff || width < 1 || width > 0x7fffffff || n_blocks < 0)
+  if (shift < 0 || N < 0 || N > 0x3fffffff || width < 1 || width > 0x7fffffff || n_blocks < 0)
     return ACORN_ERR_SHAPE;
   if (N == 0) return ACORN_OK;
   if ((n_blocks && !blocks) || !lengths || !tables) return ACORN_ERR_VALUE;

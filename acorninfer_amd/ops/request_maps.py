@@ -36,7 +36,7 @@ _MAP_DTYPES = (torch.int32, torch.int64, torch.int64, torch.int64, torch.int32, 
 
 def _page_size(page_size: int) -> int:
     P = int(page_size)
-    assert 1 <= P <= 65536 and P & (P - 1) == 0, f"page_size {P} must be a power of two"
+    assert 1 <= P <= 1 << 30 and P & (P - 1) == 0, f"page_size {P} must be a power of two"
     return P
 
 

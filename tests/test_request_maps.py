@@ -44,10 +44,11 @@ def test_entries_refuse_without_a_gpu():
     def tables(T=9, N=3, width=4, P=16, b=p):
         return L.acorn_block_tables(b, T, p, p, N, width, P, 0, None)
     assert tables(T=-1) == tables(N=-1) == tables(width=0) == tables(P=24) == _lib.ERR_SHAPE
+    assert tables(P=2**31) == tables(N=2**30) == _lib.ERR_SHAPE
     assert tables(b=None) == _lib.ERR_VALUE and tables(N=0) == 0
     def slots(N=3, R=5, width=4, P=16, t=p, seq=p):
         return L.acorn_slot_map(t, p, p, seq, p, p, p, p, p, N, R, width, P, None)
-    assert slots(N=-1) == slots(R=-1) == slots(width=0) == slots(P=0) == _lib.ERR_SHAPE
+    assert slots(N=-1) == slots(R=-1) == slots(width=0) == slots(P=0) == _lib.ERR_SHAPE == slots(P=2**31)
     assert slots(t=None) == slots(seq=None) == _lib.ERR_VALUE and slots(N=0) == 0
 
 
@@ -134,3 +135,24 @@ def test_in_a_graph():
     m = o.slot_map(out, torch.zeros_like(lengths), lengths, 16, rows)
     zero = torch.zeros_like(lengths)
     assert graph_replays_match(lambda: o.slot_map(out, zero, lengths, 16, rows, out=m), lambda: m.pages)
+
+
+@gpu
+@pytest.mark.parametrize("P", [1, 16, 2**30])
+def test_positions_at_the_ends_of_their_type(P):
+    """The first and the last starts that 32 bits hold: whole numbers of 64 bits, pages of -1."""
+    starts = torch.tensor([-2**31, -1, 2**31 - 2, 5]).int()
+    counts = torch.tensor([3, 2, 2, 1]).int()
+    tables = torch.arange(12).view(4, 3).int()
+    into = [torch.full((8,), v, dtype=t) for t, v in FIELDS]
+    got = _ops().slot_map(tables.cuda(), starts.cuda(), counts.cuda(), P, 8)
+    assert got.positions.tolist() == [-2**31, -2**31 + 1, -2**31 + 2, -1, 0, 2**31 - 2, 2**31 - 1, 5]
+    into[4] = into[4].long()                     # (a length of 2^31 stops at 2^31 - 1)
+    want = slot_map_ref(tables, starts, counts, P, 8, into)
+    want[4] = want[4].clamp_max(2**31 - 1).int()
+    for name, a, b in zip(got._fields, got, want):
+        assert torch.equal(a.cpu(), b), name
+    lengths = torch.tensor([2**31 - 1, -2**31, 1]).int()
+    blocks = torch.arange(9).int()
+    assert torch.equal(_ops().block_tables(blocks.cuda(), lengths.cuda(), P, 5, pad=-2).cpu(),
+                       block_tables_ref(blocks, lengths, P, 5, pad=-2))

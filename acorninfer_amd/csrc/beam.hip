@@ -5,6 +5,7 @@
 // All are short: a few hundred bytes, or copies of a page per layer, behind a chain of
 // dependent loads.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 
@@ -13,6 +14,7 @@ using namespace acorn;
 namespace {
 
 constexpr int kMaxBeams = 32, kMaxK = 64;
+constexpr double kMaxPenalty = 64.0;             // ln of the largest length^penalty
 
 __device__ __forceinline__ uint64_t lanes_below(int lane) { return (1ull << lane) - 1; }
 
@@ -416,7 +418,9 @@ extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, co
                        parent_log, cand_score, cand_beam, cand_token};
   for (const void* p : all)
     if (!p) return ACORN_ERR_VALUE;
-  if ((n_ends && !ends) || !(length_penalty > -INFINITY && length_penalty < INFINITY))
+  // (steps^penalty as a factor that 32 bits hold, either way; NaN and infinities fail too)
+  if ((n_ends && !ends) || !(fabs(length_penalty) * log((double)steps) <= kMaxPenalty) ||
+      !(fabs(length_penalty) < INFINITY))
     return ACORN_ERR_VALUE;
   const BeamFields in = {(float*)scores, (int32_t*)length, (int32_t*)done, nullptr,
                          (int32_t*)position, nullptr, (float*)fin_scores, (int32_t*)fin_length,

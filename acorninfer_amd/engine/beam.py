@@ -21,7 +21,7 @@ from acorninfer_amd.cache.pager import BlockExhausted, PagedCacheView
 from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, StepBuffers
 from acorninfer_amd.ops.beam import (MAX_BEAMS, MAX_CANDIDATES, BeamCandidates, BeamState,
                                      beam_advance, beam_reset, beam_select, beam_select_workspace,
-                                     beam_state, beam_trace)
+                                     beam_state, beam_trace, check_length_penalty)
 from acorninfer_amd.ops.request_maps import SlotMap, block_tables, slot_map
 
 WARMUP_STEPS = 2
@@ -59,8 +59,7 @@ class BeamSearch:
         eos = sorted(set(int(i) for i in eos_ids))
         if beams < 1 or max_tokens < 1:
             raise ValueError("beams and max_tokens must be >= 1")
-        if not math.isfinite(length_penalty):
-            raise ValueError(f"length_penalty must be finite, not {length_penalty}")
+        check_length_penalty(float(length_penalty), max_tokens + 1)
         self.candidates = beams * (len(eos) + 1)     # enough for `beams` that do not end
         if beams > MAX_BEAMS or self.candidates > MAX_CANDIDATES:
             raise NotImplementedError(f"{beams} beams with {len(eos)} end tokens: at most "

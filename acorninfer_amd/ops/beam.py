@@ -29,6 +29,7 @@ from acorninfer_amd._lib import check, dtype_code, launch, lib, one_device
 
 MAX_BEAMS = 32
 MAX_CANDIDATES = 64
+MAX_PENALTY = 64.0              # ln of the largest length ** length_penalty
 
 
 class BeamCandidates(NamedTuple):
@@ -184,6 +185,13 @@ def _check_state(s: BeamState, name: str, G: int, W: int) -> None:
     raise AssertionError("logs are [steps, G, W], of at least one step")
 
 
+def check_length_penalty(alpha: float, steps: int) -> None:
+    """Scores divided by steps ** alpha stay within 32 bits."""
+    if not (math.isfinite(alpha) and abs(alpha) * math.log(steps) <= MAX_PENALTY):
+        raise ValueError(f"length_penalty must be finite and at most {MAX_PENALTY} / ln({steps}) "
+                         f"either way, not {alpha}")
+
+
 def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Tensor, *,
                  length_penalty: float = 1.0, early_stopping: bool = False, pad: int = 0,
                  out: BeamState | None = None) -> BeamState:
@@ -194,7 +202,8 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
     is left, where the logs are full, or where it has W finished hypotheses and (early_stopping,
     or its best beam's score / length ** length_penalty is no better than the worst of them).
     Groups that are done stay (ids `pad`, every beam its own parent). k = W * (E + 1) candidates
-    are always enough for W beams; beams that get none have score -inf. Returns `out` (a state of
+    are always enough for W beams; beams that get none have score -inf. |length_penalty| * ln(steps)
+    is at most 64. Returns `out` (a state of
     the same sizes; by default `state`, in place), whose logs are written in place."""
     assert state.scores.dim() == 2 and state.token_log.dim() == 3, \
         "scores are [G, W], logs [steps, G, W]"
@@ -215,8 +224,7 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
     assert E >= 0 and end_ids.dtype is torch.int64 and end_ids.is_contiguous(), \
         "end_ids are contiguous int64 [E]"
     alpha = float(length_penalty)
-    if not math.isfinite(alpha):
-        raise ValueError(f"length_penalty must be finite, not {alpha}")
+    check_length_penalty(alpha, state.token_log.shape[0])
     if W > MAX_BEAMS or K > MAX_CANDIDATES:
         raise NotImplementedError(f"{W} beams, {K} candidates: at most {MAX_BEAMS} and "
                                   f"{MAX_CANDIDATES}")

@@ -575,7 +575,7 @@ int acorn_beam_select_workspace(int64_t groups, int64_t beams, int64_t vocab, in
  *   length and position grow by 1; the group is done where no beam is left, t + 1 == steps, or
  *   there are W finished and (early_stopping, or the worst is no worse than the best beam's
  *   score / (t + 1)^length_penalty).
- * out_* may be the same memory as the state they replace.
+ * out_* may be the same memory as the state they replace. |length_penalty| * ln(steps) <= 64.
  */
 int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t* done,
                        const int32_t* position, const float* fin_scores,

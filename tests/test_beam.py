@@ -559,3 +559,20 @@ def test_trace_refuses_logs_past_its_whole_numbers():
     from acorninfer_amd import _lib
     L, p = _lib.lib(), 64
     assert L.acorn_beam_trace(p, p, p, p, p, 2**30, 1, 1, 1, 0, None) == _lib.ERR_SHAPE
+
+
+def test_a_length_penalty_past_32_bits_is_refused():
+    """Scores / steps ** penalty would be zeros, infinities or (0 / 0) NaN that have no order."""
+    from acorninfer_amd import _lib
+    from acorninfer_amd.ops import beam as b
+    L, p = _lib.lib(), 64
+    for steps, alpha, fits in ((4, 46.0, True), (4, 47.0, False), (4, -47.0, False), (2049, 8.3, True),
+                               (2049, -8.4, False), (1, 1e300, True), (1, math.inf, False)):
+        rc = L.acorn_beam_advance(*[p] * 24, 0, 2, 4, steps, 0, alpha, 0, 0, None)
+        assert rc == 0                                      # (no groups: nothing to look at)
+        if fits:
+            b.check_length_penalty(alpha, steps)
+            continue
+        assert L.acorn_beam_advance(*[p] * 24, 1, 2, 4, steps, 0, alpha, 0, 0, None) == _lib.ERR_VALUE
+        with pytest.raises(ValueError):
+            b.check_length_penalty(alpha, steps)

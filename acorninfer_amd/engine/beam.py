@@ -26,6 +26,7 @@ from acorninfer_amd.ops.request_maps import SlotMap, block_tables, slot_map
 
 WARMUP_STEPS = 2
 CHECK_EVERY = 16
+KEPT = 4                        # numbers of groups whose buffers and step are kept
 
 
 @dataclass(frozen=True)
@@ -78,7 +79,11 @@ class BeamSearch:
 
     # ------------------------------------------------------------- one step --
     def _batch(self, G: int) -> _Batch:
-        if G not in self._batches:
+        b = self._batches.pop(G, None)
+        if b is None:
+            while len(self._batches) >= KEPT:                # the one that was used longest ago
+                torch.cuda.synchronize(self.device)          # (a search that was broken off may still run)
+                del self._batches[next(iter(self._batches))]
             W, K, V, dev = self.beams, self.candidates, self.model.cfg.vocab_size, self.device
             B = G * W
             buf = self.model.buffers(B, self.width, kv8_page=self._kv8)
@@ -90,10 +95,11 @@ class BeamSearch:
 
             cand = BeamCandidates(z(G, K, dtype=torch.float32), z(G, K), z(G, K, dtype=torch.int64),
                                   z(B))
-            self._batches[G] = _Batch(
+            b = _Batch(
                 buf, state, cand, beam_select_workspace(G, W, V, K, buf.logits.dtype, dev),
                 SlotMap(z(B), buf.positions, buf.pages, buf.slots, buf.lens, z(B)), z(B) + 1, z(B))
-        return self._batches[G]
+        self._batches[G] = b
+        return b
 
     def _advance(self, b: _Batch, cand: BeamCandidates) -> None:
         beam_advance(b.state, cand, self.end_ids, length_penalty=self.penalty,
@@ -122,9 +128,10 @@ class BeamSearch:
             for _ in range(WARMUP_STEPS):
                 self._body(b)
         torch.cuda.current_stream(self.device).wait_stream(s)
-        b.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(b.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._body(b)
+        b.graph = graph
 
     # ------------------------------------------------------------- a search --
     def _reserve(self, lens: list[int], views: list[PagedCacheView], own: list[int],

@@ -30,6 +30,7 @@ from acorninfer_amd.models.qwen3 import Qwen3DecodeModel
 from acorninfer_amd.sampler import Sampler, SamplingParams
 
 QWEN3_EOS_IDS = frozenset({151643, 151645})  # <|endoftext|>, <|im_end|>
+KEPT_SEARCHES = 4                            # settings of beam_search whose buffers are kept
 
 
 @dataclass
@@ -184,12 +185,17 @@ class Engine:
         most = min(max(16, 1 << (max_tokens - 1).bit_length()), max(max_tokens, self.max_model_len))
         key = (beams, most, length_penalty, early_stopping,
                frozenset(QWEN3_EOS_IDS if eos_ids is None else eos_ids))
-        if key not in self._searches:
-            self._searches[key] = BeamSearch(
+        search = self._searches.pop(key, None)
+        if search is None:
+            search = BeamSearch(
                 self.model, self.cache, self.allocator, beams=beams, max_tokens=most,
                 max_model_len=self.max_model_len, eos_ids=key[-1], length_penalty=length_penalty,
                 early_stopping=early_stopping, capture=self._capture)
-        return self._searches[key].search(prompts, max_tokens=max_tokens)
+        self._searches[key] = search
+        while len(self._searches) > KEPT_SEARCHES:           # the one that was used longest ago
+            torch.cuda.synchronize(self.model.device)
+            del self._searches[next(iter(self._searches))]
+        return search.search(prompts, max_tokens=max_tokens)
 
     def drop(self, seq_id: int) -> None:
         """Forget a finished sequence's record (the caller consumed its output)."""

@@ -217,3 +217,28 @@ def test_broken_logits_end_a_search():
     with pytest.raises(ValueError):
         search.search([[3, 4, 5]])
     alloc.assert_balanced()
+
+
+@gpu
+def test_steps_of_many_sizes_and_settings_are_not_all_kept():
+    """Searches over more numbers of prompts, and an engine's over more settings, than are kept: the
+    first, made again, is what it was."""
+    from acorninfer_amd.engine import beam, engine
+    from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, random_state_dict
+    model = Qwen3DecodeModel.from_state_dict(TINY, random_state_dict(TINY, seed=3, std=0.25,
+                                                                    dtype=torch.float32),
+                                             dtype=torch.float32, device="cuda")
+    search, alloc = _search(model, 200, beams=2, max_tokens=5, max_model_len=64, eos_ids={1})
+    prompts = [[i + 3, 7, 20 - i] for i in range(beam.KEPT + 2)]
+    first = search.search(prompts[:1])
+    for n in range(2, len(prompts) + 1):
+        assert len(search.search(prompts[:n])) == n
+        assert len(search._batches) == min(n, beam.KEPT)
+    assert search.search(prompts[:1]) == first
+    assert list(search._batches) == [len(prompts) - 2, len(prompts) - 1, len(prompts), 1]
+    alloc.assert_balanced()
+    eng = engine.Engine(model, num_blocks=128, max_model_len=64)
+    got = [eng.beam_search(prompts[:2], beams=2, max_tokens=5, length_penalty=i / 4, eos_ids=frozenset({1}))
+           for i in (0, 1, 2, 3, 4, 5, 0)]
+    assert got[0] == got[-1] and len(eng._searches) == engine.KEPT_SEARCHES
+    eng.assert_balanced()

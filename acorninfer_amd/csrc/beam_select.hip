@@ -16,7 +16,7 @@
 // the order they are met in. Tokens at -inf are no candidates here: the join puts
 // them behind the others where a row has too few.
 //
-// Rows of 151936 in bf16, from a graph: 1 row 9.4 us, 4 rows 10.9, 64 rows 15.6, 256 rows 25 (78 MB:
+// Rows of 151936 in bf16, from a graph: 1 row 9.2 us, 4 rows 10.4, 64 rows 15.4, 256 rows 25 (78 MB:
 // 3.1 TB/s), 1024 rows 72 (4.4 TB/s). Few rows are latency: two launches, each with a chain of
 // loads, a sort and a join. Of the 19 us of 256 rows' pieces the loads alone take 11.7 (from the
 // last cache; 13.5 from memory), with the sums 13.5; the rest comes behind the loads in all
@@ -400,6 +400,31 @@ __device__ __forceinline__ Entry merge_entries(const Entry& a, const Entry& b, i
   return exchange_entries(comes_before(b, a) ? b : a, lane);
 }
 
+// ln s to 1e-12 for normal s > 0 (2^31 pieces of sums past any need): s = 2^e f with f between
+// sqrt(1/2) and sqrt(2), ln f = 2 atanh t = 2 (t + t^3/3 + ... ), t = (f - 1) / (f + 1), |t| < 0.172: the
+// term of t^15 is below 5e-13. The library's log2 holds every size to the last place: 0.2 us more of
+// the launch's 5, in code that is cold.
+__device__ __forceinline__ double ln64(double s) {
+  double f = __builtin_amdgcn_frexp_mant(s);                   // 1/2 .. 1
+  int e = __builtin_amdgcn_frexp_exp(s);
+  const bool low = f < 0.70710678118654752;
+  f = low ? f + f : f;
+  e -= low;
+  const double d = f + 1.0;
+  double r = __builtin_amdgcn_rcp(d);                          // (two steps of Newton's)
+  r = r * __builtin_fma(-d, r, 2.0);
+  r = r * __builtin_fma(-d, r, 2.0);
+  const double t = (f - 1.0) * r, u = t * t;
+  double p = 1.0 / 13.0;
+  p = __builtin_fma(p, u, 1.0 / 11.0);
+  p = __builtin_fma(p, u, 1.0 / 9.0);
+  p = __builtin_fma(p, u, 1.0 / 7.0);
+  p = __builtin_fma(p, u, 1.0 / 5.0);
+  p = __builtin_fma(p, u, 1.0 / 3.0);
+  p = __builtin_fma(p, u, 1.0);
+  return __builtin_fma((double)e, 0.69314718055994531, (t + t) * p);
+}
+
 // A wave per row (or two): the sum of its pieces, and its k best out of their lists, sorted; then the
 // rows' lists are merged pair by pair. (Finding every entry's place by halving in the other rows'
 // lists is W^2 log k reads of LDS: as fast for 4 beams, 1 us more for 8, 11 more for 32.)
@@ -444,7 +469,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
       live = !bad && M > -INFINITY;
       // (the pieces' exponentials are powers of 2 of x * kLog2e, which as a float is 1.3e-8 off: what
       // is left of that is 1.3e-8 times the row's entropy, 1e-7)
-      log_sum = log2(S) / (double)kLog2e;
+      log_sum = ln64(S) * (1.0 / (0.69314718055994531 * (double)kLog2e));
     }
     if (live) {
       // lists begin with their largest: at least k entries reach the k-th of (the first 64 of) those

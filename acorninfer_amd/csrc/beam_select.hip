@@ -113,6 +113,9 @@ __device__ __forceinline__ u64 read_lane(u64 v, int lane) {
   return (u64)read_lane((uint32_t)(v >> 32), lane) << 32 | read_lane((uint32_t)v, lane);
 }
 
+// (of a condition, that is: __ballot makes an integer of it first)
+__device__ __forceinline__ u64 ballot(bool c) { return __builtin_amdgcn_ballot_w64(c); }
+
 __device__ __forceinline__ int lanes_before(u64 mask) {        // set bits below this lane's
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
@@ -124,6 +127,7 @@ template <int D, typename U>
 __device__ __forceinline__ U exchange(U v, int lane, bool falls) {
   const U o = lane_xor<D>(v, lane);
   const bool larger = ((lane & D) == 0) == falls;
+  if constexpr (sizeof(U) == 4) return larger ? max(o, v) : min(o, v);   // (a swap to an operand)
   return (o > v) == larger ? o : v;
 }
 template <int D, typename U>
@@ -141,6 +145,19 @@ __device__ __forceinline__ U sort_wave(U v, int lane) {
   v = exchanges<8>(v, lane, (lane & 16) != 0);
   v = exchanges<16>(v, lane, (lane & 32) != 0);
   return exchanges<32>(v, lane, false);
+}
+// The first n lanes' values in falling order, zeros (no larger than any) behind them: 10 exchanges for
+// up to 16, 15 for up to 32.
+template <typename U>
+__device__ __forceinline__ U sort_first(U v, int lane, int n) {
+  v = exchanges<1>(v, lane, (lane & 2) == 0);
+  v = exchanges<2>(v, lane, (lane & 4) == 0);
+  v = exchanges<4>(v, lane, (lane & 8) == 0);
+  v = exchanges<8>(v, lane, n <= 16 || (lane & 16) == 0);
+  if (n <= 16) return v;
+  v = exchanges<16>(v, lane, n <= 32 || (lane & 32) == 0);
+  if (n <= 32) return v;
+  return exchanges<32>(v, lane, true);
 }
 // The 64 best of a falling list and a rising one, falling.
 template <typename U>
@@ -264,7 +281,7 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
     __builtin_amdgcn_sched_barrier(0);
   }
   s = (s + lost) * __builtin_amdgcn_exp2f(-__builtin_fmaf(fmaxf(m, -kHuge), kLog2e, -R));
-  if (__ballot(fabsf(m) >= kHuge && m > -INFINITY) != 0) {     // (x log2 e is too coarse there)
+  if (ballot(fabsf(m) >= kHuge && m > -INFINITY) != 0) {     // (x log2 e is too coarse there)
     const float ref = m == -INFINITY ? 0.f : m;
     s = 0.f;
 #pragma unroll
@@ -276,14 +293,19 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
   }
 
   const uint32_t rising = sort_wave(order32(m), lane);
-  const float mw = unorder32(read_lane(rising, kWave - 1)), refw = mw == -INFINITY ? 0.f : mw;
+  const float mw = over_lanes(m, lane, [](float a, float b) { return fmaxf(a, b); });
+  const float refw = mw == -INFINITY ? 0.f : mw;
   const float sw = over_lanes(s * __builtin_amdgcn_exp2f((m - refw) * kLog2e), lane,
                               [](float a, float b) { return a + b; });
+  // (read where all lanes are active: in a branch of one, what the others' values come from may be
+  // computed for that one alone)
+  const uint32_t part_k = read_lane(rising, kWave - (k + kPartWaves - 1) / kPartWaves);
+  const uint32_t wave_k = read_lane(rising, kWave - k);
   if (lane == 0) {
     wave_m[wid] = mw;
     wave_s[wid] = sw;
-    some[wid] = read_lane(rising, kWave - (k + kPartWaves - 1) / kPartWaves);
-    most[wid] = read_lane(rising, kWave - k);
+    some[wid] = part_k;
+    most[wid] = wave_k;
   }
   __syncthreads();
   u64 least = (u64)max(max(min(min(some[0], some[1]), min(some[2], some[3])),
@@ -293,39 +315,46 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
   for (;;) {
     const float floor = unorder32((uint32_t)(least >> 32));
     int n = 0;                                                 // found by this wave
-    uint32_t todo = (uint32_t)((1ull << NV) - 1);              // its vectors (a bit for each of a lane's)
-    while (todo) {
+    // all vectors, or where the queue does not hold them as many at a time as fit for certain
+    constexpr int kTurn = kQueue / kWave;
+    uint32_t turn = ~0u;
+    for (;;) {
       int q = 0;                                               // queued
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        if (NV * kWave > kQueue && (!(todo >> u & 1) || q > kQueue - kWave)) continue;
-        todo &= ~(1u << u);
+        if (NV > kTurn && !(turn >> u & 1)) continue;
         const bool any = vmax[u] >= floor;
-        const u64 mask = __ballot(any);
+        const u64 mask = ballot(any);
         if (mask == 0) continue;
-        if (any) {
-          const int i = q + lanes_before(mask);
+        const int i = q + lanes_before(mask);
+        if (any && (NV <= kTurn || i < kQueue)) {
           queue[wid][i] = x[u];
           first[wid][i] = (uint32_t)(p0 + tid + u * kPartNT) * E;
         }
         q += __popcll(mask);
       }
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-      for (int i = lane; i < (q + kWave - 1) / kWave * kWave; i += kWave) {
-        const bs_u32x4 w = queue[wid][min(i, kQueue - 1)];
-        const uint32_t token = first[wid][min(i, kQueue - 1)];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const u64 key = key_of(vec_elem<T>(w, e), token + e);
-          const bool in = i < q && key >= least;
-          const u64 mask = __ballot(in);
-          const int to = n + lanes_before(mask);
-          if (in && to < kHeld) held[wid][to] = key;
-          n += __popcll(mask);
-        }
+      if (NV > kTurn && q > kQueue) {
+        turn = (1u << kTurn) - 1;
+        continue;
       }
       __builtin_amdgcn_wave_barrier();
+      // an element to a lane
+      const uint8_t* values = (const uint8_t*)queue[wid];
+#pragma unroll 1
+      for (int i0 = 0; i0 < q * E; i0 += kWave) {
+        const int i = i0 + lane, j = min(i, q * E - 1);
+        T value;
+        __builtin_memcpy(&value, values + j * sizeof(T), sizeof(T));
+        const u64 key = key_of((float)value, first[wid][j / E] + j % E);
+        const bool in = i < q * E && key >= least;
+        const u64 mask = ballot(in);
+        const int to = n + lanes_before(mask);
+        if (in && to < kHeld) held[wid][to] = key;
+        n += __popcll(mask);
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (NV <= kTurn || turn >> (NV - 1)) break;
+      turn <<= kTurn;
     }
     if (lane == 0) found[wid] = n;
     __syncthreads();
@@ -346,10 +375,15 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
         for (int c = 0; c < kPartWaves - 1; ++c)
           if (j >= end[c]) w = c + 1, from = j - end[c];
         const u64 v = j < end[kPartWaves - 1] ? held[w][from] : 0;
-        if (__ballot(v > read_lane(top, k - 1)) == 0) continue;
+        if (i == 0) {
+          top = sort_first(v, lane, end[kPartWaves - 1]);
+          continue;
+        }
+        if (ballot(v > read_lane(top, k - 1)) == 0) continue;
         top = merge_wave(top, sort_wave(v, lane), lane);
       }
-      if (lane == 0) limit = read_lane(top, k - 1);
+      const u64 kth = read_lane(top, k - 1);
+      if (lane == 0) limit = kth;
     }
     if (!more) {
       if (wid == 0 && lane < k) lists[at * k + lane] = top;
@@ -484,7 +518,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
         for (int a = 0; a < kAhead; ++a) {
           const int i = i0 + a * kWave + lane;
           const bool in = i < total && ahead[a] >= least;
-          const u64 mask = __ballot(in);
+          const u64 mask = ballot(in);
           if (in) buf[n + lanes_before(mask)] = ahead[a];
           n += __popcll(mask);
           ahead[a] = lp[min(i + kAhead * kWave, total - 1)];
@@ -499,7 +533,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
         }
       }
     }
-    const int have = live ? min(__popcll(__ballot(top != 0)), k) : 0;
+    const int have = live ? min(__popcll(ballot(top != 0)), k) : 0;
     uint32_t token = ~(uint32_t)top;
     u64 key = 0;
     if (lane < have)

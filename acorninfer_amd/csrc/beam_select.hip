@@ -159,10 +159,21 @@ __device__ __forceinline__ U sort_first(U v, int lane, int n) {
   if (n <= 32) return v;
   return exchanges<32>(v, lane, true);
 }
-// The 64 best of a falling list and a rising one, falling.
+// The value of lane 63 - lane.
+template <typename U>
+__device__ __forceinline__ U mirror(U v, int lane) {
+  auto row = [](uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, false);   // rows mirrored
+  };
+  if constexpr (sizeof(U) == 8)
+    return (U)mirror((uint32_t)(v >> 32), lane) << 32 | mirror((uint32_t)v, lane);
+  else
+    return lane_xor<32>(lane_xor<16>(row(v), lane), lane);
+}
+// The 64 best of two falling lists, falling.
 template <typename U>
 __device__ __forceinline__ U merge_wave(U top, U other, int lane) {
-  return exchanges<32>(max(top, other), lane, true);
+  return exchanges<32>(max(top, mirror(other, lane)), lane, true);
 }
 
 // The sum, or another fold, over the wave, in every lane.
@@ -375,12 +386,9 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
         for (int c = 0; c < kPartWaves - 1; ++c)
           if (j >= end[c]) w = c + 1, from = j - end[c];
         const u64 v = j < end[kPartWaves - 1] ? held[w][from] : 0;
-        if (i == 0) {
-          top = sort_first(v, lane, end[kPartWaves - 1]);
-          continue;
-        }
         if (ballot(v > read_lane(top, k - 1)) == 0) continue;
-        top = merge_wave(top, sort_wave(v, lane), lane);
+        const u64 batch = sort_first(v, lane, end[kPartWaves - 1] - i);
+        top = i == 0 ? batch : merge_wave(top, batch, lane);
       }
       const u64 kth = read_lane(top, k - 1);
       if (lane == 0) limit = kth;
@@ -408,7 +416,7 @@ __global__ __launch_bounds__(kPartNT, 4) void beam_part_kernel(
 
 // ---- the join ---------------------------------------------------------------------------------
 constexpr int kJoinWaves = 16;
-constexpr int kAhead = 4;                      // loads of a lane in flight
+constexpr int kAhead = 5;                      // loads of a lane in flight
 
 // An entry of the group's list: s as a key, then its place (beam * 64 + rank in the beam's list): the
 // larger key first, of equal ones the lower place.
@@ -511,6 +519,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
       const u64 least = max((u64)reaches << 32, (u64)1);
       u64* buf = reach[wid];
       int n = 0;
+      bool empty = true;
 #pragma unroll 1
       for (int i0 = 0; i0 < total; i0 += kAhead * kWave) {
         const bool rest = i0 + kAhead * kWave >= total;
@@ -526,9 +535,11 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
 #pragma unroll 1
         while (n >= kWave || (n > 0 && rest)) {                // 64 of them into the list
           __builtin_amdgcn_wave_barrier();
-          n -= kWave;
-          const u64 e = n + lane >= 0 ? buf[n + lane] : 0;
-          top = merge_wave(top, sort_wave(e, lane), lane);
+          const int from = max(n - kWave, 0), some = n - from;
+          const u64 batch = sort_first(lane < some ? buf[from + lane] : (u64)0, lane, some);
+          top = empty ? batch : merge_wave(top, batch, lane);
+          empty = false;
+          n = from;
           __builtin_amdgcn_wave_barrier();
         }
       }

@@ -430,16 +430,16 @@ __device__ __forceinline__ bool comes_before(const Entry& a, const Entry& b) {
 __device__ __forceinline__ Entry entry_of(const u64 (*keys)[kMaxK], int w, int k, int i) {
   return i < k ? Entry{keys[w][i], (uint32_t)(w * kWave + i)} : Entry{0, 0xFFFFFFFFu};
 }
-template <int D = 32>
-__device__ __forceinline__ Entry exchange_entries(const Entry& v, int lane) {
+template <int D>
+__device__ __forceinline__ Entry exchange_entries(const Entry& v, int lane, bool ordered) {
   const Entry o = {lane_xor<D>(v.key, lane), lane_xor<D>(v.place, lane)};
-  const Entry r = comes_before(o, v) == ((lane & D) == 0) ? o : v;
-  if constexpr (D > 1) return exchange_entries<D / 2>(r, lane);
+  const Entry r = comes_before(o, v) == (((lane & D) == 0) == ordered) ? o : v;
+  if constexpr (D > 1) return exchange_entries<D / 2>(r, lane, ordered);
   return r;
 }
 // The 64 first of a list in order and one in the opposite order, in order.
 __device__ __forceinline__ Entry merge_entries(const Entry& a, const Entry& b, int lane) {
-  return exchange_entries(comes_before(b, a) ? b : a, lane);
+  return exchange_entries<32>(comes_before(b, a) ? b : a, lane, true);
 }
 
 // ln s to 1e-12 for normal s > 0 (2^31 pieces of sums past any need): s = 2^e f with f between
@@ -571,14 +571,26 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     if (lane == 0) status[row] = bad;
   }
   __syncthreads();
-  // the waves' lists pair by pair
-  Entry best = entry_of(keys, wid, k, lane);
-  if (wid + waves < W) best = merge_entries(best, entry_of(keys, wid + waves, k, kWave - 1 - lane), lane);
-  for (int half = waves > 1 ? 1 << (31 - __builtin_clz(waves - 1)) : 0; half > 0; half >>= 1) {
+  // a wave takes as many lists as fit into its lanes, every second one turned round, and merges them
+  // in pairs; then the waves' lists pair by pair
+  const int size = k <= 8 ? 8 : k <= 16 ? 16 : k <= 32 ? 32 : kWave, per = kWave / size;
+  const int parts = (W + per - 1) / per, most = min(W, per) * size;
+  Entry best = {0, 0xFFFFFFFFu};
+  if (wid < parts) {
+    const int w = wid * per + lane / size, i = lane % size;
+    if (w < W) best = entry_of(keys, w, k, (w & 1) && size < kWave ? size - 1 - i : i);
+    if (size <= 8 && most > 8) best = exchange_entries<8>(best, lane, (lane & 16) == 0);
+    if (size <= 16 && most > 16) best = exchange_entries<16>(best, lane, (lane & 32) == 0);
+    if (size <= 32 && most > 32) best = exchange_entries<32>(best, lane, true);
+    if (wid + waves < parts)                                   // (more than 16 lists of more than 32)
+      best = merge_entries(best, entry_of(keys, wid + waves, k, kWave - 1 - lane), lane);
+  }
+  const int lists_left = min(parts, waves);
+  for (int half = lists_left > 1 ? 1 << (31 - __builtin_clz(lists_left - 1)) : 0; half > 0; half >>= 1) {
     pair_key[wid][lane] = best.key;
     pair_place[wid][lane] = best.place;
     __syncthreads();
-    if (wid < half && wid + half < waves)
+    if (wid < half && wid + half < lists_left)
       best = merge_entries(best, Entry{pair_key[wid + half][kWave - 1 - lane],
                                        pair_place[wid + half][kWave - 1 - lane]}, lane);
     __syncthreads();

@@ -280,12 +280,20 @@ __global__ __launch_bounds__(kTableNT) void beam_tables_kernel(int32_t* tables, 
 // steps of a group. Every stretch is walked from each beam at its end: a map of beams. A
 // hypothesis's beam at a stretch's end comes out of the maps of the stretches behind it (those
 // of a wave composed by doubling), and the stretch is walked once more from there with the tokens.
-// 16 groups of 8 beams, 2048 steps: 16 dependent steps, 16 more with the tokens, 16 us (73 with one
-// stretch to a wave); the exchanges between lanes (LDS) of the 16 CUs that have a group.
-// 1 group of 4 beams, 100 steps: 6.4 us.
+// Up to four workgroups take a group: each makes all the maps and writes the tokens of a quarter of the
+// waves (of consecutive ones, so that a SIMD has one each). 16 groups of 8 beams, 2048 steps: 16
+// dependent steps, 16 more with the tokens, 12 us (16 with one workgroup, 73 with one stretch to a
+// wave): instructions and exchanges between lanes of the CUs that have a group. 1 group of 4 beams,
+// 100 steps: 4.2 us.
 constexpr int kTraceWaves = 16;
+constexpr int kPlaces = 256;                       // workgroups that run side by side
 constexpr int kTile = 16;                          // steps whose rows are loaded together
+// Stretches up to here are written as they come, others 16 tokens of a hypothesis at a time out of LDS:
+// 4 groups of 4 beams, 256 steps (stretches of 1) 6.0 us and 7.4, 16 of 4, 2048 steps (8) 8.8 and
+// 10.0; of stretches of 16 64 groups of 8 beams take 16.5 and 15.1, 128 groups 34 and 23.
+constexpr int kDirect = 8;
 
+template <bool DIRECT>
 __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
     const int32_t* __restrict__ tokens, const int32_t* __restrict__ parents,
     const int32_t* __restrict__ steps, const int32_t* __restrict__ beams,
@@ -293,7 +301,7 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
   // beam at a stretch's end -> before its first step; and through the wave's stretches behind it too
   __shared__ int8_t one[kTraceWaves * kWave], rest[kTraceWaves * kWave];
   __shared__ int8_t part[kMaxBeams];               // a hypothesis's beam before the stretch it ends in
-  __shared__ int64_t stage[kTraceWaves][kWave][kTile + 1];
+  __shared__ int64_t stage[DIRECT ? 1 : kTraceWaves][kWave][kTile + 1];
   const int g = blockIdx.x, lane = threadIdx.x % kWave, wid = threadIdx.x / kWave;
   const int B = 1 << shift, S = kWave >> shift, j = lane >> shift, h = lane & (B - 1);
   const int own = lane - h;                        // the first lane of the stretch
@@ -306,14 +314,24 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
     return cur < 0 ? -1 : inside(next);
   };
   // steps a + L - kTile (i + 1) .. of every stretch, one beam to a lane
+  const uint32_t stride = (uint32_t)G * W;         // (below 2^31: the host's check)
+  const int64_t column = (int64_t)g * W + min(h, W - 1);
   auto load = [&](const int32_t* from, int i, int (&x)[kTile]) {
+    const int t0 = a + L - kTile * (i + 1);
 #pragma unroll
-    for (int o = 0; o < kTile; ++o) {
-      const int t = min(max(a + L - kTile * (i + 1) + o, 0), T - 1);
-      x[o] = from[((size_t)t * G + g) * W + min(h, W - 1)];
+    for (int o = kTile - 1; o >= 0; --o) {
+      if (kTile * (i + 1) - o > L) break;          // (before every stretch)
+      x[o] = from[column + (uint64_t)(uint32_t)min(t0 + o, T - 1) * stride];
     }
   };
   const int tiles = (L + kTile - 1) / kTile;
+  // (a wave may have no steps, and the tokens are taken by one workgroup of the group)
+  const bool some_steps = (int64_t)wid * S * L < T;
+  const bool takes = some_steps && wid / (kTraceWaves / (int)gridDim.y) == (int)blockIdx.y;
+  // where a stretch is one tile both passes' rows are loaded here, once
+  int row[kTile], token[kTile];
+  if (some_steps) load(parents, 0, row);
+  if (takes) load(tokens, 0, token);
   int all = h < W ? h : -1;
   for (int h0 = 0; h0 < M; h0 += B) {
     const int m = h0 + h;
@@ -323,9 +341,8 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
     const int ends = last >= 0 ? last / L : -1;    // the stretch it ends in
     int mine = -1;
     const bool some = __ballot(q == ends) != 0;    // a hypothesis ends in one of the wave's stretches
-    for (int i = 0; i < ((int64_t)wid * S * L < T && (h0 == 0 || some) ? tiles : 0); ++i) {
-      int row[kTile];
-      load(parents, i, row);
+    for (int i = 0; i < (some_steps && (h0 == 0 || some) ? tiles : 0); ++i) {
+      if (tiles > 1) load(parents, i, row);
 #pragma unroll
       for (int o = kTile - 1; o >= 0; --o) {
         if (kTile * (i + 1) - o > L) break;        // (before every stretch)
@@ -364,20 +381,26 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
       }
     }
     __syncthreads();                               // (part is written again)
-    for (int i = 0; i < ((int64_t)wid * S * L < T ? tiles : 0); ++i) {  // (a wave may have no steps)
-      int row[kTile], token[kTile];
-      load(parents, i, row);
-      load(tokens, i, token);
+    for (int i = 0; i < (takes ? tiles : 0); ++i) {
+      if (tiles > 1) {
+        load(parents, i, row);
+        load(tokens, i, token);
+      }
 #pragma unroll
       for (int o = kTile - 1; o >= 0; --o) {
         if (kTile * (i + 1) - o > L) break;
         const int t = a + L - kTile * (i + 1) + o;
         if (t == last) cur = beam;
         const int tok = at(token[o], cur);
-        stage[wid][lane][o] = cur < 0 || t > last ? pad : (int64_t)tok;
+        const int64_t value = cur < 0 || t > last ? pad : (int64_t)tok;
+        if (!DIRECT)
+          stage[wid][lane][o] = value;
+        else if (hyp && t < e)
+          out[((size_t)g * M + m) * T + t] = value;
         const int next = hop(row[o], cur);
         if (t < e && t <= last) cur = next;
       }
+      if (DIRECT) continue;
       __builtin_amdgcn_wave_barrier();
       // kTile tokens of a lane side by side
       for (int r = 0; r < kWave * kTile; r += kWave) {
@@ -480,14 +503,19 @@ extern "C" int acorn_beam_trace(const int32_t* tokens, const int32_t* parents,
       M > 0x7fffffff - kMaxBeams)
     return ACORN_ERR_SHAPE;
   if (W > kMaxBeams) return ACORN_ERR_UNSUPPORTED;
+  if (groups * W > 0x7fffffff) return ACORN_ERR_SHAPE;
   if (T == 0 || groups == 0 || M == 0) return ACORN_OK;
   if (!tokens || !parents || !steps || !beams || !out) return ACORN_ERR_VALUE;
   int shift = 0;
   while ((1 << shift) < W) ++shift;
   const int64_t stretches = (int64_t)kTraceWaves * (kWave >> shift);
-  beam_trace_kernel<<<dim3((unsigned)groups), dim3(kTraceWaves * kWave), 0, (hipStream_t)stream>>>(
-      tokens, parents, steps, beams, out, (int)T, (int)groups, (int)W, (int)M,
-      (int)((T + stretches - 1) / stretches), shift, pad);
+  // (where the chip has a place, a CU, for each of them: 128 groups of 8 beams, 2048 steps, 26 us with
+  // one workgroup each, 23 with two, 37 with four)
+  const unsigned parts = groups * 4 <= kPlaces ? 4 : groups * 2 <= kPlaces ? 2 : 1;
+  const int L = (int)((T + stretches - 1) / stretches);
+  (L <= kDirect ? beam_trace_kernel<true> : beam_trace_kernel<false>)<<<
+      dim3((unsigned)groups, parts), dim3(kTraceWaves * kWave), 0, (hipStream_t)stream>>>(
+      tokens, parents, steps, beams, out, (int)T, (int)groups, (int)W, (int)M, L, shift, pad);
   ACORN_LAUNCH_CHECK();
   return ACORN_OK;
 }

@@ -609,7 +609,8 @@ int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, int32_t* ta
 /*
  * Hypotheses out of the logs tokens, parents [T, G, W]: out[g, m, t] (int64 [G, M, T]) =
  * tokens[t, g, b_t] for t < steps[g, m], with b of the last step beams[g, m] and
- * b_{t-1} = parents[t, g, b_t]; pad behind, and before a beam outside [0, W). T < 2^30.
+ * b_{t-1} = parents[t, g, b_t]; pad behind, and before a beam outside [0, W). T < 2^30,
+ * groups * W < 2^31.
  */
 int acorn_beam_trace(const int32_t* tokens, const int32_t* parents, const int32_t* steps,
                      const int32_t* beams, int64_t* out, int64_t T, int64_t groups, int64_t W,

@@ -559,6 +559,7 @@ def test_trace_refuses_logs_past_its_whole_numbers():
     from acorninfer_amd import _lib
     L, p = _lib.lib(), 64
     assert L.acorn_beam_trace(p, p, p, p, p, 2**30, 1, 1, 1, 0, None) == _lib.ERR_SHAPE
+    assert L.acorn_beam_trace(p, p, p, p, p, 1, 2**27, 16, 1, 0, None) == _lib.ERR_SHAPE
 
 
 def test_a_length_penalty_past_32_bits_is_refused():
@@ -576,3 +577,25 @@ def test_a_length_penalty_past_32_bits_is_refused():
         assert L.acorn_beam_advance(*[p] * 24, 1, 2, 4, steps, 0, alpha, 0, 0, None) == _lib.ERR_VALUE
         with pytest.raises(ValueError):
             b.check_length_penalty(alpha, steps)
+
+
+@gpu
+@pytest.mark.parametrize("T,G,W,M", [(600, 100, 4, 4), (600, 200, 4, 5), (2100, 130, 8, 8), (4500, 70, 32, 3),
+                                     (1025, 65, 2, 2), (1030, 3, 4, 9)])
+def test_trace_of_many_groups(T, G, W, M):
+    """Batches whose groups are taken by one, two and four workgroups, stretches of 1 to 141 steps."""
+    g = torch.Generator().manual_seed(T + G)
+    tokens = torch.randint(0, 150000, (T, G, W), generator=g).int()
+    parents = torch.randint(0, W, (T, G, W), generator=g).int()
+    steps = torch.randint(T - 9, T + 1, (G, M), generator=g).int()
+    steps[::7, 0] = torch.randint(0, T, (len(steps[::7]),), generator=g).int()
+    beams = torch.randint(0, W, (G, M), generator=g).int()
+    got = _beam().beam_trace(tokens.cuda(), parents.cuda(), steps.cuda(), beams.cuda(), pad=-7).cpu()
+    want = torch.full((G, M, T), -7, dtype=torch.int64)       # (the oracle's steps, groups side by side)
+    at, rows = beams.long(), torch.arange(G)[:, None]
+    for t in range(T - 1, -1, -1):
+        on = t < steps
+        want[:, :, t] = torch.where(on, tokens[t][rows, at].long(), -7)
+        at = torch.where(on, parents[t][rows, at].long(), at)
+    assert torch.equal(got, want)
+    assert torch.equal(want[:2], ref.trace_ref(tokens[:, :2], parents[:, :2], steps[:2], beams[:2], pad=-7))

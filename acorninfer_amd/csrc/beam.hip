@@ -33,7 +33,7 @@ struct BeamFields {
 
 // One wave per group, a candidate to a lane; a group's old state is in registers before any of the
 // new one is written, so that both may be the same memory. Latency: one round of loads, then some
-// ballots and 2 W comparisons across lanes. 1 group of 4 beams 3.4 us, 64 of 16 5.3.
+// ballots and 2 W comparisons across lanes. 1 group of 4 beams 3.2 us, 64 of 16 4.6.
 __global__ __launch_bounds__(kWave) void beam_advance_kernel(
     const BeamFields in, const BeamFields out, int32_t* token_log, int32_t* parent_log,
     const float* cand_score, const int32_t* cand_beam, const int64_t* cand_token,
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kWave) void beam_advance_kernel(
   const int ft = beam ? fin_token : took ? fresh_token : 0;
   int rank = 0;
   for (int j = 0; j < 2 * W; ++j) {
-    const float o = __shfl(fs, j);
+    const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fs), j));
     rank += o > fs || (o == fs && j < lane);
   }
   const bool kept = lane < 2 * W && rank < W;
@@ -142,7 +142,7 @@ struct Plan {
 __device__ __forceinline__ Plan plan_pages(int parent, int page, int W, int lane) {
   bool first = lane < W, child = false;
   for (int j = 0; j < W; ++j) {
-    const int pj = __shfl(parent, j);
+    const int pj = __builtin_amdgcn_readlane(parent, j);
     first &= !(j < lane && pj == parent);
     child |= pj == lane;
   }
@@ -235,41 +235,41 @@ __global__ __launch_bounds__(kCopyNT) void beam_copy_kernel(
   }
 }
 
-// A thread per column, which reads the group's entries of it before it writes them; the plan comes
-// out of the column that these hold. A launch of its own, as every workgroup of the copy reads the
+// A thread per column, which reads the group's entries of it before it writes them; the wave that has
+// the column with the partly filled pages works the plan out. A launch of its own, as every workgroup of the copy reads the
 // pages that it replaces: 2.6 us for 1 group, 4 for 16.
-constexpr int kTableNT = 256;
+constexpr int kTableNT = 256, kTableUnroll = 8;
 
 __global__ __launch_bounds__(kTableNT) void beam_tables_kernel(int32_t* tables, const int32_t* lens,
                                                                const int32_t* parents, int W, int P,
                                                                int width) {
-  __shared__ int32_t held[kMaxBeams][kTableNT];
-  __shared__ int32_t par[kMaxBeams], taken[kMaxBeams];
-  const int g = blockIdx.y, lane = threadIdx.x % kWave;
+  __shared__ int32_t held[kMaxBeams][kTableNT];                // (each wave reads its own columns)
+  const int g = blockIdx.y, lane = threadIdx.x % kWave, w0 = threadIdx.x - lane;
   const size_t gw = (size_t)g * W;
-  const int c0 = blockIdx.x * kTableNT, column = c0 + threadIdx.x;
-  int32_t* t = tables + gw * width + min(column, width - 1);
+  const int first = blockIdx.x * kTableNT + w0, column = first + lane;
   const int n = max(lens[gw], 0), fill = n % P, c = n / P;
   const int parent = parent_of(parents, gw, W, lane);
-  for (int w = 0; w < W; ++w) held[w][threadIdx.x] = t[(size_t)w * width];
-  if (c0 > c) return;                                          // columns of the future
-  __syncthreads();
-  if (threadIdx.x < kWave) {
-    const bool here = fill && c < width && c < c0 + kTableNT;
-    const int page = held[lane < W ? lane : 0][here ? c - c0 : 0];
-    const Plan plan = plan_pages(parent, page, W, lane);
-    if (lane < W) {
-      par[lane] = parent;
-      taken[lane] = plan.to;
-    }
+  int32_t* t = tables + gw * width;
+  for (int b = 0; b < W; b += kTableUnroll) {
+    int32_t x[kTableUnroll];
+#pragma unroll
+    for (int i = 0; i < kTableUnroll; ++i)
+      if (b + i < W) x[i] = (t + (size_t)(b + i) * width)[min(column, width - 1)];
+#pragma unroll
+    for (int i = 0; i < kTableUnroll; ++i)
+      if (b + i < W) held[b + i][threadIdx.x] = x[i];
   }
-  __syncthreads();
-  if (column >= width || column > c || (column == c && !fill)) return;
+  if (first > c) return;                                       // columns of the future
+  __builtin_amdgcn_wave_barrier();
+  int to = 0;
+  if (fill && c < width && c < first + kWave)
+    to = plan_pages(parent, held[lane < W ? lane : 0][w0 + c - first], W, lane).to;
+  const bool mine = column < width && (column < c || (column == c && fill));
+#pragma unroll 4
   for (int w = 0; w < W; ++w) {
-    if (column == c)
-      t[(size_t)w * width] = taken[w];
-    else if (par[w] != w)
-      t[(size_t)w * width] = held[par[w]][threadIdx.x];
+    const int from = __builtin_amdgcn_readlane(parent, w), page = __builtin_amdgcn_readlane(to, w);
+    if (mine && (column == c || from != w))
+      (t + (size_t)w * width)[column] = column == c ? page : held[from][threadIdx.x];
   }
 }
 

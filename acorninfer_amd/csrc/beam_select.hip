@@ -16,12 +16,12 @@
 // the order they are met in. Tokens at -inf are no candidates here: the join puts
 // them behind the others where a row has too few.
 //
-// Rows of 151936 in bf16, from a graph: 1 row 9.2 us, 4 rows 10.4, 64 rows 15.4, 256 rows 25 (78 MB:
-// 3.1 TB/s), 1024 rows 72 (4.4 TB/s). Few rows are latency: two launches, each with a chain of
-// loads, a sort and a join. Of the 19 us of 256 rows' pieces the loads alone take 11.7 (from the
-// last cache; 13.5 from memory), with the sums 13.5; the rest comes behind the loads in all
-// workgroups at once: queue 2.9, look 1, sort 1.5, write 1.5. Many rows are bound by VALU work
-// (46 instructions per vector of 8, 9 of them exponentials) beside the loads.
+// Rows of 151936 in bf16, from a graph: 1 row 7.6 us, 4 rows 8.4, 64 rows 13.2, 256 rows 23.4 (78 MB:
+// 3.3 TB/s), 1024 rows 71 (4.4 TB/s). Few rows are latency: two launches, each with a chain of
+// loads, a sort and a join. Of 256 rows' pieces, 19 us, the workgroups have their loads after 6 to
+// 15.5 us, and each takes 3 more: threshold 0.7, queue 1.1, look 0.4, sort and write 0.9; that of the
+// last ones has nothing beside it. Many rows are bound by VALU work (46 instructions per vector of 8,
+// 9 of them exponentials) beside the loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -445,7 +445,7 @@ __device__ __forceinline__ Entry merge_entries(const Entry& a, const Entry& b, i
 // ln s to 1e-12 for normal s > 0 (2^31 pieces of sums past any need): s = 2^e f with f between
 // sqrt(1/2) and sqrt(2), ln f = 2 atanh t = 2 (t + t^3/3 + ... ), t = (f - 1) / (f + 1), |t| < 0.172: the
 // term of t^15 is below 5e-13. The library's log2 holds every size to the last place: 0.2 us more of
-// the launch's 5, in code that is cold.
+// the launch's 4, in code that is cold.
 __device__ __forceinline__ double ln64(double s) {
   double f = __builtin_amdgcn_frexp_mant(s);                   // 1/2 .. 1
   int e = __builtin_amdgcn_frexp_exp(s);
@@ -605,9 +605,9 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
 
 // Vectors of a lane and pieces of a row: the shortest pieces with which a batch has no more
 // workgroups than the chip has places for them (four to a CU), so that it runs in one round, each
-// with one sort. 16 / 32 / 128 / 256 rows of 151936, 4 beams: 12.4 / 12.5 / 18.6 / 24.5 us; with up
-// to 512 workgroups 11.7 / 12.8 / 19.3 / 25.4, with up to 2048 12.6 / 15.5 / 20.5 / 25.0. 19 vectors
-// is the most that 128 registers hold beside their maxima (20 spill: 1 us more for 256 rows).
+// with one sort. 16 / 32 / 128 / 256 rows of 151936, 4 beams: 9.9 / 10.6 / 16.3 / 21.9 us; with up to
+// 512 workgroups 9.3 / 10.5 / 16.7 / 22.1, with up to 2048 9.8 / 11.8 / 16.6 / 22.6. 19 vectors is
+// the most that 128 registers hold beside their maxima (20 spill: 1 us more for 256 rows).
 struct Pieces {
   int count, nv;
 };

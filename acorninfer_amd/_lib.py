@@ -93,8 +93,11 @@ _SIGNATURES = {
     "acorn_paged_prefill_workspace_kv8": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
     "acorn_beam_select": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
                           _vp],
+    "acorn_beam_select_low": [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _i64, _i32, _vp],
     "acorn_beam_select_workspace": [_i64, _i64, _i64, _i64, _i32, _vp],
     "acorn_beam_advance": [_vp] * 24 + [_i64] * 5 + [ctypes.c_double, _i32, _i64, _vp],
+    "acorn_beam_advance_low": [_vp] * 26 + [_i64] * 5 + [ctypes.c_double, _i32, _i64, _vp],
     "acorn_beam_reorder": [_vp] * 6 + [_i64] * 9 + [_vp],
     "acorn_beam_trace": [_vp] * 5 + [_i64] * 5 + [_vp],
     "acorn_block_tables": [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp],

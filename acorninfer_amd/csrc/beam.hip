@@ -37,8 +37,8 @@ struct BeamFields {
 __global__ __launch_bounds__(kWave) void beam_advance_kernel(
     const BeamFields in, const BeamFields out, int32_t* token_log, int32_t* parent_log,
     const float* cand_score, const int32_t* cand_beam, const int64_t* cand_token,
-    const int64_t* ends, int G, int W, int K, int T, int n_ends, double alpha, int early,
-    int64_t pad) {
+    const int64_t* ends, const float* cand_low, float* low, int G, int W, int K, int T, int n_ends,
+    double alpha, int early, int64_t pad) {
   const int g = blockIdx.x, lane = threadIdx.x;
   const size_t gw = (size_t)g * W;
   const bool beam = lane < W, cand = lane < K;
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kWave) void beam_advance_kernel(
   const int fin_length = in.fin_length[gw + l], fin_beam = in.fin_beam[gw + l],
             fin_token = in.fin_token[gw + l];
   const size_t ck = (size_t)g * K + (cand ? lane : 0);
-  const float cs = cand_score[ck];
+  const float cs = cand_score[ck], cl = cand_low ? cand_low[ck] : 0.f;
   const int cb = cand_beam[ck];
   const int64_t ct = cand_token[ck];
   bool end = false;
@@ -76,28 +76,30 @@ __global__ __launch_bounds__(kWave) void beam_advance_kernel(
   }
 
   // the next beams: the first W candidates that go on
-  const bool valid = cand && cs > -INFINITY && cb >= 0 && cb < W;
+  const double sum = (double)cs + (double)cl;
+  const bool valid = cand && sum > -INFINITY && cb >= 0 && cb < W;
   const bool goes = valid && !end;
   const uint64_t gm = __ballot(goes);
   const int slot = __popcll(gm & lanes_below(lane)), live = min(__popcll(gm), W);
   const size_t log = ((size_t)t * G + g) * W;
-  auto put = [&](int i, float s, int64_t id, int parent) {
+  auto put = [&](int i, float s, float rest, int64_t id, int parent) {
     out.scores[gw + i] = s;
+    if (low) low[gw + i] = rest;
     out.ids[gw + i] = id;
     out.parents[gw + i] = parent;
     token_log[log + i] = (int32_t)id;
     parent_log[log + i] = parent;
   };
-  if (goes && slot < W) put(slot, cs, ct, cb);
-  if (beam && lane >= live) put(lane, -INFINITY, pad, lane);
-  const float best = gm ? __shfl(cs, __ffsll((unsigned long long)gm) - 1) : -INFINITY;
+  if (goes && slot < W) put(slot, cs, cl, ct, cb);
+  if (beam && lane >= live) put(lane, -INFINITY, 0.f, pad, lane);
+  const double best = gm ? __shfl(sum, __ffsll((unsigned long long)gm) - 1) : -INFINITY;
 
   // the finished: the best W of those there were (lanes 0 .. W - 1, sorted) and those that end
   // now (lanes W .. 2 W - 1: candidates 0 .. W - 1), of equal ones the lower lane
   const double power = pow((double)(t + 1), alpha);
   const int from = lane >= W ? lane - W : 0;
   const bool took = __shfl((int)(valid && end), from) && lane >= W && lane < 2 * W;
-  const float fresh = (float)((double)__shfl(cs, from) / power);
+  const float fresh = (float)(__shfl(sum, from) / power);
   const int fresh_beam = __shfl(cb, from), fresh_token = (int)__shfl((long long)ct, from);
   const float fs = beam ? fin_score : took ? fresh : -INFINITY;
   const int fl = beam ? fin_length : took ? t + 1 : 0;
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kWave) void beam_advance_kernel(
   const bool full = last && __shfl(fl, max(ll, 0)) > 0;
   if (beam) out.position[gw + lane] = position + 1;
   if (lane == 0) {
-    const float reach = (float)((double)best / power);
+    const float reach = (float)(best / power);
     const bool stop = best == -INFINITY || t + 1 >= T || (full && (early || worst >= reach));
     out.length[g] = t + 1;
     out.done[g] = stop;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(kTraceWaves* kWave) void beam_trace_kernel(
 
 }  // namespace
 
-extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t* done,
+extern "C" int acorn_beam_advance_low(const float* scores, const int32_t* length, const int32_t* done,
                                   const int32_t* position, const float* fin_scores,
                                   const int32_t* fin_length, const int32_t* fin_beam,
                                   const int32_t* fin_token, float* out_scores, int32_t* out_length,
@@ -426,7 +428,8 @@ extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, co
                                   int32_t* out_fin_length, int32_t* out_fin_beam,
                                   int32_t* out_fin_token, int32_t* token_log, int32_t* parent_log,
                                   const float* cand_score, const int32_t* cand_beam,
-                                  const int64_t* cand_token, const int64_t* ends, int64_t groups,
+                                  const int64_t* cand_token, const int64_t* ends,
+                                  const float* cand_low, float* low, int64_t groups,
                                   int64_t beams, int64_t k, int64_t steps, int64_t n_ends,
                                   double length_penalty, int early_stopping, int64_t pad,
                                   void* stream) {
@@ -451,10 +454,31 @@ extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, co
   const BeamFields out = {out_scores, out_length, out_done, out_ids, out_position, out_parents,
                           out_fin_scores, out_fin_length, out_fin_beam, out_fin_token};
   beam_advance_kernel<<<dim3((unsigned)groups), dim3(kWave), 0, (hipStream_t)stream>>>(
-      in, out, token_log, parent_log, cand_score, cand_beam, cand_token, ends, (int)groups,
-      (int)beams, (int)k, (int)steps, (int)n_ends, length_penalty, early_stopping, pad);
+      in, out, token_log, parent_log, cand_score, cand_beam, cand_token, ends, cand_low, low,
+      (int)groups, (int)beams, (int)k, (int)steps, (int)n_ends, length_penalty, early_stopping, pad);
   ACORN_LAUNCH_CHECK();
   return ACORN_OK;
+}
+
+extern "C" int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t* done,
+                                  const int32_t* position, const float* fin_scores,
+                                  const int32_t* fin_length, const int32_t* fin_beam,
+                                  const int32_t* fin_token, float* out_scores, int32_t* out_length,
+                                  int32_t* out_done, int64_t* out_ids, int32_t* out_position,
+                                  int32_t* out_parents, float* out_fin_scores,
+                                  int32_t* out_fin_length, int32_t* out_fin_beam,
+                                  int32_t* out_fin_token, int32_t* token_log, int32_t* parent_log,
+                                  const float* cand_score, const int32_t* cand_beam,
+                                  const int64_t* cand_token, const int64_t* ends, int64_t groups,
+                                  int64_t beams, int64_t k, int64_t steps, int64_t n_ends,
+                                  double length_penalty, int early_stopping, int64_t pad,
+                                  void* stream) {
+  return acorn_beam_advance_low(scores, length, done, position, fin_scores, fin_length, fin_beam,
+                                fin_token, out_scores, out_length, out_done, out_ids, out_position,
+                                out_parents, out_fin_scores, out_fin_length, out_fin_beam,
+                                out_fin_token, token_log, parent_log, cand_score, cand_beam,
+                                cand_token, ends, nullptr, nullptr, groups, beams, k, steps, n_ends,
+                                length_penalty, early_stopping, pad, stream);
 }
 
 extern "C" int acorn_beam_reorder(void* k_pool, void* v_pool, void* scale_pool, int32_t* tables,

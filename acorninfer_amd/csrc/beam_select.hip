@@ -9,7 +9,8 @@
 // row's sum nor the beam's score. beam_join_kernel, one workgroup per group, joins a
 // row's pieces, then the rows, by s in 64 bits: beams are compared through sums over the
 // whole vocabulary, and 32 bits of s (2^-20 at 10) would tie or turn round what the
-// logits tell apart.
+// logits tell apart. A score may come and go in two words of 32 bits (the caller adds up thousands of
+// steps, and each rounding of the sum to 32 bits would be as coarse).
 //
 // A value's key is its order-preserving image in 32 bits, then ~token: keys differ
 // from one another, the larger is the better, and the k largest do not depend on
@@ -23,6 +24,7 @@
 // last ones has nothing beside it. Many rows are bound by VALU work (46 instructions per vector of 8,
 // 9 of them exponentials) beside the loads.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.h"
@@ -470,10 +472,13 @@ __device__ __forceinline__ double ln64(double s) {
 // A wave per row (or two): the sum of its pieces, and its k best out of their lists, sorted; then the
 // rows' lists are merged pair by pair. (Finding every entry's place by halving in the other rows'
 // lists is W^2 log k reads of LDS: as fast for 4 beams, 1 us more for 8, 11 more for 32.)
+// TWO: scores come or go in two words (a branch on the pointers at run time: 0.1 to 0.2 us).
+template <bool TWO>
 __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     const u64* __restrict__ lists, const Piece* __restrict__ pieces,
-    const float* __restrict__ scores, int W, int V, int k, int C, float* __restrict__ out_score,
-    int32_t* __restrict__ out_beam, int64_t* __restrict__ out_token, int32_t* __restrict__ status) {
+    const float* __restrict__ scores, const float* __restrict__ low, int W, int V, int k, int C,
+    float* __restrict__ out_score, float* __restrict__ out_low, int32_t* __restrict__ out_beam,
+    int64_t* __restrict__ out_token, int32_t* __restrict__ status) {
   __shared__ uint32_t tokens[kMaxBeams][kMaxK];
   __shared__ u64 keys[kMaxBeams][kMaxK];                       // s, 0: no entry
   __shared__ u64 reach[kJoinWaves][(kAhead + 1) * kWave];      // of a row's entries, those that may count
@@ -486,7 +491,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     const Piece* pc = pieces + row * C;
     const u64* lp = lists + row * C * k;
     const int total = C * k;
-    const float score = scores[row];
+    double score = (double)scores[row];
+    if (TWO && low) score += (double)low[row];
     // (the first loads together: what they find of a row that was not read is not used)
     const Piece b = pc[min(lane, C - 1)];
     const uint32_t head = (uint32_t)(lp[(int64_t)min(lane, C - 1) * k] >> 32);
@@ -549,7 +555,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
     u64 key = 0;
     if (lane < have)
       // (x - ref first: where logits are of the type's lowest value, their sum would swallow log_sum)
-      key = order64((double)score + (((double)unorder32((uint32_t)(top >> 32)) - ref) - log_sum));
+      key = order64(score + (((double)unorder32((uint32_t)(top >> 32)) - ref) - log_sum));
     if (lane < k) {
       keys[w][lane] = key;
       tokens[w][lane] = token;
@@ -597,7 +603,9 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
   }
   if (wid == 0 && lane < k) {
     const int64_t at = (int64_t)g * k + lane;
-    out_score[at] = (float)unorder64(best.key);
+    const double s = unorder64(best.key);
+    out_score[at] = (float)s;
+    if (TWO && out_low) out_low[at] = fabs(s) <= FLT_MAX ? (float)(s - (double)(float)s) : 0.f;
     out_beam[at] = (int32_t)(best.place / kWave);
     out_token[at] = (int64_t)tokens[best.place / kWave][best.place % kWave];
   }
@@ -656,11 +664,11 @@ extern "C" int acorn_beam_select_workspace(int64_t groups, int64_t beams, int64_
   return ACORN_OK;
 }
 
-extern "C" int acorn_beam_select(const void* logits, int64_t row_stride, const float* scores,
-                                 int64_t groups, int64_t beams, int64_t vocab, int64_t k,
-                                 float* out_score, int32_t* out_beam, int64_t* out_token,
-                                 int32_t* status, void* ws, int64_t ws_bytes, int dtype,
-                                 void* stream) {
+extern "C" int acorn_beam_select_low(const void* logits, int64_t row_stride, const float* scores,
+                                     const float* low, int64_t groups, int64_t beams, int64_t vocab,
+                                     int64_t k, float* out_score, float* out_low, int32_t* out_beam,
+                                     int64_t* out_token, int32_t* status, void* ws,
+                                     int64_t ws_bytes, int dtype, void* stream) {
   int64_t need = 0;
   const int rc = acorn_beam_select_workspace(groups, beams, vocab, k, dtype, &need);
   if (rc != ACORN_OK) return rc;
@@ -680,9 +688,19 @@ extern "C" int acorn_beam_select(const void* logits, int64_t row_stride, const f
   if (dtype == ACORN_BF16) part<__bf16>(logits, row_stride, scores, rows, vocab, k, pc, lists, pieces, st);
   ACORN_LAUNCH_CHECK();
   const unsigned waves = (unsigned)std::min<int64_t>(beams, kJoinWaves);
-  beam_join_kernel<<<dim3((unsigned)groups), dim3(waves * kWave), 0, st>>>(
-      lists, pieces, scores, (int)beams, (int)vocab, (int)k, pc.count, out_score, out_beam,
-      out_token, status);
+  (low || out_low ? beam_join_kernel<true> : beam_join_kernel<false>)<<<dim3((unsigned)groups),
+                                                                      dim3(waves * kWave), 0, st>>>(
+      lists, pieces, scores, low, (int)beams, (int)vocab, (int)k, pc.count, out_score, out_low,
+      out_beam, out_token, status);
   ACORN_LAUNCH_CHECK();
   return ACORN_OK;
+}
+
+extern "C" int acorn_beam_select(const void* logits, int64_t row_stride, const float* scores,
+                                 int64_t groups, int64_t beams, int64_t vocab, int64_t k,
+                                 float* out_score, int32_t* out_beam, int64_t* out_token,
+                                 int32_t* status, void* ws, int64_t ws_bytes, int dtype,
+                                 void* stream) {
+  return acorn_beam_select_low(logits, row_stride, scores, nullptr, groups, beams, vocab, k, out_score,
+                               nullptr, out_beam, out_token, status, ws, ws_bytes, dtype, stream);
 }

@@ -48,6 +48,8 @@ class _Batch:
     slots: SlotMap
     ones: torch.Tensor
     broken: torch.Tensor
+    # scores are sums of thousands of terms: what their 32 bits leave out, of candidates and beams
+    low: tuple[torch.Tensor, torch.Tensor]
     graph: torch.cuda.CUDAGraph | None = None
 
 
@@ -97,13 +99,14 @@ class BeamSearch:
                                   z(B))
             b = _Batch(
                 buf, state, cand, beam_select_workspace(G, W, V, K, buf.logits.dtype, dev),
-                SlotMap(z(B), buf.positions, buf.pages, buf.slots, buf.lens, z(B)), z(B) + 1, z(B))
+                SlotMap(z(B), buf.positions, buf.pages, buf.slots, buf.lens, z(B)), z(B) + 1, z(B),
+                (z(G, K, dtype=torch.float32), z(G, W, dtype=torch.float32)))
         self._batches[G] = b
         return b
 
     def _advance(self, b: _Batch, cand: BeamCandidates) -> None:
         beam_advance(b.state, cand, self.end_ids, length_penalty=self.penalty,
-                     early_stopping=self.early)
+                     early_stopping=self.early, low=b.low)
         self.cache.reorder_beams(b.buf.tables, b.state.position, b.state.parents)
 
     def _body(self, b: _Batch) -> None:
@@ -112,7 +115,8 @@ class BeamSearch:
         slot_map(b.buf.tables, b.state.position.view(B), b.ones, self.page, B, out=b.slots)
         self.model.step(b.buf, c.k_pool, c.v_pool, c.num_blocks, self.page, sample=False,
                         scale_pool=c.scale_pool)
-        beam_select(b.buf.logits, b.state.scores, self.candidates, out=b.cand, workspace=b.ws)
+        beam_select(b.buf.logits, b.state.scores, self.candidates, out=b.cand, workspace=b.ws,
+                    low=b.low[1], out_low=b.low[0])
         torch.maximum(b.broken, b.cand.status, out=b.broken)
         self._advance(b, b.cand)
 
@@ -197,7 +201,7 @@ class BeamSearch:
             ids[i, :len(p)] = torch.tensor(p, dtype=torch.int64)
         logits = self.model.forward_prefill_batch(ids.to(dev), views, real_lens=lens)
         zero = torch.zeros(G, 1, dtype=torch.float32, device=dev)
-        cand = beam_select(logits, zero, self.candidates)
+        cand = beam_select(logits, zero, self.candidates, out_low=b.low[0])
         b.broken[:G] = torch.maximum(b.broken[:G], cand.status)
         self._advance(b, cand)
         for t in range(1, steps):
@@ -219,7 +223,8 @@ class BeamSearch:
                           torch.cat([s.fin_beam, at], 1).contiguous()).tolist()
         if int(b.broken.max()) != 0:
             raise ValueError("logits contain NaN/inf; model forward is broken")
-        length, done, scores = s.length.tolist(), s.done.tolist(), s.scores.tolist()
+        length, done = s.length.tolist(), s.done.tolist()
+        scores = (s.scores.double() + b.low[1].double()).tolist()
         fin = [t.tolist() for t in (s.fin_scores, s.fin_length, s.fin_token)]
         answers = []
         for g in range(G):

@@ -11,7 +11,8 @@ and at the end
 
 `engine.beam.BeamSearch` runs them behind the model's decode step, in one graph.
 They stand beside the sampler (sampler.py) and the paged caches (cache/pager.py),
-with the same block tables. Kernels: csrc/beam_select.hip, csrc/beam.hip. Up to 32
+with the same block tables. A score rounded to 32 bits at every step would drift (by 0.1 in 2000 steps,
+at sums of -15000): `low` operands carry what the rounding leaves out, as BeamSearch does. Kernels: csrc/beam_select.hip, csrc/beam.hip. Up to 32
 beams and 64 candidates. Everything launches on the current stream of its tensors'
 device, never synchronises, and can be captured in a graph; calls that overlap must
 not share outputs or a workspace.
@@ -25,7 +26,7 @@ from typing import NamedTuple
 
 import torch
 
-from acorninfer_amd._lib import check, dtype_code, launch, lib, one_device
+from acorninfer_amd._lib import check, dtype_code, launch, lib, one_device, ptr
 
 MAX_BEAMS = 32
 MAX_CANDIDATES = 64
@@ -117,15 +118,19 @@ def _check(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
-                out: BeamCandidates | None = None, workspace: torch.Tensor | None = None
+                out: BeamCandidates | None = None, workspace: torch.Tensor | None = None,
+                low: torch.Tensor | None = None, out_low: torch.Tensor | None = None
                 ) -> BeamCandidates:
     """The k (at most 64) best continuations of every group by the beam's score plus the token's
-    log-probability, compared in 64 bits; equal ones by beam and then token. logits [G * W, V]
+    log-probability, compared in 64 bits; equal ones by beam and then token. (A row's sum of
+    exponentials is good to 2e-7 as a rule: nearer scores of different beams come in the order of
+    that error.) logits [G * W, V]
     fp32 / fp16 / bf16, rows any distance apart; scores [G, W] fp32. Tokens at -inf are banned; a
     beam of score -inf has only continuations of -inf, which come last (its logits are not read).
     A beam whose score or logits hold NaN or +inf counts as one of score -inf, and its status is
     1. `out` / `workspace` (beam_select_workspace of the same sizes) let a caller pass
-    address-stable buffers."""
+    address-stable buffers. Scores in two words: `low` [G, W] fp32 is added to `scores`, `out_low`
+    [G, k] fp32 gets what rounding the candidates' scores to fp32 left out."""
     assert scores.dim() == 2 and logits.dim() == 2, "scores are [G, W], logits [G * W, V]"
     G, W = scores.shape
     rows, V = logits.shape
@@ -157,9 +162,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *,
         assert workspace.get_device() == dev and workspace.is_contiguous() and \
             workspace.numel() * workspace.element_size() >= need and \
             workspace.data_ptr() % 16 == 0, "workspace: beam_select_workspace of the same sizes"
-    launch("beam_select", dev, logits.data_ptr(), logits.stride(0), scores.data_ptr(), G, W, V, k,
-           out.score.data_ptr(), out.beam.data_ptr(), out.token.data_ptr(), out.status.data_ptr(),
-           workspace.data_ptr(), workspace.numel() * workspace.element_size(), code)
+    if low is None and out_low is None:
+        launch("beam_select", dev, logits.data_ptr(), logits.stride(0), scores.data_ptr(), G, W, V, k,
+               out.score.data_ptr(), out.beam.data_ptr(), out.token.data_ptr(), out.status.data_ptr(),
+               workspace.data_ptr(), workspace.numel() * workspace.element_size(), code)
+        return out
+    for name, t, n in (("low", low, W), ("out_low", out_low, k)):
+        if t is not None:
+            _check(t, name, (G, n), torch.float32)
+            one_device(logits, t)
+    launch("beam_select_low", dev, logits.data_ptr(), logits.stride(0), scores.data_ptr(), ptr(low),
+           G, W, V, k, out.score.data_ptr(), ptr(out_low), out.beam.data_ptr(), out.token.data_ptr(),
+           out.status.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+           code)
     return out
 
 
@@ -194,7 +209,8 @@ def check_length_penalty(alpha: float, steps: int) -> None:
 
 def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Tensor, *,
                  length_penalty: float = 1.0, early_stopping: bool = False, pad: int = 0,
-                 out: BeamState | None = None) -> BeamState:
+                 out: BeamState | None = None,
+                 low: tuple[torch.Tensor, torch.Tensor] | None = None) -> BeamState:
     """One step of the bookkeeping: of a group's candidates (best first, at most 64) the first W
     that do not end (token in end_ids [E] int64) become its beams, row `length` of the logs holds
     their tokens and parents; those among the first W that end join the finished hypotheses, of
@@ -203,8 +219,9 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
     or its best beam's score / length ** length_penalty is no better than the worst of them).
     Groups that are done stay (ids `pad`, every beam its own parent). k = W * (E + 1) candidates
     are always enough for W beams; beams that get none have score -inf. |length_penalty| * ln(steps)
-    is at most 64. Returns `out` (a state of
-    the same sizes; by default `state`, in place), whose logs are written in place."""
+    is at most 64. Returns `out` (a state of the same sizes; by default `state`, in place), whose logs
+    are written in place. Scores in two words, in place only: `low` = (the candidates' low words
+    [G, K], the beams' [G, W], written), fp32."""
     assert state.scores.dim() == 2 and state.token_log.dim() == 3, \
         "scores are [G, W], logs [steps, G, W]"
     G, W = state.scores.shape
@@ -230,10 +247,17 @@ def beam_advance(state: BeamState, candidates: BeamCandidates, end_ids: torch.Te
                                   f"{MAX_CANDIDATES}")
     dev = one_device(*state, score, beam, token, end_ids, *(() if out is state else out))
     s, o = state, out
-    launch("beam_advance", dev, *map(torch.Tensor.data_ptr, (
+    words = ()
+    if low is not None:
+        assert out is state and len(low) == 2, "scores in two words are advanced in place"
+        words = tuple(low)
+        for name, t, n in zip(("low[0]", "low[1]"), words, (K, W)):
+            _check(t, name, (G, n), torch.float32)
+        one_device(score, *words)
+    launch("beam_advance_low" if words else "beam_advance", dev, *map(torch.Tensor.data_ptr, (
         s.scores, s.length, s.done, s.position, s.fin_scores, s.fin_length, s.fin_beam, s.fin_token,
         o.scores, o.length, o.done, o.ids, o.position, o.parents, o.fin_scores, o.fin_length,
-        o.fin_beam, o.fin_token, o.token_log, o.parent_log, score, beam, token, end_ids)),
+        o.fin_beam, o.fin_token, o.token_log, o.parent_log, score, beam, token, end_ids, *words)),
         G, W, K, s.token_log.shape[0], E, alpha, int(bool(early_stopping)), int(pad))
     return out
 

@@ -544,8 +544,9 @@ int acorn_paged_prefill_workspace_kv8(int64_t N, int64_t R, int64_t max_nq, int6
  *
  * acorn_beam_select: the k (1 to 64) best continuations of every group by
  *   s(w, v) = scores[g, w] + x[w, v] - ln sum_u exp(x[w, u]),
- * x [G*W, vocab] rows of `dtype`, row_stride elements apart, compared in 64 bits. In falling
- * order of s, equal ones by beam and then token: out_score [G, k] (s rounded to fp32), out_beam,
+ * x [G*W, vocab] rows of `dtype`, row_stride elements apart. s is compared in 64 bits; its ln sum,
+ * of 32-bit exponentials, is good to 2e-7 as a rule, and nearer scores of different beams come in
+ * the order of that error (those of one beam in the order of x). In falling order of s, equal ones by beam and then token: out_score [G, k] (s rounded to fp32), out_beam,
  * out_token. -inf logits are banned tokens, beams of score -inf have only continuations of -inf
  * and their rows are not read. status [G*W]: 1 for a beam whose score or row holds NaN or +inf
  * (it counts as one of score -inf), else 0. ws: 16-byte aligned, at least the bytes
@@ -556,7 +557,13 @@ int acorn_beam_select(const void* logits, int64_t row_stride, const float* score
                       int64_t beams, int64_t vocab, int64_t k, float* out_score,
                       int32_t* out_beam, int64_t* out_token, int32_t* status, void* ws,
                       int64_t ws_bytes, int dtype, void* stream);
-/* *bytes = workspace of acorn_beam_select. No GPU access. */
+/* The same with scores in two words, scores[g, w] + low[g, w], and out_low [G, k]: what rounding s to
+ * fp32 left out. low (all zeros) and out_low may each be null. */
+int acorn_beam_select_low(const void* logits, int64_t row_stride, const float* scores,
+                          const float* low, int64_t groups, int64_t beams, int64_t vocab, int64_t k,
+                          float* out_score, float* out_low, int32_t* out_beam, int64_t* out_token,
+                          int32_t* status, void* ws, int64_t ws_bytes, int dtype, void* stream);
+/* *bytes = workspace of both. No GPU access. */
 int acorn_beam_select_workspace(int64_t groups, int64_t beams, int64_t vocab, int64_t k, int dtype,
                                 int64_t* bytes);
 
@@ -588,6 +595,21 @@ int acorn_beam_advance(const float* scores, const int32_t* length, const int32_t
                        const int64_t* cand_token, const int64_t* ends, int64_t groups,
                        int64_t beams, int64_t k, int64_t steps, int64_t n_ends,
                        double length_penalty, int early_stopping, int64_t pad, void* stream);
+/* The same with scores in two words: the candidates' are cand_score + cand_low [G, k], the beams' low
+ * words low [G, W] are written (of groups that stay: not). Each may be null. */
+int acorn_beam_advance_low(const float* scores, const int32_t* length, const int32_t* done,
+                           const int32_t* position, const float* fin_scores,
+                           const int32_t* fin_length, const int32_t* fin_beam,
+                           const int32_t* fin_token, float* out_scores, int32_t* out_length,
+                           int32_t* out_done, int64_t* out_ids, int32_t* out_position,
+                           int32_t* out_parents, float* out_fin_scores,
+                           int32_t* out_fin_length, int32_t* out_fin_beam,
+                           int32_t* out_fin_token, int32_t* token_log, int32_t* parent_log,
+                           const float* cand_score, const int32_t* cand_beam,
+                           const int64_t* cand_token, const int64_t* ends, const float* cand_low,
+                           float* low, int64_t groups, int64_t beams, int64_t k, int64_t steps,
+                           int64_t n_ends, double length_penalty, int early_stopping, int64_t pad,
+                           void* stream);
 
 /*
  * The cache follows the beams: beam w of a group continues beam parents[g, w] (outside [0, W):

@@ -21,6 +21,84 @@ def _beam():
     return beam
 
 
+def _ln_sum_bound(vocab):
+    """Of a row in pieces of two vectors a lane, whatever the vocabulary: pieces are added in 64 bits.
+    In 2^-24 of the sum: a power 14 (1 ulp is 2, and its exponent's rounding 2^-24 |t| ln 2 e^t-weighted,
+    |t| < 16), a vector's sum 7, a new maximum 5, the lane's sum 3, its last factor 3, lanes 6 + 6,
+    waves 3 * 6; and the entropy's share."""
+    return 2.0 ** -24 * 62 + LOG2E_OFF * math.log(vocab)
+
+
+# ---- a selection's sum ------------------------------------------------------------------------
+
+
+def _select(x, k, W=1):
+    """(s in 64 bits, beam, token) of beams at score 0."""
+    zero = torch.zeros(x.shape[0] // W, W, device="cuda")
+    low = torch.empty(x.shape[0] // W, k, device="cuda")
+    got = _beam().beam_select(x.cuda(), zero, k, out_low=low)
+    assert int(got.status.max()) == 0
+    return (got.score.double() + low.double()).cpu(), got.beam.cpu().long(), got.token.cpu()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,tail", [(torch.bfloat16, -18.75), (torch.float16, -18.75),
+                                        (torch.float32, -18.0625)])
+def test_what_additions_round_off_is_kept(dtype, tail):
+    """Rows with nearly all of their probability in one token, each of whose others that a lane meets,
+    a vector of them at a time, is less than half a unit in the last place beside it. More than 1024
+    rows, so that a lane's piece is the longest, 19 vectors; the lane differs from row to row."""
+    E = 16 // dtype.itemsize
+    rows, V = 1030, 19 * 256 * E
+    lane = torch.arange(V) // E % 256
+    x = torch.where(lane == torch.arange(rows)[:, None] % 256, tail, -INF)
+    first = torch.arange(rows) % 256 * E + torch.arange(rows) % E
+    x[torch.arange(rows), first] = 0.0
+    s, _, token = _select(x.to(dtype), 1)
+    assert torch.equal(token[:, 0], first)
+    w = math.exp(tail)
+    # what the peak's own vector drops, and the last rounding
+    bound = (E - 1) * w + 2.0 ** -24
+    assert E * w < 2.0 ** -24 and 18 * E * w > 5 * bound    # (lost without the compensation)
+    assert ((s[:, 0] + math.log1p((19 * E - 1) * w)).abs() <= bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("value", [0.0, 1.5, -7.25])
+@pytest.mark.parametrize("rows,V", [(1, 1), (3, 37), (2, 4099), (1, 151936), (300, 20003)])
+def test_the_sum_of_even_rows(dtype, value, rows, V):
+    """Every token's log-probability is -ln V: exactly, but for the entropy's share and ln's 1e-12, where
+    the powers are 1. Else in 2^-24: a power 2, a vector's sum 7, the lane's 3, its last factor 3, lanes
+    6, waves 3."""
+    k = min(V, 5)
+    s, _, token = _select(torch.full((rows, V), value, dtype=dtype), k)
+    assert torch.equal(token, torch.arange(k).expand(rows, k))
+    bound = LOG2E_OFF * math.log(V) + 1e-11 + (0.0 if value == 0 else 2.0 ** -24 * 24)
+    assert ((s + math.log(V)).abs() <= bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,W,k", [(1, 1, 2), (4, 4, 8), (4, 1, 64), (8, 8, 33)])
+@pytest.mark.parametrize("late", [False, True])
+def test_rows_of_many_pieces(dtype, rows, W, k, late):
+    """A vocabulary of 151936 in few rows: 38 pieces in 16 bits, 75 in 32, more than a wave of the
+    join has lanes. late: a row's maximum and its best tokens are in the last ones."""
+    V = 151936
+    g = torch.Generator().manual_seed(rows + k)
+    x = 2.0 * torch.randn(rows, V, generator=g) + torch.randn(rows, 1, generator=g)
+    for _ in range(2 * k):
+        at = torch.randint(140000 if late else 0, V, (rows,), generator=g)
+        x[torch.arange(rows), at] = 8.0 + 6.0 * torch.rand(rows, generator=g)
+    x = x.to(dtype)
+    s, beam, token = _select(x, k, W)
+    want = ref.select_ref(x, torch.zeros(rows // W, W), k)
+    assert torch.equal(beam, want[1]) and torch.equal(token, want[2])
+    assert not late or int(token[:, 0].min()) >= 140000
+    assert ((s - want[0]).abs() <= _ln_sum_bound(V) + 2.0 ** -48 * want[0].abs()).all()
+
+
 # ---- scores in two words ----------------------------------------------------------------------
 
 
@@ -75,9 +153,7 @@ def test_select_of_scores_in_two_words(dtype, V, k):
     fine = want[0] > -INF
     hi, rest = got.score.cpu().double(), out_low.cpu().double()
     assert torch.equal(hi > -INF, fine) and (rest[~fine] == 0).all()
-    # the ln sum as _step_bound, with 8 elements to a vector and |t| < 16: 2^-24 * (14 + 7 + 41); two words
-    # of 24 bits and a sign hold s to 2^-49
-    bound = 2.0 ** -24 * 62 + LOG2E_OFF * math.log(VOCAB) + 2.0 ** -48 * want[0].abs()
+    bound = _ln_sum_bound(V) + 2.0 ** -48 * want[0].abs()    # (two words hold s to 2^-49)
     assert ((hi + rest - want[0]).abs() <= bound)[fine].all()
     assert (rest.abs() <= 2.0 ** -24 * hi.abs())[fine].all()
     assert torch.equal(hi.float(), (hi + rest).float())

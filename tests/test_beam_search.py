@@ -242,3 +242,26 @@ def test_steps_of_many_sizes_and_settings_are_not_all_kept():
            for i in (0, 1, 2, 3, 4, 5, 0)]
     assert got[0] == got[-1] and len(eng._searches) == engine.KEPT_SEARCHES
     eng.assert_balanced()
+
+
+@gpu
+@pytest.mark.parametrize("beams,prompts,steps", [(32, 3, 6), (4, 40, 5), (16, 70, 1)])
+def test_searches_of_more_rows_than_an_engine_decodes(beams, prompts, steps):
+    """96 to 1120 rows to a step, fp32 against the oracle, and all 32 beams."""
+    from acorninfer_amd.models.qwen3 import Qwen3DecodeModel, random_state_dict
+    from oracle.qwen3_ref import Qwen3Ref
+    sd = random_state_dict(TINY, seed=3, std=0.25, dtype=torch.float32)
+    model = Qwen3DecodeModel.from_state_dict(TINY, sd, dtype=torch.float32, device="cuda")
+    oracle = Qwen3Ref(TINY, sd, torch.float32)
+    g = torch.Generator().manual_seed(6)
+    rows = [torch.randint(0, 256, (5 + i % 29,), generator=g).tolist() for i in range(prompts)]
+    search, alloc = _search(model, 3000, beams=beams, max_tokens=6, max_model_len=64, eos_ids={1})
+    got = search.search(rows, max_tokens=steps)
+    alloc.assert_balanced()
+    assert len(got) == prompts
+    for i in (0, prompts // 2, prompts - 1):
+        def logits_of(toks):
+            return oracle.forward(torch.tensor([rows[i] + list(toks)]), oracle.new_cache())[0, -1]
+        want = search_ref(logits_of, beams, steps, {1})
+        assert [tuple(h.tokens) for h in got[i]] == [w[1] for w in want]
+        assert all(abs(h.score - w[0]) < 2.0 ** -12 for h, w in zip(got[i], want))

@@ -239,7 +239,8 @@ __global__ __launch_bounds__(kCopyNT) void beam_copy_kernel(
 
 // A thread per column, which reads the group's entries of it before it writes them; the wave that has
 // the column with the partly filled pages works the plan out. A launch of its own, as every workgroup
-// of the copy reads the pages that it replaces: 2.4 us for 1 group, 3.5 for 16 behind their copies.
+// of the copy reads the pages that it replaces: 2.4 us for 1 group, 4.0 for 16 behind their copies
+// (under the profiler; 3 of 14.0 in a graph).
 constexpr int kTableNT = 256, kTableUnroll = 8;
 
 __global__ __launch_bounds__(kTableNT) void beam_tables_kernel(int32_t* tables, const int32_t* lens,

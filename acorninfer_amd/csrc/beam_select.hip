@@ -9,20 +9,20 @@
 // row's sum nor the beam's score. beam_join_kernel, one workgroup per group, joins a
 // row's pieces, then the rows, by s in 64 bits: beams are compared through sums over the
 // whole vocabulary, and 32 bits of s (2^-20 at 10) would tie or turn round what the
-// logits tell apart. A score may come and go in two words of 32 bits (the caller adds up thousands of
-// steps, and each rounding of the sum to 32 bits would be as coarse).
+// logits tell apart. A score may come and go in two words of 32 bits: a search adds up
+// thousands of steps, and a sum rounded to 32 bits at each of them would be as coarse.
 //
 // A value's key is its order-preserving image in 32 bits, then ~token: keys differ
 // from one another, the larger is the better, and the k largest do not depend on
 // the order they are met in. Tokens at -inf are no candidates here: the join puts
 // them behind the others where a row has too few.
 //
-// Rows of 151936 in bf16, from a graph: 1 row 7.6 us, 4 rows 8.4, 64 rows 13.2, 256 rows 23.4 (78 MB:
-// 3.3 TB/s), 1024 rows 71 (4.4 TB/s). Few rows are latency: two launches, each with a chain of
-// loads, a sort and a join. Of 256 rows' pieces, 19 us, the workgroups have their loads after 6 to
-// 15.5 us, and each takes 3 more: threshold 0.7, queue 1.1, look 0.4, sort and write 0.9; that of the
-// last ones has nothing beside it. Many rows are bound by VALU work (46 instructions per vector of 8,
-// 9 of them exponentials) beside the loads.
+// Rows of 151936 in bf16, from a graph: 1 row 7.8 us (k 2), 4 rows 8.4 (4 beams, k 8), 64 rows 13.4, 256
+// rows 22.3 (8 beams, k 16: 23.5; 78 MB, 3.3 TB/s), 1024 rows 65 (4.8 TB/s). Few rows are latency: two
+// launches, each with a chain of loads, a sort and a join. Of 256 rows' pieces, 19 us, the workgroups
+// have their loads after 6 to 15.5 us, and each takes 3 more: threshold 0.7, queue 1.1, look 0.4, sort
+// and write 0.9; that of the last ones has nothing beside it. Many rows are bound by VALU work (46
+// instructions per vector of 8, 9 of them exponentials) beside the loads.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -611,11 +611,16 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void beam_join_kernel(
   }
 }
 
-// Vectors of a lane and pieces of a row: the shortest pieces with which a batch has no more
-// workgroups than the chip has places for them (four to a CU), so that it runs in one round, each
-// with one sort. 16 / 32 / 128 / 256 rows of 151936, 4 beams: 9.9 / 10.6 / 16.3 / 21.9 us; with up to
-// 512 workgroups 9.3 / 10.5 / 16.7 / 22.1, with up to 2048 9.8 / 11.8 / 16.6 / 22.6. 19 vectors is
-// the most that 128 registers hold beside their maxima (20 spill: 1 us more for 256 rows).
+// Vectors of a lane and pieces of a row: the shortest pieces with which a batch has at most 1024
+// workgroups, as many as the chip has places for (four to a CU), so that it runs in one round, each with
+// one sort; the longest where none gives so few. Rows of 151936 in bf16, 4 beams, k 8, us with 2 / 5 /
+// 10 / 19 vectors: 16 rows 10.0 / 9.3 / 10.8 / 11.8, 32 11.9 / 10.5 / 11.1 / 12.2, 64 15.9 / 13.3 / 13.4 /
+// 14.3, 128 22.5 / 17.0 / 16.8 / 16.9, 256 35.6 / 23.7 / 22.8 / 22.5, 1024 126 / 75 / 66 / 64. 19 vectors
+// is the most that 128 registers hold beside their maxima (20 spill: 1 us more for 256 rows).
+// The rule does not count a piece's vectors behind the row's end, which are worked off like the others.
+// Past 1024 rows of a short vocabulary most of the longest piece is such: 2048 rows of 500 17.2 / 19.6 /
+// 24.2 / 31.3, of 3000 17.8 / 19.7 / 24.0 / 31.2, of 8000 23.8 / 20.4 / 24.6 / 31.8; 1025 rows of 8000
+// 25.1 / 22.3 / 25.3 / 30.2 (1024, which take 5: 19.9); 512 rows of 50257 28.4 / 20.2 / 20.1 / 22.2.
 struct Pieces {
   int count, nv;
 };

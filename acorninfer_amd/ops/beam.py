@@ -11,8 +11,9 @@ and at the end
 
 `engine.beam.BeamSearch` runs them behind the model's decode step, in one graph.
 They stand beside the sampler (sampler.py) and the paged caches (cache/pager.py),
-with the same block tables. A score rounded to 32 bits at every step would drift (by 0.1 in 2000 steps,
-at sums of -15000): `low` operands carry what the rounding leaves out, as BeamSearch does. Kernels: csrc/beam_select.hip, csrc/beam.hip. Up to 32
+with the same block tables. Scores that are rounded to 32 bits at every step drift (by
+0.1 in 2000 steps at sums of -15000): `low` operands carry what the rounding leaves out,
+as BeamSearch does. Kernels: csrc/beam_select.hip, csrc/beam.hip. Up to 32
 beams and 64 candidates. Everything launches on the current stream of its tensors'
 device, never synchronises, and can be captured in a graph; calls that overlap must
 not share outputs or a workspace.
